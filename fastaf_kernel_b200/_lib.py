@@ -29,11 +29,15 @@ GDN_PREFILL_TCGEN05 = 3
 
 GDN_FLAG_QK_L2NORM = 1
 
+GDN_ACTIVATION_NONE = 0
+GDN_ACTIVATION_SILU = 1
+
 # Every symbol include/gdn_b200.h declares.
 EXPORTED_SYMBOLS = ("gdn_prefill", "gdn_prefill_ex", "gdn_prefill_ws", "gdn_prefill_workspace_size",
                     "gdn_prefill_resolve", "gdn_prefill_tc_launches", "gdn_prefill_noalloc", "gdn_prefill_flags",
                     "gdn_prefill_gated", "gdn_prefill_strided", "gdn_decode_strided",
-                    "gdn_decode", "gdn_decode_flags", "gdn_output_gate", "gdn_device_status",
+                    "gdn_decode", "gdn_decode_flags", "gdn_output_gate", "gdn_conv_prefill",
+                    "gdn_conv_decode", "gdn_ssm_prefill", "gdn_ssm_resolve", "gdn_ssm_decode", "gdn_device_status",
                     "gdn_set_wait_limit_ns", "gdn_last_error", "gdn_version")
 
 _lock = threading.Lock()
@@ -100,6 +104,17 @@ def load() -> ctypes.CDLL:
         lib.gdn_prefill_gated.restype = i32
         lib.gdn_output_gate.argtypes = [vp, vp, vp, i32, i64, i32, f32, vp]
         lib.gdn_output_gate.restype = i32
+        lib.gdn_conv_prefill.argtypes = [vp, i64, vp, vp, i32, vp, vp, i64, i64, i64, i32, i32, vp, vp, i32, vp, vp]
+        lib.gdn_conv_prefill.restype = i32
+        lib.gdn_conv_decode.argtypes = [vp, i64, vp, vp, i32, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp]
+        lib.gdn_conv_decode.restype = i32
+        ssm_rows = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, vp, i64, vp]
+        lib.gdn_ssm_prefill.argtypes = ssm_rows + [vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp]
+        lib.gdn_ssm_prefill.restype = i32
+        lib.gdn_ssm_resolve.argtypes = [i64, i64, i32]
+        lib.gdn_ssm_resolve.restype = i32
+        lib.gdn_ssm_decode.argtypes = ssm_rows + [i64, i32, i32, i32, i32, i32, i32, vp, vp, vp]
+        lib.gdn_ssm_decode.restype = i32
         lib.gdn_device_status.argtypes = [vp]
         lib.gdn_device_status.restype = i32
         lib.gdn_set_wait_limit_ns.argtypes = [ctypes.c_uint64]

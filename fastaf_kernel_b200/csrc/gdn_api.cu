@@ -61,6 +61,10 @@ int cuda_status(cudaError_t e, const char *what) {
     return fail(GDN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+}  // namespace
+
+namespace gdn {
+
 // Stream-ordered workspace for callers that pass none: a library-owned memory pool
 // per device whose release threshold keeps its memory between calls, so a
 // steady-state call takes its workspace from the pool without a driver allocation.
@@ -94,9 +98,6 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream) {
     return cudaMallocFromPoolAsync(ptr, bytes, pool, stream);
 }
 
-}  // namespace
-
-namespace gdn {
 void set_last_error(const char *msg) { std::snprintf(g_last_error, sizeof(g_last_error), "%s", msg); }
 }  // namespace gdn
 
@@ -198,7 +199,7 @@ static int prefill_tc_call(const gdn::PrefillArgs &p, void *workspace, size_t wo
     }
     // The pool block also holds the sequences' launch order (need is a multiple of 256 bytes).
     void *ws = nullptr;
-    cudaError_t e = pool_alloc(&ws, need + static_cast<size_t>(p.num_seqs) * sizeof(int32_t), s);
+    cudaError_t e = gdn::pool_alloc(&ws, need + static_cast<size_t>(p.num_seqs) * sizeof(int32_t), s);
     if (e != cudaSuccess) return cuda_status(e, "gdn_prefill (tcgen05) workspace");
     e = gdn::launch_prefill_tc(p, ws, s, /*overlap=*/true,
                                reinterpret_cast<int32_t *>(static_cast<char *>(ws) + need));
@@ -265,7 +266,7 @@ static int prefill_impl(const void *q, const void *k, const void *v, const float
                                 new_state, method, workspace, workspace_bytes, stream, 0, out_gate, norm_w,
                                 norm_w_dtype, norm_eps, a_stride, b_stride);
         void *qk = nullptr;
-        cudaError_t e = pool_alloc(&qk, 2 * qk_bytes, s);
+        cudaError_t e = gdn::pool_alloc(&qk, 2 * qk_bytes, s);
         if (e != cudaSuccess) return cuda_status(e, "gdn_prefill (qk l2norm) scratch");
         void *qn = qk, *kn = static_cast<char *>(qk) + qk_bytes;
         e = gdn::launch_qk_l2norm(q, k, total_tokens * num_qk_heads, qn, kn, s);

@@ -1,0 +1,272 @@
+// gdn_conv.cu -- the short depthwise causal convolution in front of a linear-attention
+// layer's recurrence (not part of the reference, which starts at q, k and v):
+//
+//   y[t][c] = act(bias[c] + sum_{w < W} weight[c][w] * x[t - (W-1) + w][c]),   W = 2, 3, 4,
+//
+// per packed sequence, where the W-1 rows in front of its first token are its state (zero
+// without one), act is the identity or silu(y) = y / (1 + exp(-y)), and the new state is
+// the last W-1 rows of [state; x].  fp32 arithmetic from bf16 rows, one rounding of y.
+//
+// Both kernels are HBM-bound (4 bytes a token and channel against 2 W flops and one silu).
+// A thread owns 8 channels (one 16-byte word of a row) and a run of consecutive tokens, so
+// the window slides through its registers: every row is read from HBM once, plus W-1 rows
+// of overlap per run that mostly hit in L2.
+#include "gdn_common.cuh"
+#include "gdn_launch.h"
+
+namespace gdn {
+
+namespace {
+
+constexpr int kVec = 8;            // channels of a thread
+constexpr int kConvThreads = 128;
+constexpr int kBatchRows = 4;      // rows a thread has in flight
+
+// silu from the hardware exponential and division (a few units of 2^-22 relative, far below
+// the bf16 rounding of the result); -> 0 for large negative y.
+__device__ __forceinline__ float silu_fast(float y) { return __fdividef(y, 1.0f + __expf(-y)); }
+
+struct Row {                       // 8 channels as packed fp32 pairs
+    uint64_t v[4];
+};
+
+__device__ __forceinline__ Row unpack_row(uint4 w) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    Row r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[e] = f2(bf16_lo(u[e]), bf16_hi(u[e]));
+    return r;
+}
+
+__device__ __forceinline__ uint4 load_row(const __nv_bfloat16 *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
+
+// The 8 channels' weights, tap by tap, and bias.
+template <int W>
+struct Taps {
+    Row w[W], b;
+    __device__ __forceinline__ void load(const ConvArgs &p, int64_t c) {
+        float t[kVec * W];
+#pragma unroll
+        for (int i = 0; i < kVec * W; ++i) t[i] = load_scalar(p.weight, c * W + i, p.weight_dtype);
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[k].v[e] = f2(t[(2 * e) * W + k], t[(2 * e + 1) * W + k]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            b.v[e] = p.bias ? f2(load_scalar(p.bias, c + 2 * e, p.weight_dtype), load_scalar(p.bias, c + 2 * e + 1, p.weight_dtype))
+                            : f2(0.0f, 0.0f);
+    }
+};
+
+// One output row's 8 channels from the window (win[0] oldest) and the current row.
+template <int W>
+__device__ __forceinline__ uint4 conv_row(const Taps<W> &k, const Row (&win)[W - 1], const Row &x, bool silu) {
+    uint32_t r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint64_t acc = k.b.v[e];
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) acc = fma_f2(k.w[i].v[e], win[i].v[e], acc);
+        acc = fma_f2(k.w[W - 1].v[e], x.v[e], acc);
+        float y0, y1;
+        unf2(acc, y0, y1);
+        if (silu) {
+            y0 = silu_fast(y0);
+            y1 = silu_fast(y1);
+        }
+        r[e] = pack_bf16x2(y0, y1);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Where channel c goes: the output tensor that holds it, as a pointer to its first row and
+// the row's width.
+__device__ __forceinline__ __nv_bfloat16 *out_of(const ConvArgs &p, int64_t c, int64_t &width) {
+    int64_t first = 0;
+#pragma unroll
+    for (int j = 0; j < kConvMaxOutputs - 1; ++j) {
+        if (j + 1 >= p.num_outputs || c < first + p.out_width[j]) {
+            width = p.out_width[j];
+            return static_cast<__nv_bfloat16 *>(p.out[j]) + (c - first);
+        }
+        first += p.out_width[j];
+    }
+    width = p.out_width[kConvMaxOutputs - 1];
+    return static_cast<__nv_bfloat16 *>(p.out[kConvMaxOutputs - 1]) + (c - first);
+}
+
+template <int W>
+__global__ void __launch_bounds__(kConvThreads)
+conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * kConvThreads + threadIdx.x;
+    const int64_t groups = p.channels / kVec;
+    const int64_t tile = id / groups, c = (id - tile * groups) * kVec;
+    const auto *x = static_cast<const __nv_bfloat16 *>(p.x) + c;
+    const auto *state = p.state ? static_cast<const __nv_bfloat16 *>(p.state) + c : nullptr;
+    const int64_t T = p.rows, N = p.num_seqs, C = p.channels;
+    const int32_t *cu = p.cu_seqlens;
+    if (tile >= runs) {
+        // The new state of sequence n: rows [len, len + W - 1) of [state; x].
+        const int64_t n = tile - runs;
+        if (n >= N) return;
+        if (c == 0) check_seq_bounds(cu, n, N, T, p.status);
+        int64_t s0 = cu[n], s1 = cu[n + 1];
+        s0 = s0 < 0 ? 0 : (s0 > T ? T : s0);
+        s1 = s1 < s0 ? s0 : (s1 > T ? T : s1);
+        auto *dst = static_cast<__nv_bfloat16 *>(p.new_state) + n * (W - 1) * C + c;
+#pragma unroll
+        for (int r = 0; r < W - 1; ++r) {
+            const int64_t e = s1 - s0 + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (e >= W - 1) v = load_row(x + (s0 + e - (W - 1)) * p.x_stride);
+            else if (state) v = load_row(state + (n * (W - 1) + e) * C);
+            *reinterpret_cast<uint4 *>(dst + r * C) = v;
+        }
+        return;
+    }
+    const int64_t t0 = tile * run;
+    const int64_t t1 = t0 + run < T ? t0 + run : T;
+    uint4 raw[kBatchRows];
+#pragma unroll
+    for (int u = 0; u < kBatchRows; ++u)
+        raw[u] = t0 + u < t1 ? load_row(x + (t0 + u) * p.x_stride) : make_uint4(0, 0, 0, 0);
+    Taps<W> taps;
+    taps.load(p, c);
+    int64_t width;
+    __nv_bfloat16 *out = out_of(p, c, width);
+    // The sequence of token t0: the last one that starts at or before it.
+    int64_t lo = 0, hi = N - 1;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) >> 1;
+        if (cu[mid] <= t0) lo = mid;
+        else hi = mid - 1;
+    }
+    int64_t n = lo;
+    int64_t s0 = cu[n];
+    s0 = s0 < 0 ? 0 : (s0 > t0 ? t0 : s0);
+    int64_t next = cu[n + 1];
+    // row `back` rows in front of token t of sequence n that starts at s0
+    auto before = [&](int64_t t, int back) -> Row {
+        const int64_t at = t - back - s0;
+        if (at >= 0) return unpack_row(load_row(x + (t - back) * p.x_stride));
+        if (state) return unpack_row(load_row(state + (n * (W - 1) + (W - 1) + at) * C));
+        return unpack_row(make_uint4(0, 0, 0, 0));
+    };
+    Row win[W - 1];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) win[i] = before(t0, W - 1 - i);
+    for (int64_t t = t0; t < t1; t += kBatchRows) {
+        uint4 nxt[kBatchRows];
+#pragma unroll
+        for (int u = 0; u < kBatchRows; ++u)
+            nxt[u] = t + kBatchRows + u < t1 ? load_row(x + (t + kBatchRows + u) * p.x_stride) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < kBatchRows; ++u) {
+            const int64_t tt = t + u;
+            if (tt < t1) {
+                if (tt >= next && n + 1 < N) {     // the next sequence that has tokens starts here
+                    do {
+                        ++n;
+                        next = cu[n + 1];
+                    } while (tt >= next && n + 1 < N);
+                    s0 = tt;
+#pragma unroll
+                    for (int i = 0; i < W - 1; ++i) win[i] = before(tt, W - 1 - i);
+                }
+                const Row cur = unpack_row(raw[u]);
+                *reinterpret_cast<uint4 *>(out + tt * width) = conv_row<W>(taps, win, cur, p.silu);
+#pragma unroll
+                for (int i = 0; i + 1 < W - 1; ++i) win[i] = win[i + 1];
+                win[W - 2] = cur;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatchRows; ++u) raw[u] = nxt[u];
+    }
+}
+
+// One token of each sequence; new_state may be state (a thread reads its own words of all
+// rows before it writes any).
+template <int W>
+__global__ void __launch_bounds__(kConvThreads)
+conv_decode_kernel(const ConvArgs p, int run, int64_t runs) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * kConvThreads + threadIdx.x;
+    const int64_t groups = p.channels / kVec, C = p.channels;
+    const int64_t tile = id / groups, c = (id - tile * groups) * kVec;
+    if (tile >= runs) return;
+    const auto *x = static_cast<const __nv_bfloat16 *>(p.x) + c;
+    const auto *state = static_cast<const __nv_bfloat16 *>(p.state);
+    auto *new_state = static_cast<__nv_bfloat16 *>(p.new_state);
+    Taps<W> taps;
+    taps.load(p, c);
+    int64_t width;
+    __nv_bfloat16 *out = out_of(p, c, width);
+    const int64_t b1 = (tile + 1) * run < p.rows ? (tile + 1) * run : p.rows;
+    for (int64_t b = tile * run; b < b1; ++b) {
+        uint4 raw[W];
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i)
+            raw[i] = state ? *reinterpret_cast<const uint4 *>(state + (b * (W - 1) + i) * C + c) : make_uint4(0, 0, 0, 0);
+        raw[W - 1] = load_row(x + b * p.x_stride);
+        Row win[W - 1];
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) win[i] = unpack_row(raw[i]);
+        *reinterpret_cast<uint4 *>(out + b * width) = conv_row<W>(taps, win, unpack_row(raw[W - 1]), p.silu);
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i)
+            *reinterpret_cast<uint4 *>(new_state + (b * (W - 1) + i) * C + c) = raw[i + 1];
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    return sms;
+}
+
+// Rows per thread: the longest run (less overlap, the weights read less often) that still
+// gives every SM `want` threads.
+int pick_run(int64_t rows, int64_t groups, int longest, int shortest) {
+    const int64_t want = static_cast<int64_t>(sm_count()) * 1024;
+    int run = longest;
+    while (run > shortest && ((rows + run - 1) / run) * groups < want) run /= 2;
+    return run;
+}
+
+template <typename F>
+cudaError_t launch_flat(F kernel, const ConvArgs &p, int run, int64_t runs, int64_t tiles, cudaStream_t stream) {
+    const int64_t threads = tiles * (p.channels / kVec);
+    const int64_t blocks = (threads + kConvThreads - 1) / kConvThreads;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    kernel<<<static_cast<unsigned>(blocks), kConvThreads, 0, stream>>>(p, run, runs);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_conv_prefill(const ConvArgs &p, cudaStream_t stream) {
+    const int run = pick_run(p.rows, p.channels / kVec, 32, kBatchRows);
+    const int64_t runs = (p.rows + run - 1) / run, tiles = runs + p.num_seqs;
+    switch (p.width) {
+        case 2: return launch_flat(conv_prefill_kernel<2>, p, run, runs, tiles, stream);
+        case 3: return launch_flat(conv_prefill_kernel<3>, p, run, runs, tiles, stream);
+        default: return launch_flat(conv_prefill_kernel<4>, p, run, runs, tiles, stream);
+    }
+}
+
+cudaError_t launch_conv_decode(const ConvArgs &p, cudaStream_t stream) {
+    const int run = pick_run(p.rows, p.channels / kVec, 4, 1);
+    const int64_t runs = (p.rows + run - 1) / run;
+    switch (p.width) {
+        case 2: return launch_flat(conv_decode_kernel<2>, p, run, runs, runs, stream);
+        case 3: return launch_flat(conv_decode_kernel<3>, p, run, runs, runs, stream);
+        default: return launch_flat(conv_decode_kernel<4>, p, run, runs, runs, stream);
+    }
+}
+
+}  // namespace gdn

@@ -49,8 +49,59 @@ struct PrefillArgs {
     int64_t a_stride = 0, b_stride = 0;
 };
 
+// The short causal convolution (gdn_conv.cu): prefill over packed sequences, or decode of
+// one row per sequence.
+constexpr int kConvMaxOutputs = 4;
+struct ConvArgs {
+    const void *x;               // bf16 rows of `channels`, x_stride elements apart
+    int64_t x_stride;
+    const void *weight, *bias;   // [channels][width], [channels] or nullptr (weight_dtype)
+    int weight_dtype;
+    const void *state;           // bf16 [num_seqs][width - 1][channels] or nullptr (zero)
+    const int32_t *cu_seqlens;   // [num_seqs + 1], device (prefill only)
+    int64_t num_seqs, rows;      // rows: tokens (prefill) or sequences (decode)
+    int64_t channels;            // a multiple of 8
+    int width;                   // 2, 3 or 4
+    int silu;
+    int num_outputs;             // packed outputs [rows][out_width[j]], side by side in the channels
+    void *out[kConvMaxOutputs];
+    int64_t out_width[kConvMaxOutputs];
+    void *new_state;             // decode: may be state
+    int *status = nullptr;       // as PrefillArgs::status
+};
+
+// The selective scan with one decay per head (gdn_ssm.cu, gdn_ssm_tc.cu).  Strides are in
+// elements between the rows of consecutive tokens (sequences for decode).
+struct SsmArgs {
+    const void *x;               // bf16 rows [heads][head_size]
+    int64_t x_stride;
+    const void *dt;              // rows [heads] (dt_dtype)
+    int64_t dt_stride;
+    const void *B, *C;           // bf16 rows [groups][128]
+    int64_t B_stride, C_stride;
+    const void *z;               // bf16 rows [heads][head_size] or nullptr (no output gate)
+    int64_t z_stride;
+    const void *A_log, *D, *dt_bias;   // [heads] (param_dtype); D, dt_bias may be nullptr (zero)
+    int dt_dtype, param_dtype;
+    const float *state;          // fp32 [num_seqs][heads][head_size][128] or nullptr (zero)
+    const int32_t *cu_seqlens;   // prefill only
+    int64_t num_seqs, rows;      // rows: tokens (prefill) or sequences (decode)
+    int heads, groups, head_size;
+    void *out;                   // bf16 [rows][heads][head_size]
+    float *new_state;            // decode: may be state
+    int *status = nullptr;       // as PrefillArgs::status
+};
+
 // Set the message gdn_last_error() returns on this thread.
 void set_last_error(const char *msg);
+
+// Stream-ordered device memory from the library's pool (see gdn_api.cu).
+cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream);
+
+cudaError_t launch_conv_prefill(const ConvArgs &p, cudaStream_t stream);
+cudaError_t launch_conv_decode(const ConvArgs &p, cudaStream_t stream);
+cudaError_t launch_ssm_decode(const SsmArgs &p, cudaStream_t stream);
+cudaError_t launch_ssm_prefill_recurrent(const SsmArgs &p, cudaStream_t stream);
 
 cudaError_t launch_decode(const DecodeArgs &p, cudaStream_t stream);
 // o <- bf16(o / sqrt(mean(o^2) + eps) * w * silu(z)) per 128-element vector, in place.

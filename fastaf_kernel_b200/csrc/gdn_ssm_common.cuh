@@ -1,0 +1,27 @@
+// gdn_ssm_common.cuh -- what the selective scan kernels share.
+//
+//   dt' = softplus(dt + dt_bias),  a = -exp(A_log) dt'          (per token and head)
+//   S_t = exp(a_t) S_{t-1} + dt'_t x_t B_t^T,   y_t = S_t C_t + D x_t,   [y_t <- y_t silu(z_t)]
+//
+// with S [head_size][128] fp32 per head (k-last), x, z [head_size] per head and B, C [128]
+// shared by the heads / groups consecutive heads of a group.
+#pragma once
+
+#include "gdn_common.cuh"
+#include "gdn_launch.h"
+
+namespace gdn {
+
+constexpr int kSsmState = 128;   // the only state size the kernels are built for
+
+// dt' of one token and head, in fp32.
+__device__ __forceinline__ float ssm_step(const SsmArgs &p, int64_t row, int h) {
+    float v = load_scalar(p.dt, row * p.dt_stride + h, p.dt_dtype);
+    if (p.dt_bias) v += load_scalar(p.dt_bias, h, p.param_dtype);
+    return softplus_torch(v);
+}
+
+// silu from the hardware exponential and division (a few units of 2^-22 relative).
+__device__ __forceinline__ float ssm_silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
+
+}  // namespace gdn

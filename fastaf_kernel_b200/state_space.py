@@ -1,0 +1,330 @@
+"""State space layers beside Gated DeltaNet ones: the short causal convolution in front of
+either layer's recurrence, and the selective scan with one decay per head, for prompts and
+for single tokens.
+
+The manner is that of ``kernel`` and ``kernel_decode``: packed varlen prompts with
+``cu_seqlens``, bf16 rows, gate inputs and parameters in fp32 or bf16, an fp32 k-last state,
+value-returning calls with keyword-only ``output=`` / ``new_state=`` destinations, on the
+current torch CUDA stream of the inputs' device, with no CPU path.  Rows may be slices of a
+wider projection output: they are read through their row stride, without a copy.
+
+The reference has neither operator; its entry points start at q, k and v.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .api import _GATE_DTYPES, _check_cu_seqlens_host, _gate, _on_device, _ptr
+
+__all__ = ["conv_prefill", "conv_decode", "ssm_prefill", "ssm_decode", "ssm_method"]
+
+_ACTIVATIONS = {None: _lib.GDN_ACTIVATION_NONE, "silu": _lib.GDN_ACTIVATION_SILU}
+_METHODS = {"auto": _lib.GDN_PREFILL_AUTO, "recurrent": _lib.GDN_PREFILL_RECURRENT,
+            "tcgen05": _lib.GDN_PREFILL_TCGEN05}
+_MAX_OUTPUTS = 4
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+Outputs = Union[torch.Tensor, Tuple[torch.Tensor, ...]]
+
+
+def _on(device: torch.device, named) -> None:
+    """Every given tensor is a CUDA tensor on ``device``."""
+    for name, t in named:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got {t.device}")
+        if t.get_device() != device.index:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _rows(name: str, t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+    """bf16 rows of ``width`` elements (the last dimensions of ``t``, packed among
+    themselves) as the kernels read them: the tensor and its row stride in elements.  Rows
+    that do not start on a 16-byte boundary or are not packed become a packed copy."""
+    if t.dtype != _BF16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.is_contiguous():
+        # (a contiguous slice may still start off a 16-byte boundary)
+        return (t if t.data_ptr() % 16 == 0 else t.clone()), width
+    rows, shape, strides = t.shape[0], t.shape[1:], t.stride()
+    step, packed = 1, True
+    for n, st in zip(reversed(shape), reversed(strides[1:])):
+        packed = packed and (n == 1 or st == step)
+        step *= n
+    stride = strides[0] if rows > 1 else width
+    if packed and stride >= width and stride % 8 == 0 and stride < 1 << 31 and t.data_ptr() % 16 == 0:
+        return t, stride
+    return t.contiguous(), width
+
+
+def _dt_rows(t: torch.Tensor, heads: int) -> Tuple[torch.Tensor, int]:
+    """dt as the kernels read it: fp32 or bf16 rows of ``heads`` elements and their stride."""
+    if t.dtype not in _GATE_DTYPES:
+        t = t.float()
+    if t.is_contiguous():
+        return t, heads
+    if t.stride(-1) == 1 or heads == 1:
+        stride = t.stride(0) if t.shape[0] > 1 else heads
+        if heads <= stride < 1 << 31:
+            return t, stride
+    return t.contiguous(), heads
+
+
+def _destination(name: str, t: Optional[torch.Tensor], shape, dtype, device) -> torch.Tensor:
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    return t
+
+
+def _state(state: Optional[torch.Tensor], new_state: Optional[torch.Tensor], shape, dtype):
+    """The state as the kernels read it.  A state that is also the destination has to be
+    readable as it is: a converted copy would leave it half old."""
+    if state is None:
+        return None
+    if tuple(state.shape) != tuple(shape):
+        raise ValueError(f"state must have shape {tuple(shape)}, got {tuple(state.shape)}")
+    if state.dtype == dtype and state.is_contiguous() and state.data_ptr() % 16 == 0:
+        return state
+    if new_state is not None and new_state.data_ptr() == state.data_ptr():
+        raise ValueError(f"an in-place state must be a contiguous, 16-byte aligned {dtype} tensor")
+    return state.to(dtype).contiguous().clone()
+
+
+def _cu(cu_seqlens: torch.Tensor, T: int, device: torch.device, validate: bool) -> Tuple[torch.Tensor, int]:
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be a 1-D tensor of at least one entry")
+    if cu_seqlens.is_cuda:
+        if cu_seqlens.get_device() != device.index:
+            raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, expected {device}")
+    elif validate:
+        _check_cu_seqlens_host(cu_seqlens.detach().to(torch.int64), T)
+    if cu_seqlens.shape[0] == 1 and T:
+        raise ValueError("cu_seqlens names no sequence but there are tokens")
+    if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_cuda or not cu_seqlens.is_contiguous():
+        cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+    return cu_seqlens, cu_seqlens.shape[0] - 1
+
+
+# ------------------------------------------------------------------------ the convolution
+
+def _conv(x, weight, bias, state, num_seqs, activation, split, output, new_state):
+    """The checks and conversions of both convolution calls: the C call's arguments (without
+    cu_seqlens and sizes that only prefill has), the outputs and the new state."""
+    device = x.device
+    if x.dim() != 2:
+        raise ValueError("x must be [rows, channels]")
+    T, C = x.shape
+    if weight.dim() != 2 or weight.shape[0] != C:
+        raise ValueError(f"weight must be [channels, width] = [{C}, width], got {tuple(weight.shape)}")
+    W = weight.shape[1]
+    if W < 2 or W > 4:
+        raise NotImplementedError(f"width={W} is not supported (2, 3 or 4)")
+    if C == 0 or C % 8:
+        raise ValueError(f"channels={C} must be a positive multiple of 8")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be None or 'silu'")
+    if bias is not None and tuple(bias.shape) != (C,):
+        raise ValueError(f"bias must be [{C}]")
+    weight = _gate(weight)
+    if bias is not None:
+        bias = _gate(bias)
+        if bias.dtype != weight.dtype:
+            weight, bias = weight.float(), bias.float()
+    x, stride = _rows("x", x, C)
+    widths: Sequence[int] = (C,) if split is None else tuple(int(n) for n in split)
+    if not 1 <= len(widths) <= _MAX_OUTPUTS or any(n <= 0 or n % 8 for n in widths) or sum(widths) != C:
+        raise ValueError(f"split must be 1 to {_MAX_OUTPUTS} positive multiples of 8 that add up to {C} channels")
+    if split is None:
+        outs: List[torch.Tensor] = [_destination("output", output, (T, C), _BF16, device)]
+    else:
+        if output is not None and len(output) != len(widths):
+            raise ValueError("output must hold one tensor per split")
+        outs = [_destination("output", None if output is None else output[j], (T, n), _BF16, device)
+                for j, n in enumerate(widths)]
+    shape = (num_seqs, W - 1, C)
+    new_state = _destination("new_state", new_state, shape, _BF16, device)
+    state = _state(state, new_state, shape, _BF16)
+    n = len(widths)
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
+    head = (_ptr(x), stride, _ptr(weight), _ptr(bias), _GATE_DTYPES[weight.dtype], _ptr(state))
+    tail = (_ACTIVATIONS[activation], ptrs, (ctypes.c_int64 * n)(*widths), n, _ptr(new_state))
+    # (the converted copies live until the call has been enqueued)
+    return head, tail, (T, C, W), outs[0] if split is None else tuple(outs), new_state, (x, weight, bias, state)
+
+
+def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                 state: Optional[torch.Tensor], cu_seqlens: torch.Tensor, *,
+                 activation: Optional[str] = "silu", split: Optional[Sequence[int]] = None,
+                 output=None, new_state: Optional[torch.Tensor] = None,
+                 validate: bool = True) -> Tuple[Outputs, torch.Tensor]:
+    """Short depthwise causal convolution over packed sequences:
+    y[t, c] = act(bias[c] + sum_w weight[c, w] * x[t - (W-1) + w, c]).
+
+    x [T, C] bf16 (C a multiple of 8; a slice of wider rows is read in place); weight [C, W]
+    with W = 2, 3 or 4, and bias [C] or None, fp32 or bf16; state [N, W-1, C] bf16 (the rows
+    in front of each sequence, oldest first) or None for zeros; cu_seqlens [N+1] as for
+    ``kernel``.  ``activation`` is "silu" or None.  Returns (y [T, C] bf16, new_state
+    [N, W-1, C] bf16), the new state being the last W-1 rows of [state; x].
+
+    ``split`` gives the widths of up to four packed tensors that take the channels side by
+    side, such as q, k and v for ``kernel`` or x, B and C for ``ssm_prefill``; y (and
+    ``output``) is then a tuple of [T, width] tensors.  new_state must not overlap state.
+    """
+    device = x.device
+    _on(device, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    if x.dim() != 2:
+        raise ValueError("x must be [T, channels]")
+    cu, N = _cu(cu_seqlens, x.shape[0], device, validate)
+    head, tail, (T, C, W), y, new_state, held = _conv(x, weight, bias, state, N, activation, split, output, new_state)
+    lib = _lib.load()
+    ctx, stream = _on_device(device)
+    with ctx:
+        _lib.check(lib.gdn_conv_prefill(*head, _ptr(cu), N, T, C, W, *tail, stream))
+    return y, new_state
+
+
+def conv_decode(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                state: Optional[torch.Tensor], *, activation: Optional[str] = "silu",
+                split: Optional[Sequence[int]] = None, output=None,
+                new_state: Optional[torch.Tensor] = None) -> Tuple[Outputs, torch.Tensor]:
+    """``conv_prefill`` for one token of each sequence: x [B, C], state [B, W-1, C] bf16 or
+    None.  Returns (y [B, C], new_state); pass ``new_state=state`` to update it in place."""
+    device = x.device
+    _on(device, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    head, tail, (B, C, W), y, new_state, held = _conv(x, weight, bias, state, x.shape[0], activation, split, output,
+                                                      new_state)
+    lib = _lib.load()
+    ctx, stream = _on_device(device)
+    with ctx:
+        _lib.check(lib.gdn_conv_decode(*head, B, C, W, *tail, stream))
+    return y, new_state
+
+
+# ------------------------------------------------------------------------------- the scan
+
+def ssm_method(total_tokens: int, method: str = "auto", num_seqs: int = 1) -> str:
+    """Name of the scan kernel an ``ssm_prefill`` call with ``method`` runs for
+    ``total_tokens`` packed tokens in ``num_seqs`` sequences on the current CUDA device."""
+    if method not in _METHODS:
+        raise ValueError(f"method must be one of {sorted(_METHODS)}")
+    code = _lib.load().gdn_ssm_resolve(int(total_tokens), int(num_seqs), _METHODS[method])
+    return {v: k for k, v in _METHODS.items()}[code]
+
+
+def _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, num_seqs, output, new_state):
+    """The checks and conversions of both scan calls."""
+    device = x.device
+    lead = tuple(x.shape[:-2])
+    H, P = x.shape[-2:]
+    if P != 64 and P != 128:
+        raise NotImplementedError(f"head_size={P} is not supported (64 or 128)")
+    if B.dim() != x.dim() or tuple(B.shape[:-2]) != lead:
+        raise ValueError(f"B must be [..., groups, state_size] with x's leading shape {lead}, got {tuple(B.shape)}")
+    G, S = B.shape[-2:]
+    if S != 128:
+        raise NotImplementedError(f"state_size={S} is not supported (only 128)")
+    if C.shape != B.shape:
+        raise ValueError(f"C shape {tuple(C.shape)} must equal B shape {tuple(B.shape)}")
+    if H == 0 or G == 0 or H % G:
+        raise ValueError(f"{H} heads must be a positive multiple of {G} groups")
+    if tuple(dt.shape) != lead + (H,):
+        raise ValueError(f"dt must be {list(lead + (H,))}, got {list(dt.shape)}")
+    for name, t in (("A_log", A_log), ("D", D), ("dt_bias", dt_bias)):
+        if t is not None and tuple(t.shape) != (H,):
+            raise ValueError(f"{name} must be [heads] = [{H}]")
+    if z is not None and z.shape != x.shape:
+        raise ValueError(f"z shape {tuple(z.shape)} must equal x shape {tuple(x.shape)}")
+    x, sx = _rows("x", x, H * P)
+    B, sB = _rows("B", B, G * S)
+    C, sC = _rows("C", C, G * S)
+    if z is not None:
+        z, sz = _rows("z", z, H * P)
+    else:
+        sz = 0
+    dt, sdt = _dt_rows(dt, H)
+    A_log = _gate(A_log)
+    D = None if D is None else _gate(D)
+    dt_bias = None if dt_bias is None else _gate(dt_bias)
+    if (D is not None and D.dtype != A_log.dtype) or (dt_bias is not None and dt_bias.dtype != A_log.dtype):
+        A_log = A_log.float()
+        D = None if D is None else D.float()
+        dt_bias = None if dt_bias is None else dt_bias.float()
+    output = _destination("output", output, lead + (H, P), _BF16, device)
+    shape = (num_seqs, H, P, S)
+    new_state = _destination("new_state", new_state, shape, _F32, device)
+    state = _state(state, new_state, shape, _F32)
+    head = (_ptr(x), sx, _ptr(dt), sdt, _ptr(A_log), _ptr(B), sB, _ptr(C), sC, _ptr(D), _ptr(dt_bias), _ptr(z), sz,
+            _ptr(state))
+    tail = (H, G, P, S, _GATE_DTYPES[dt.dtype], _GATE_DTYPES[A_log.dtype], _ptr(output), _ptr(new_state))
+    # (the converted copies live until the call has been enqueued)
+    return head, tail, output, new_state, (x, dt, A_log, B, C, D, dt_bias, z, state)
+
+
+def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                D: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], state: Optional[torch.Tensor],
+                cu_seqlens: torch.Tensor, *, z: Optional[torch.Tensor] = None,
+                output: Optional[torch.Tensor] = None, new_state: Optional[torch.Tensor] = None,
+                method: str = "auto", validate: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Selective scan with one decay per head over packed sequences:
+
+        dt' = softplus(dt + dt_bias),  S <- exp(-exp(A_log) dt') S + dt' x B^T,
+        y = S C + D x,  and with ``z``  y <- y * silu(z).
+
+    x, z [T, H, P] bf16 (P = 64 or 128); dt [T, H]; B, C [T, G, 128] bf16, shared by the
+    H / G consecutive heads of a group; A_log, D, dt_bias [H] (D and dt_bias may be None);
+    state [N, H, P, 128] fp32 or None for zeros; cu_seqlens [N+1] as for ``kernel``.  Returns
+    (y [T, H, P] bf16, new_state [N, H, P, 128] fp32); a sequence of length 0 keeps its
+    state.  new_state must not overlap state.
+
+    ``method`` chooses the kernel: "tcgen05" (64-token chunks on the tensor cores, from 64
+    tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what
+    ``ssm_method`` reports).
+    """
+    device = x.device
+    _on(device, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
+                 ("state", state), ("z", z)))
+    if x.dim() != 3:
+        raise ValueError("x must be [T, heads, head_size]")
+    if method not in _METHODS:
+        raise ValueError(f"method must be one of {sorted(_METHODS)}")
+    T = x.shape[0]
+    cu, N = _cu(cu_seqlens, T, device, validate)
+    head, tail, output, new_state, held = _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, N, output, new_state)
+    lib = _lib.load()
+    ctx, stream = _on_device(device)
+    with ctx:
+        _lib.check(lib.gdn_ssm_prefill(*head, _ptr(cu), N, T, *tail, _METHODS[method], stream))
+    return output, new_state
+
+
+def ssm_decode(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+               D: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], state: Optional[torch.Tensor], *,
+               z: Optional[torch.Tensor] = None, output: Optional[torch.Tensor] = None,
+               new_state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step of ``ssm_prefill``'s scan for each sequence: x, z [B, 1, H, P]; dt [B, 1, H];
+    B, C [B, 1, G, 128]; state [B, H, P, 128] fp32 or None.  Returns (y [B, 1, H, P] bf16,
+    new_state); pass ``new_state=state`` to update the state in place."""
+    device = x.device
+    _on(device, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
+                 ("state", state), ("z", z)))
+    if x.dim() != 4 or x.shape[1] != 1:
+        raise ValueError("x must be [B, 1, heads, head_size]")
+    batch = x.shape[0]
+    head, tail, output, new_state, held = _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, batch, output, new_state)
+    lib = _lib.load()
+    ctx, stream = _on_device(device)
+    with ctx:
+        _lib.check(lib.gdn_ssm_decode(*head, batch, *tail, stream))
+    return output, new_state

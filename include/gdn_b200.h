@@ -46,6 +46,10 @@ extern "C" {
 /* Option bits for gdn_prefill_flags() / gdn_decode_flags(). */
 #define GDN_FLAG_QK_L2NORM 1   /* L2-normalise every q and k head vector first (see below) */
 
+/* Activation of the short convolution. */
+#define GDN_ACTIVATION_NONE 0
+#define GDN_ACTIVATION_SILU 1          /* y / (1 + exp(-y)) */
+
 /* Prefill kernel choice for gdn_prefill_ex(). */
 #define GDN_PREFILL_AUTO 0      /* see gdn_prefill_resolve() */
 #define GDN_PREFILL_CHUNKED 1   /* chunked (C=64) WY/UT kernel on the tensor cores (mma.sync) */
@@ -268,6 +272,96 @@ GDN_API int gdn_decode_strided(const void *q, const void *k, const void *v, cons
                        float scale, int gate_dtype, int param_dtype, void *output,
                        float *new_state, int64_t a_row_stride, int64_t b_row_stride, int flags,
                        void *stream);
+
+/*
+ * The short causal convolution in front of a linear-attention layer's recurrence (its q, k
+ * and v, or a state space layer's x, B and C), over packed sequences:
+ *
+ *   y[t][c] = act(bias[c] + sum_{w < width} weight[c][w] * x[t - (width-1) + w][c])
+ *
+ * with the width-1 rows of `state` in front of each sequence's first token, in fp32 from
+ * bf16 rows and rounded once.  No counterpart in the reference (its entry points take q, k
+ * and v).
+ *
+ *   x           bf16 rows [total_tokens][channels], x_row_stride elements apart (0: packed);
+ *               x and x_row_stride * 2 bytes 16-byte aligned, so a slice of the
+ *               projection's output passes as it is
+ *   weight      [channels][width] (weight_dtype: GDN_DTYPE_F32 or GDN_DTYPE_BF16)
+ *   bias        [channels] (weight_dtype) or NULL
+ *   state       bf16 [num_seqs][width-1][channels], oldest row first, or NULL for zeros
+ *   cu_seqlens  as gdn_prefill's, checked on the device in the same way
+ *   outputs     num_outputs (1 to 4) packed bf16 tensors [total_tokens][output_widths[j]]
+ *               that take the channels side by side; `outputs` and `output_widths` are host
+ *               arrays, read during the call
+ *   new_state   bf16 [num_seqs][width-1][channels]: the last width-1 rows of [state; x] of
+ *               each sequence (its state unchanged when it is empty); must not overlap state
+ *
+ * Requirements: width 2, 3 or 4; channels and every output width multiples of 8; 16-byte
+ * aligned pointers (weight and bias: their element's alignment).  Outputs must not overlap
+ * inputs.
+ */
+GDN_API int gdn_conv_prefill(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
+                     int weight_dtype, const void *state, const int32_t *cu_seqlens, int64_t num_seqs,
+                     int64_t total_tokens, int64_t channels, int width, int activation, void *const *outputs,
+                     const int64_t *output_widths, int num_outputs, void *new_state, void *stream);
+
+/* The same convolution for one token of each of `batch` sequences: x [batch][channels]
+ * (rows x_row_stride apart), outputs [batch][output_widths[j]].  new_state may be the same
+ * pointer as state (in place), but must not partially overlap it. */
+GDN_API int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
+                    int weight_dtype, const void *state, int64_t batch, int64_t channels, int width,
+                    int activation, void *const *outputs, const int64_t *output_widths, int num_outputs,
+                    void *new_state, void *stream);
+
+/*
+ * Selective scan of a state space layer with one decay per head, over packed sequences:
+ *
+ *   dt'_t = softplus(dt_t + dt_bias),   alpha_t = exp(-exp(A_log) dt'_t)
+ *   S_t   = alpha_t S_{t-1} + dt'_t x_t B_t^T
+ *   y_t   = S_t C_t + D x_t,   and with z:  y_t <- y_t * z_t / (1 + exp(-z_t))
+ *
+ * with S [head_size][state_size] per head, k-last as gdn_prefill's, and B and C shared by
+ * the num_heads / num_groups consecutive heads of a group.  No counterpart in the reference.
+ *
+ *   x, z        bf16 rows [total_tokens][num_heads][head_size]; z may be NULL
+ *   dt          [total_tokens][num_heads] (dt_dtype)
+ *   B, C        bf16 rows [total_tokens][num_groups][state_size]
+ *   A_log, D, dt_bias   [num_heads] (param_dtype); D and dt_bias may be NULL (zero)
+ *   state       fp32 [num_seqs][num_heads][head_size][state_size] or NULL for zeros
+ *   cu_seqlens  as gdn_prefill's, checked on the device in the same way
+ *   output      bf16 [total_tokens][num_heads][head_size], packed
+ *   new_state   as state; a sequence of length 0 keeps its state; must not overlap state
+ *   *_row_stride  elements between the rows of consecutive tokens (0: packed), so slices of
+ *               a projection's or the convolution's output pass as they are
+ *   method      GDN_PREFILL_AUTO (gdn_ssm_resolve()), GDN_PREFILL_RECURRENT (token-serial,
+ *               CUDA cores) or GDN_PREFILL_TCGEN05 (64-token chunks on the tensor cores;
+ *               total_tokens >= 64)
+ *
+ * Requirements: head_size 64 or 128, state_size 128, num_heads % num_groups == 0; x, z, B,
+ * C, output, state and new_state 16-byte aligned and the row strides of x, z, B and C
+ * multiples of 8.  The output must not overlap inputs.  A sequence's outputs and state
+ * depend on its own rows alone.  Within a sequence, GDN_PREFILL_TCGEN05 lets an infinity or
+ * NaN in x, B or C also reach the outputs of the tokens before it in its 64-token chunk.
+ */
+GDN_API int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
+                    const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,
+                    const void *D, const void *dt_bias, const void *z, int64_t z_row_stride, const float *state,
+                    const int32_t *cu_seqlens, int64_t num_seqs, int64_t total_tokens, int num_heads,
+                    int num_groups, int head_size, int state_size, int dt_dtype, int param_dtype, void *output,
+                    float *new_state, int method, void *stream);
+
+/* The scan kernel (GDN_PREFILL_*) a gdn_ssm_prefill call with `method` runs on the current
+ * device. */
+GDN_API int gdn_ssm_resolve(int64_t total_tokens, int64_t num_seqs, int method);
+
+/* One step of the scan for each of `batch` sequences (rows of one token each; state, and
+ * output [batch][num_heads][head_size]).  new_state may be the same pointer as state (in
+ * place), but must not partially overlap it. */
+GDN_API int gdn_ssm_decode(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
+                   const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,
+                   const void *D, const void *dt_bias, const void *z, int64_t z_row_stride, const float *state,
+                   int64_t batch, int num_heads, int num_groups, int head_size, int state_size, int dt_dtype,
+                   int param_dtype, void *output, float *new_state, void *stream);
 
 /*
  * Synchronizes `stream` and reports the library's device status word since the last
