@@ -101,6 +101,9 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream);
 cudaError_t launch_conv_prefill(const ConvArgs &p, cudaStream_t stream);
 cudaError_t launch_conv_decode(const ConvArgs &p, cudaStream_t stream);
 cudaError_t launch_ssm_decode(const SsmArgs &p, cudaStream_t stream);
+// The chunked scan on tcgen05 (gdn_ssm_tc.cu).
+bool ssm_prefill_tc_supported(int64_t total_tokens);
+cudaError_t launch_ssm_prefill_tc(const SsmArgs &p, cudaStream_t stream);
 cudaError_t launch_ssm_prefill_recurrent(const SsmArgs &p, cudaStream_t stream);
 
 cudaError_t launch_decode(const DecodeArgs &p, cudaStream_t stream);
@@ -158,5 +161,7 @@ int *device_status_word();
 // Limit of every bounded device wait of the tcgen05 chains, in ns (0: the default 2 s);
 // returns the previous setting.
 uint64_t set_wait_limit_ns(uint64_t ns);
+// The limit in force.
+uint64_t wait_limit_ns();
 
 }  // namespace gdn

@@ -900,8 +900,7 @@ cudaError_t launch_prefill_tc(const PrefillArgs &p, void *workspace, cudaStream_
                                          SMEM_BYTES_GATED);
     const uint32_t smem = p.out_gate ? SMEM_BYTES_GATED : SMEM_BYTES;
     if (e != cudaSuccess) return e;
-    const uint64_t limit = g_wait_limit_ns.load(std::memory_order_relaxed);
-    const uint64_t wait_ns = limit ? limit : kDefaultWaitNs;
+    const uint64_t wait_ns = wait_limit_ns();
     // The split: the last `tail` chains (0: none) on the overlap stream.
     std::unique_lock<std::mutex> lock(g_overlap_mu, std::defer_lock);
     OverlapStream *o = nullptr;
@@ -954,6 +953,11 @@ cudaError_t launch_prefill_tc(const PrefillArgs &p, void *workspace, cudaStream_
 }
 
 uint64_t set_wait_limit_ns(uint64_t ns) { return g_wait_limit_ns.exchange(ns); }
+
+uint64_t wait_limit_ns() {
+    const uint64_t limit = g_wait_limit_ns.load(std::memory_order_relaxed);
+    return limit ? limit : kDefaultWaitNs;
+}
 
 int *device_status_word() {
     void *ptr = nullptr;

@@ -12,6 +12,8 @@ namespace {
 
 constexpr int64_t kMaxStride = 0x7fffffff;
 constexpr int64_t kMaxRows = int64_t(1) << 31;
+constexpr int64_t kAutoTcMinTokens = 64;
+constexpr int64_t kAutoTcMinPerSeq = 8;
 
 int fail(int code, const char *fmt, ...) {
     char buf[512];
@@ -203,9 +205,11 @@ int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *weight, con
 
 int gdn_ssm_resolve(int64_t total_tokens, int64_t num_seqs, int method) {
     if (method != GDN_PREFILL_AUTO) return method;
-    (void)total_tokens;
-    (void)num_seqs;
-    return GDN_PREFILL_RECURRENT;
+    // Short prompts: the token-serial kernel, which also keeps every product in fp32.
+    if (total_tokens < kAutoTcMinTokens || total_tokens < kAutoTcMinPerSeq * num_seqs ||
+        !gdn::ssm_prefill_tc_supported(total_tokens))
+        return GDN_PREFILL_RECURRENT;
+    return GDN_PREFILL_TCGEN05;
 }
 
 int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride, const void *A_log,
@@ -223,12 +227,16 @@ int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t
         return fail(GDN_ERR_INVALID_ARGUMENT, "unknown scan method %d", method);
     if (num_seqs == 0) return GDN_OK;
     if (!cu_seqlens) return fail(GDN_ERR_INVALID_ARGUMENT, "null cu_seqlens");
-    if (method == GDN_PREFILL_TCGEN05) return fail(GDN_ERR_UNSUPPORTED, "the tensor-core scan is not built yet");
     if (state && ranges_overlap(state, ssm_state_bytes(p), new_state, ssm_state_bytes(p)))
         return fail(GDN_ERR_INVALID_ARGUMENT, "prefill new_state must not overlap state");
     p.cu_seqlens = cu_seqlens;
     p.status = gdn::device_status_word();
     const auto s = static_cast<cudaStream_t>(stream);
+    if (gdn_ssm_resolve(total_tokens, num_seqs, method) == GDN_PREFILL_TCGEN05) {
+        if (!gdn::ssm_prefill_tc_supported(total_tokens))
+            return fail(GDN_ERR_UNSUPPORTED, "the tcgen05 scan needs an sm_100 device and total_tokens >= 64");
+        return cuda_status(gdn::launch_ssm_prefill_tc(p, s), "gdn_ssm_prefill (tcgen05) launch");
+    }
     return cuda_status(gdn::launch_ssm_prefill_recurrent(p, s), "gdn_ssm_prefill (recurrent) launch");
 }
 

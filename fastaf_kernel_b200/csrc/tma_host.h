@@ -40,4 +40,20 @@ inline bool make_tmap_thd_bf16(CUtensorMap *map, const void *base, int64_t T, in
     return r == CUDA_SUCCESS;
 }
 
+// Tensor map over bf16 rows of `width` elements, `stride` elements apart (both multiples of
+// 8), whose box is 64 elements x 64 rows, written to shared memory with the 128-byte
+// swizzle.  Rows past the last one read as zero.
+inline bool make_tmap_rows_bf16(CUtensorMap *map, const void *base, int64_t rows, int64_t width, int64_t stride) {
+    auto enc = tensor_map_encoder();
+    if (enc == nullptr || rows <= 0 || width <= 0) return false;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+    cuuint32_t box[2] = {64, 64};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 }  // namespace gdn

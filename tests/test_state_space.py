@@ -22,7 +22,7 @@ DEV = torch.device("cuda", 0)
 HALF = torch.finfo(torch.bfloat16).eps / 2      # 2^-8
 F64 = torch.float64
 TINY = 1e-30
-METHODS = ["recurrent"]
+METHODS = ["recurrent", "tcgen05"]
 
 
 # --------------------------------------------------------------------------- references
