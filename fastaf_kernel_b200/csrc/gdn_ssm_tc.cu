@@ -17,21 +17,32 @@
 //                                of the M = 128 tile read what lies behind it and are unused)
 //   Yi^T = bf16(S) C^T           the state's part, scaled by exp(la_i) per column afterwards
 //   Ya^T = x^T bf16(M)^T         the chunk's own part; D sits on M's diagonal
-//   S   += (w x)^T B             w x split into bf16 hi + lo (two products), so the fp32
-//                                state loses 2^-17 per term, not 2^-9
-// M's exponentials: la_i - la_j <= 0 on and below the diagonal, so none overflows; the block
-// of rows 32..63 and columns 0..31 factors into exp(la_i - la_31) exp(la_31 - la_j), both at
-// most 1, and only the two diagonal 32 x 32 blocks take one exponential per element.
+//   S   += (w x)^T B             w x as bf16 hi + lo (two products), so the fp32 state loses
+//                                2^-16 per term, not 2^-8: with w = wh + wl in bf16,
+//                                hi = bf16(x wh) and lo = bf16(x wl + (x wh - hi)), whose
+//                                inner difference is exact -- three bf16 operations for two
+//                                terms; a TMEM operand, which keeps 48 KB a chunk out of the
+//                                shared memory's bandwidth
+// M's exponentials factor by blocks of 8 columns: exp(la_i - la_j) = exp(la_i - la_r)
+// exp(la_r - la_j) with r the block's last column, both at most 1 for the rows below the
+// block; the 8 rows of the block itself take one exponential per element.  So a row of 32
+// columns takes 12 exponentials, and none overflows however strong the decays are.
 //
 // Roles (20 warps), handing chunks to each other through mbarriers:
-//   warp 0       allocates TMEM; lane 0 issues every MMA as soon as its inputs are ready,
-//                the state update first
-//   warp 1       copies (TMA), two stages of C, B and x, and of z
-//   warps 2, 3   the chunk's gates, one head each
-//   warps 4-7    state path: S -> bf16 copy (TMEM operand of Yi) and the decay of S
-//   warps 8-11   outputs: Yi, Ya from TMEM, the gate z, bf16 rows through shared memory
-//   warps 12, 13, 17   M, a 32 x 32 block each
-//   warps 14, 15, 18, 19   w x hi / lo; the rows behind the last token set to zero
+//   warp 0        allocates TMEM and issues the MMAs in a fixed order per chunk c: the state
+//                 update(c), G(c + 1), Yi(c), Ya(c)
+//   warp 18       copies (TMA): three stages of C, B and x, two of z, and boxes further ahead
+//                 into L2
+//   warps 2, 3    the chunk's gates: one head each, or one head's chunks in turn
+//   warps 4-7     state path: S -> bf16 copy (TMEM operand of Yi) and the decay of S
+//   warps 12-15   w x hi / lo into TMEM; the rows behind the last token set to zero
+//   warps 16, 17, 1   M, a 32 x 32 block each
+//   warps 8-11    outputs: Yi, Ya from TMEM as accumulator fragments, the gate z, transposed
+//                 into bf16 rows in shared memory (stmatrix)
+//   warp 19       output rows to global memory (TMA; the last, partial chunk by hand)
+// The loops are kept rolled and the waits out of line: together they have to fit the SM's
+// instruction caches (with everything unrolled a chunk took 7,200 cycles, two thirds of the
+// issue slots waiting for instructions).
 //
 // Every wait is bounded as in gdn_prefill_tc.cu: one that gives up records its site in the
 // device status word and raises a shared flag, every role stops at its next wait, the
@@ -39,6 +50,7 @@
 #include <cuda_bf16.h>
 #include <cstring>
 
+#include "gdn_mma_sync.cuh"
 #include "gdn_ssm_common.cuh"
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -48,47 +60,58 @@ namespace gdn {
 namespace {
 
 using namespace sm100;
+using msync::ldsm_x4_t;
+using msync::stsm_x4_t;
 
 constexpr int kL = 64;              // tokens of a chunk
 constexpr int kThreads = 640;
 constexpr int kRows = 128;          // state rows of a CTA
-constexpr int kSplitWarps = 4, kMWarps = 3;
+constexpr int kStages = 3;          // of C, B, x
+constexpr int kGateStages = 4;
+constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
+constexpr int kMWarps = 3;
+constexpr int kUpdateWarps = 8;      // of the state path and the split
 
 // Shared memory (bytes from the 1024-aligned base).  Tiles are 64 rows of 64 bf16 (one
 // 128-byte swizzled atom, 8 KB), two atoms side by side.
 constexpr uint32_t kTile = 16 * 1024;
-constexpr uint32_t OFF_STAGE = 0;                       // 2 x [C | B | x]
+constexpr uint32_t OFF_STAGE = 0;                                // kStages x [C | B | x]
 constexpr uint32_t STAGE = 3 * kTile;
 constexpr uint32_t ST_C = 0, ST_B = kTile, ST_X = 2 * kTile;
-constexpr uint32_t OFF_WX = OFF_STAGE + 2 * STAGE;      // [hi | lo], each as x
-constexpr uint32_t OFF_M = OFF_WX + 2 * kTile;          // [head][i][j], K-major, 8 KB each
-constexpr uint32_t OFF_Y = OFF_M + kTile;               // bf16 [64][128] output rows
-constexpr uint32_t OFF_GATE = OFF_Y + kTile;            // 2 x 2 heads x Gates
-constexpr uint32_t GATE = 1536;
-constexpr uint32_t OFF_Z = OFF_GATE + 6 * 1024;         // 2 x z, only with the output gate
-constexpr uint32_t SMEM_PLAIN = OFF_Z, SMEM_GATED = OFF_Z + 2 * kTile;
-static_assert(OFF_Z % 1024 == 0 && SMEM_GATED <= 227 * 1024, "shared memory map");
+constexpr uint32_t OFF_M = OFF_STAGE + kStages * STAGE;          // [head][i][j], K-major, 8 KB each
+constexpr uint32_t OFF_Y = OFF_M + kTile;                        // 2 x z, then the output rows in its place
+constexpr uint32_t OFF_GATE = OFF_Y + 2 * kTile;                 // kGateStages x 2 heads x Gates
+constexpr uint32_t GATE = 1408;
+constexpr uint32_t SMEM_BYTES = OFF_GATE + kGateStages * 2 * GATE;
+static_assert(SMEM_BYTES <= 227 * 1024 - 1024, "shared memory map");
 
-struct Gates {
-    float la[64];    // sum of the log2 decays from the start of the token's 32-token half
-    float dt[64];    // dt'
-    float e[64];     // exp(la_i) from the start of the chunk
-    float w[64];     // exp(la_63 - la_j) dt'_j
-    float cf[32];    // exp(la_31 - la_j) dt'_j, j < 32
-    float rf[32];    // exp(la_{32 + i} - la_31)
-    float total;     // exp(la_63)
+struct alignas(16) Gates {
+    float la[64];         // log2 of the decays' products from the start of the chunk
+    float lb[64];         // la_j - log2(dt'_j): 2^(la_i - lb_j) = exp(la_i - la_j) dt'_j
+    float cf[64];         // exp(la_r - la_j) dt'_j, r = j | 7
+    float e[64];          // exp(la_i)
+    uint32_t wh[32], wl[32];   // w_j = exp(la_63 - la_j) dt'_j as bf16 hi + lo, two tokens a word
+    float total;          // exp(la_63)
 };
 static_assert(sizeof(Gates) <= GATE, "gate block");
 
-// TMEM columns (all 512 allocated).
-constexpr uint32_t TM_S = 0;       // [0, 128)   fp32 state
-constexpr uint32_t TM_SB = 128;    // 2 x 64     bf16x2 copy of the state in front of a chunk
-constexpr uint32_t TM_G = 256;     // [256, 320) G, lanes 0..63
-constexpr uint32_t TM_YI = 320;    // [320, 384) Yi^T
-constexpr uint32_t TM_YA = 384;    // [384, 512) Ya^T: 64 columns, or 64 per head of a pair
+// TMEM columns (all 512 allocated).  One head: two copies of bf16(S), so that the state path
+// of a chunk need not wait for Yi of the one before; two heads: one copy, since Ya takes 64
+// columns per head (rows 0..63 use the first head's, rows 64..127 the second's).
+template <bool PAIR>
+struct Tm {
+    static constexpr uint32_t S = 0;                         // [0, 128) fp32 state
+    static constexpr uint32_t SB = 128;                      // bf16x2, 64 columns a copy
+    static constexpr int kCopies = PAIR ? 1 : 2;
+    static constexpr uint32_t G = SB + 64 * kCopies;         // lanes 0..63
+    static constexpr uint32_t YI = G + 64, YA = YI + 64;
+    static constexpr uint32_t W = YA + (PAIR ? 128 : 64);    // bf16x2 w x: 32 columns hi, 32 lo
+    static_assert(W + 64 == 512, "TMEM map");
+};
 
-enum WaitSite { kSsmTma = 41, kSsmZ = 42, kSsmGates = 43, kSsmG = 44, kSsmM = 45, kSsmS = 46, kSsmCS = 47,
-                kSsmMX = 48, kSsmIssue = 49, kSsmY = 50, kSsmStage = 51, kSsmFree = 52 };
+enum WaitSite { kSsmTma = 41, kSsmZ = 42, kSsmGates = 43, kSsmG = 44, kSsmM = 45, kSsmS = 46,
+                kSsmMX = 48, kSsmUpdate = 47, kSsmIssue = 49, kSsmY = 50, kSsmStage = 51, kSsmFree = 52,
+                kSsmRead = 54 };
 constexpr uint64_t kDrainNs = 2000000000ull;
 constexpr uint32_t kMaxSuspendNs = 1000000;
 
@@ -99,44 +122,69 @@ struct TcArgs {
 };
 
 struct Bars {
-    uint64_t full[2], empty[2], zfull[2], gates[2], ydone[2], cs[2];
-    uint64_t g, mread, mready, mx, s, sready, split, yread, yst, yfree;
+    uint64_t full[kStages], empty[kStages], gates[kGateStages], ydone[kGateStages];
+    uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2];
+    uint64_t g, mread, s, update, yread, last;
 };
 
-struct Waiter {
-    volatile int *abort;
-    int *status;
+// What a wait looks at besides its barrier, at the end of the dynamic shared memory.
+struct WaitControl {
     uint64_t limit;
+    int *status;
+    volatile int abort;
+};
+__device__ __forceinline__ WaitControl *wait_control() {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    return reinterpret_cast<WaitControl *>(sm + SMEM_BYTES);
+}
 
-    __device__ __forceinline__ bool one(uint32_t bar, uint32_t parity, int site) const {
-        if (mbar_try_wait(bar, parity)) return true;
-        const uint64_t t0 = global_timer_ns();
-        const uint32_t hint = limit < kMaxSuspendNs ? static_cast<uint32_t>(limit) : kMaxSuspendNs;
-        for (;;) {
-            if (mbar_try_wait_hint(bar, parity, hint)) return true;
-            if (*abort) return false;
-            if (global_timer_ns() - t0 > limit) {
-                give_up(site);
-                return false;
-            }
+// A wait behind its first probe, out of line (see above).  `key` is the phase's parity and,
+// above it, the WaitSite.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t key) {
+    WaitControl *ctl = wait_control();
+    const uint64_t t0 = global_timer_ns(), limit = ctl->limit;
+    const uint32_t hint = limit < kMaxSuspendNs ? static_cast<uint32_t>(limit) : kMaxSuspendNs;
+    for (;;) {
+        if (mbar_try_wait_hint(bar, key & 1, hint)) return true;
+        if (ctl->abort) return false;
+        if (global_timer_ns() - t0 > limit) {
+            if (ctl->status) atomicCAS(ctl->status, 0, static_cast<int>(key >> 1));
+            ctl->abort = 1;
+            return false;
         }
     }
-    __device__ __forceinline__ void give_up(int site) const {
-        if (status) atomicCAS(status, 0, site);
-        *abort = 1;
+}
+// This CTA's own copies and MMAs, also after a give-up.
+__device__ __noinline__ void wait_own(uint32_t bar, uint32_t key) {
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait_hint(bar, key & 1, kMaxSuspendNs)) {
+        if (global_timer_ns() - t0 > kDrainNs) {
+            WaitControl *ctl = wait_control();
+            if (ctl->status) atomicCAS(ctl->status, 0, static_cast<int>(key >> 1));
+            return;
+        }
     }
-    // The whole warp; reconverges it for the next .aligned tcgen05 instruction.
-    __device__ __forceinline__ bool warp(uint32_t bar, uint32_t parity, int site) const {
-        const bool ok = one(bar, parity, site);
-        __syncwarp();
+}
+
+// A barrier's phases are told apart by parity, so a wait for phase k (0, 1, ...) may only
+// look while phase k + 1 cannot be complete; tests/test_ssm_chain_protocol.py models it.
+struct Waiter {
+    static __device__ __forceinline__ uint32_t key(uint32_t phase, int site) { return (phase & 1u) | (site << 1); }
+    __device__ __forceinline__ bool one(uint32_t bar, uint32_t phase, int site) const {
+        return mbar_try_wait(bar, phase & 1) || wait_slow(bar, key(phase, site));
+    }
+    // The whole warp; it stays converged for the next .aligned tcgen05 instruction.
+    __device__ __forceinline__ bool warp(uint32_t bar, uint32_t phase, int site) const {
+        bool ok = mbar_try_wait(bar, phase & 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+            if (!ok) ok = wait_slow(bar, key(phase, site));
+            if (!__all_sync(0xffffffffu, ok)) return false;
+        }
         tc_fence_after();
-        return __all_sync(0xffffffffu, ok);
+        return true;
     }
-    // This CTA's own copies and MMAs, also after a give-up.
-    __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, int site) const {
-        volatile int never = 0;
-        Waiter w{&never, status, kDrainNs};
-        w.one(bar, parity, site);
+    __device__ __forceinline__ void drain(uint32_t bar, uint32_t phase, int site) const {
+        wait_own(bar, key(phase, site));
     }
 };
 
@@ -145,19 +193,62 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
     if (lane == 0) mbar_arrive(bar);
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t bits2(uint32_t lo, uint32_t hi) {
+    return f2(__uint_as_float(lo), __uint_as_float(hi));
+}
+// Two bf16 products / fused multiply-adds, one rounding each.
+__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+// softplus(x) = max(x, 0) + log(1 + u), u = exp(-|x|) in (0, 1], with the logarithm from the
+// series log(1 + u) = 2 (s + s^3/3 + s^5/5 + ...), s = u / (2 + u) <= 1/3, whose first term
+// left out is below 2^-22 of the sum: a few instructions, and accurate relative to small
+// results too.  (torch's softplus is x itself above 20, which this rounds to as well.)
+__device__ __forceinline__ float softplus_series(float x) {
+    const float u = ex2(-1.4426950408889634f * fabsf(x));
+    const float s = __fdividef(u, 2.0f + u), q = s * s;
+    float v = fmaf(q, 1.0f / 11.0f, 1.0f / 9.0f);
+    v = fmaf(q, v, 1.0f / 7.0f);
+    v = fmaf(q, v, 1.0f / 5.0f);
+    v = fmaf(q, v, 1.0f / 3.0f);
+    v = fmaf(q * v, s, s);
+    return fmaxf(x, 0.0f) + 2.0f * v;
+}
+
 // PAIR: two heads of 64 rows; else one head of 128.
 template <bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap bmap,
-              const __grid_constant__ CUtensorMap cmap, const __grid_constant__ CUtensorMap zmap, const TcArgs args) {
+              const __grid_constant__ CUtensorMap cmap, const __grid_constant__ CUtensorMap zmap,
+              const __grid_constant__ CUtensorMap ymap, const TcArgs args) {
     extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ Bars bars;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    using TM = Tm<PAIR>;
     const SsmArgs &p = args.a;
     constexpr int kHeads = PAIR ? 2 : 1;
+    constexpr int kMBuffers = PAIR ? 1 : 2;    // M tiles: one of both heads, or two of the one
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (warp-uniform for the compiler too, so that the MMA warp's loop and descriptors are)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) * 32;
     const int row = static_cast<int>(lane_base) + lane;    // this thread's TMEM lane
     const int64_t n = blockIdx.x / args.slabs;
@@ -174,13 +265,15 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     const bool gated = p.z != nullptr;
     const uint32_t sbase = smem_u32(sm);
     auto bar = [&](const uint64_t &b) { return smem_u32(&b); };
-    const Waiter wait{&abort_flag, p.status, args.wait_ns};
+    const Waiter wait;
 
     // this thread's state row: of head h0, or for the second half of a pair of head h0 + 1
     const int hrow = PAIR ? row >> 6 : 0;
     const bool dead = lone && hrow == 1;
     const int64_t state_at =
         ((n * p.heads + h0 + hrow) * p.head_size + (PAIR ? row & 63 : row)) * static_cast<int64_t>(kSsmState);
+    // the slab's columns in the rows of x, z and y (a lone head's twice: the copy is not stored)
+    const int xc0 = h0 * p.head_size, xc1 = lone ? xc0 : xc0 + 64;
 
     if (nch == 0) {
         // An empty sequence keeps its state (or starts at zero).
@@ -193,25 +286,31 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     }
     if (warp == 0) {
         if (lane == 0) {
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kStages; ++i) {
                 mbar_init(bar(bars.full[i]), 1);
                 mbar_init(bar(bars.empty[i]), 1);
-                mbar_init(bar(bars.zfull[i]), 1);
+            }
+            for (int i = 0; i < kGateStages; ++i) {
                 mbar_init(bar(bars.gates[i]), kHeads);
                 mbar_init(bar(bars.ydone[i]), 4);
-                mbar_init(bar(bars.cs[i]), 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(bar(bars.zfull[i]), 1);
+                mbar_init(bar(bars.yst[i]), 4);
+                mbar_init(bar(bars.yfree[i]), 1);
+                mbar_init(bar(bars.mx[i]), 1);
+                mbar_init(bar(bars.mready[i]), kMWarps);
             }
             mbar_init(bar(bars.g), 1);
             mbar_init(bar(bars.mread), kMWarps);
-            mbar_init(bar(bars.mready), kMWarps);
-            mbar_init(bar(bars.mx), 1);
             mbar_init(bar(bars.s), 1);
-            mbar_init(bar(bars.sready), 4);
-            mbar_init(bar(bars.split), kSplitWarps);
+            mbar_init(bar(bars.update), kUpdateWarps);
             mbar_init(bar(bars.yread), 4);
-            mbar_init(bar(bars.yst), 4);
-            mbar_init(bar(bars.yfree), 4);
-            abort_flag = 0;
+            mbar_init(bar(bars.last), 1);
+            WaitControl *ctl = wait_control();
+            ctl->limit = args.wait_ns;
+            ctl->status = p.status;
+            ctl->abort = 0;
             fence_mbar_init();
         }
         __syncwarp();
@@ -227,117 +326,113 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     tc_fence_after();
     const uint32_t tm = tmem_slot;
     auto gates_of = [&](int c, int head) -> Gates * {
-        return reinterpret_cast<Gates *>(sm + OFF_GATE + ((c & 1) * 2 + head) * GATE);
+        return reinterpret_cast<Gates *>(sm + OFF_GATE + ((c & (kGateStages - 1)) * 2 + head) * GATE);
     };
+    auto gates_full = [&](int c) { return wait.warp(bar(bars.gates[c & (kGateStages - 1)]), c / kGateStages, kSsmGates); };
 
     if (warp == 0) {
         // -------------------------------------------------------------- MMA issue
-        if (lane == 0) {
-            const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
-            const uint64_t dBk = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 16, 1024);     // K-major
-            const uint64_t dBm = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 8192, 1024);   // MN-major
-            const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
-            const uint64_t dW = smem_desc_sw128(sbase + OFF_WX, 8192, 1024);              // MN-major
-            const uint64_t dM = smem_desc_sw128(sbase + OFF_M, 16, 1024);                 // K-major
-            constexpr uint32_t kAtom = 8192 >> 4, kStep = 2048 >> 4, kSt = STAGE >> 4, kLo = kTile >> 4;
-            constexpr uint32_t id_g = idesc_bf16_f32(128, 64, false, false);
-            constexpr uint32_t id_s = idesc_bf16_f32(128, 128, true, true);
-            constexpr uint32_t id_m = idesc_bf16_f32(128, 64 * kHeads, true, false);
-            int ng = 0, nmx = 0, ncs = 0, ns = 0, nfree = 0;
-            bool ok = true;
-            uint32_t idle = 0;
-            uint64_t t_idle = 0;
-            while (ok && nfree < nch) {
-                bool progress = false;
-                // A barrier is looked at by the parity of its phase, so only while it cannot be
-                // two phases on: where the state update of a chunk is out (ns ahead), its
-                // inputs' barriers were seen then and may have moved on since.
-                // The state update (its stage has landed when G of the chunk is out):
-                if (ns < ng && mbar_test_wait(bar(bars.sready), ns & 1) && mbar_test_wait(bar(bars.split), ns & 1)) {
-                    tc_fence_after();
-                    const uint32_t st = (ns & 1) * kSt;
+        // The whole warp runs this loop, so that its control flow and the descriptors stay
+        // uniform; one elected lane issues.
+        const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
+        const uint64_t dBk = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 16, 1024);     // K-major
+        const uint64_t dBm = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 8192, 1024);   // MN-major
+        const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
+        const uint64_t dM = smem_desc_sw128(sbase + OFF_M, 16, 1024);                 // K-major
+        constexpr int kAtom = 8192 >> 4, kStep = 2048 >> 4, kSt = STAGE >> 4;
+        constexpr uint32_t id_g = idesc_bf16_f32(128, 64, false, false);
+        constexpr uint32_t id_s = idesc_bf16_f32(128, 128, false, true);
+        constexpr uint32_t id_m = idesc_bf16_f32(128, 64 * kHeads, true, false);
+        int ng = 0, nmx = 0, ns = 0;
+        auto scores = [&](int c) -> bool {      // G(c)
+            const uint32_t st = (c % kStages) * kSt;
+            if (!wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) return false;
+            if (c >= 1 && !wait.warp(bar(bars.mread), c - 1, kSsmM)) return false;
+            if (elect_one()) {
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_ss(tm + TM_S, dW + part * kLo + k * kStep, dBm + st + k * kStep, id_s, 1);
-                    mma_commit(bar(bars.s));
-                    ++ns;
-                    progress = true;
-                }
-                if (ncs < ng && (ncs < ns || mbar_test_wait(bar(bars.sready), ncs & 1)) &&
-                    (ncs == 0 || mbar_test_wait(bar(bars.yread), (ncs - 1) & 1))) {
-                    tc_fence_after();
-                    const uint32_t st = (ncs & 1) * kSt;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        mma_ts(tm + TM_YI, tm + TM_SB + (ncs & 1) * 64 + 8 * k, dC + st + (k >> 2) * kAtom + 2 * (k & 3),
-                               id_g, k > 0);
-                    mma_commit(bar(bars.cs[ncs & 1]));
-                    ++ncs;
-                    progress = true;
-                }
-                if (nmx < ng && mbar_test_wait(bar(bars.mready), nmx & 1) &&
-                    (nmx < ns || mbar_test_wait(bar(bars.split), nmx & 1)) &&
-                    (nmx == 0 || mbar_test_wait(bar(bars.yread), (nmx - 1) & 1))) {
-                    tc_fence_after();
-                    const uint32_t st = (nmx & 1) * kSt;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ss(tm + TM_YA, dX + st + k * kStep, dM + 2 * k, id_m, k > 0);
-                    mma_commit(bar(bars.mx));
-                    ++nmx;
-                    progress = true;
-                }
-                // G goes at most one chunk ahead of the slowest other product (the barriers
-                // of a chunk are looked at by parity)
-                if (ng < nch && ng <= nfree + 1 && mbar_test_wait(bar(bars.full[ng & 1]), (ng >> 1) & 1) &&
-                    (ng == 0 || mbar_test_wait(bar(bars.mread), (ng - 1) & 1))) {
-                    tc_fence_after();
-                    const uint32_t st = (ng & 1) * kSt;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        mma_ss(tm + TM_G, dC + st + (k >> 2) * kAtom + 2 * (k & 3), dBk + st + (k >> 2) * kAtom + 2 * (k & 3),
-                               id_g, k > 0);
-                    mma_commit(bar(bars.g));
-                    ++ng;
-                    progress = true;
-                }
-                if (nfree < ns && nfree < ncs && nfree < nmx) {
-                    mma_commit(bar(bars.empty[nfree & 1]));
-                    ++nfree;
-                }
-                if (progress) {
-                    idle = 0;
-                } else if ((++idle & 255u) == 0) {
-                    if (idle == 256) {
-                        t_idle = global_timer_ns();
-                    } else if (*wait.abort) {
-                        ok = false;
-                    } else if (global_timer_ns() - t_idle > wait.limit) {
-                        wait.give_up(kSsmIssue);
-                        ok = false;
-                    }
-                }
+                for (int k = 0; k < 8; ++k)
+                    mma_ss(tm + TM::G, dC + st + (k >> 2) * kAtom + 2 * (k & 3), dBk + st + (k >> 2) * kAtom + 2 * (k & 3),
+                           id_g, k > 0);
+                mma_commit(bar(bars.g));
             }
-            // No MMA or barrier arrive is in flight when the CTA leaves.
-            if (ng) wait.drain(bar(bars.g), (ng - 1) & 1, kSsmG);
-            for (int c = ncs > 2 ? ncs - 2 : 0; c < ncs; ++c) wait.drain(bar(bars.cs[c & 1]), (c >> 1) & 1, kSsmCS);
-            if (nmx) wait.drain(bar(bars.mx), (nmx - 1) & 1, kSsmMX);
-            if (ns) wait.drain(bar(bars.s), (ns - 1) & 1, kSsmS);
-            for (int c = nfree > 2 ? nfree - 2 : 0; c < nfree; ++c)
-                wait.drain(bar(bars.empty[c & 1]), (c >> 1) & 1, kSsmFree);
+            __syncwarp();
+            ++ng;
+            return true;
+        };
+        auto from_state = [&](int c) -> bool {  // Yi(c)
+            const uint32_t st = (c % kStages) * kSt;
+            if (c >= 1 && !wait.warp(bar(bars.yread), c - 1, kSsmRead)) return false;
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tm + TM::YI, tm + TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0) + 8 * k,
+                           dC + st + (k >> 2) * kAtom + 2 * (k & 3), id_g, k > 0);
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = scores(0);
+        for (int c = 0; ok && c < nch; ++c) {
+            const uint32_t st = (c % kStages) * kSt;
+            // (the state path's and the split's warps)
+            if (!(ok = wait.warp(bar(bars.update), c, kSsmUpdate))) break;
+            // (with one copy of bf16(S), Yi has to read it before the state path goes on)
+            if (TM::kCopies == 1 && !(ok = from_state(c))) break;
+            if (elect_one()) {                  // S += (w x)^T B: hi, then lo against the same B
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mma_ts(tm + TM::S, tm + TM::W + 8 * k, dBm + st + (k & 3) * kStep, id_s, 1);
+                mma_commit(bar(bars.s));
+            }
+            __syncwarp();
+            ++ns;
+            if (c + 1 < nch && !(ok = scores(c + 1))) break;
+            if (TM::kCopies == 2 && !(ok = from_state(c))) break;
+            if (!(ok = wait.warp(bar(bars.mready[c & (kMBuffers - 1)]), c / kMBuffers, kSsmM))) break;
+            if (elect_one()) {                  // Ya(c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mma_ss(tm + TM::YA, dX + st + k * kStep, dM + (PAIR ? 0 : (c & 1) * kAtom) + 2 * k, id_m, k > 0);
+                mma_commit(bar(bars.mx[c & (kMBuffers - 1)]));
+                mma_commit(bar(bars.empty[c % kStages]));   // (the chunk's last product)
+            }
+            __syncwarp();
+            ++nmx;
         }
+        // No MMA or barrier arrive is in flight when the CTA leaves (after a give-up some may
+        // have gone out without a commit of their own).
+        if (elect_one()) mma_commit(bar(bars.last));
         __syncwarp();
-    } else if (warp == 1) {
+        wait.drain(bar(bars.last), 0, kSsmIssue);
+        if (ng) wait.drain(bar(bars.g), ng - 1, kSsmG);
+        if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
+#pragma unroll 1
+        for (int c = nmx > kMBuffers ? nmx - kMBuffers : 0; c < nmx; ++c)
+            wait.drain(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX);
+#pragma unroll 1
+        for (int c = nmx > kStages ? nmx - kStages : 0; c < nmx; ++c)
+            wait.drain(bar(bars.empty[c % kStages]), c / kStages, kSsmFree);
+        __syncwarp();
+    } else if (warp == 18) {
         // -------------------------------------------------------------- copies
         if (lane == 0) {
-            const int xc0 = PAIR ? h0 * 64 : h0 * 128;
-            const int xc1 = lone ? xc0 : xc0 + 64;      // (a lone head twice: its copy is not stored)
+            auto token = [&](int c) { return static_cast<int>(s0 + static_cast<int64_t>(c) * kL); };
+            auto ahead = [&](int c) {
+                const int t = token(c);
+                tma_prefetch_2d(&cmap, g * 128, t);
+                tma_prefetch_2d(&cmap, g * 128 + 64, t);
+                tma_prefetch_2d(&bmap, g * 128, t);
+                tma_prefetch_2d(&bmap, g * 128 + 64, t);
+                tma_prefetch_2d(&xmap, xc0, t);
+                if (xc1 != xc0) tma_prefetch_2d(&xmap, xc1, t);
+                if (gated) {
+                    tma_prefetch_2d(&zmap, xc0, t);
+                    if (xc1 != xc0) tma_prefetch_2d(&zmap, xc1, t);
+                }
+            };
             int issued = 0, zissued = 0;
             for (int c = 0; c < nch; ++c) {
-                const int st = c & 1, t = static_cast<int>(s0 + static_cast<int64_t>(c) * kL);
-                if (c >= 2 && !wait.one(bar(bars.empty[st]), ((c - 2) >> 1) & 1, kSsmFree)) break;
+                const int st = c % kStages, t = token(c);
+                if (c >= kStages && !wait.one(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
                 const uint32_t base = sbase + OFF_STAGE + st * STAGE, b = bar(bars.full[st]);
                 mbar_arrive_expect_tx(b, STAGE);
                 tma_load_2d(base + ST_C, &cmap, b, g * 128, t);
@@ -347,69 +442,75 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 tma_load_2d(base + ST_X, &xmap, b, xc0, t);
                 tma_load_2d(base + ST_X + 8192, &xmap, b, xc1, t);
                 ++issued;
+                if (c + kPrefetch < nch) ahead(c + kPrefetch);
                 if (gated) {
-                    if (c >= 2 && !wait.one(bar(bars.ydone[st]), ((c - 2) >> 1) & 1, kSsmY)) break;
-                    const uint32_t zb = bar(bars.zfull[st]);
+                    // (into the staging rows that the stores two chunks before have read)
+                    if (c >= 2 && !wait.one(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
+                    const uint32_t zb = bar(bars.zfull[c & 1]), dst = sbase + OFF_Y + (c & 1) * kTile;
                     mbar_arrive_expect_tx(zb, kTile);
-                    tma_load_2d(sbase + OFF_Z + st * kTile, &zmap, zb, xc0, t);
-                    tma_load_2d(sbase + OFF_Z + st * kTile + 8192, &zmap, zb, xc1, t);
+                    tma_load_2d(dst, &zmap, zb, xc0, t);
+                    tma_load_2d(dst + 8192, &zmap, zb, xc1, t);
                     ++zissued;
                 }
             }
-            for (int c = issued > 2 ? issued - 2 : 0; c < issued; ++c)
-                wait.drain(bar(bars.full[c & 1]), (c >> 1) & 1, kSsmTma);
+#pragma unroll 1
+            for (int c = issued > kStages ? issued - kStages : 0; c < issued; ++c)
+                wait.drain(bar(bars.full[c % kStages]), c / kStages, kSsmTma);
+#pragma unroll 1
             for (int c = zissued > 2 ? zissued - 2 : 0; c < zissued; ++c)
-                wait.drain(bar(bars.zfull[c & 1]), (c >> 1) & 1, kSsmZ);
+                wait.drain(bar(bars.zfull[c & 1]), c >> 1, kSsmZ);
         }
         __syncwarp();
-    } else if (warp < 2 + kHeads) {
-        // -------------------------------------------------------------- gates of one head
-        const int head = warp - 2;
+    } else if (warp == 2 || warp == 3) {
+        // -------------------------------------------------------------- gates
+        // a warp for each of two heads, or two taking the one head's chunks in turn
+        const int head = PAIR ? warp - 2 : 0;
+        constexpr int kTurn = PAIR ? 1 : 2;
         const int h = lone ? h0 : h0 + head;
         const float negA2 = -expf(load_scalar(p.A_log, h, p.param_dtype)) * 1.4426950408889634f;   // log2 decays
-        auto step_of = [&](int64_t t) { return t < s1 ? ssm_step(p, t, h) : 0.0f; };
-        float d0 = step_of(s0 + lane), d1 = step_of(s0 + 32 + lane);
-        for (int c = 0; c < nch; ++c) {
-            const float a0 = negA2 * d0, a1 = negA2 * d1;
-            // sums up to and including a token, and behind it, of each 32-token half: both
-            // directions are summed, none is a difference of long sums
-            float p0 = a0, p1 = a1, q0 = a0, q1 = a1;
+        const float bias = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
+        auto raw = [&](int64_t t) { return t < s1 ? load_scalar(p.dt, t * p.dt_stride + h, p.dt_dtype) : 0.0f; };
+        // a lane holds tokens 2 lane and 2 lane + 1
+        const int c0 = PAIR ? 0 : warp - 2;
+        float r0 = raw(s0 + c0 * kL + 2 * lane), r1 = raw(s0 + c0 * kL + 2 * lane + 1);
+        for (int c = c0; c < nch; c += kTurn) {
+            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL + 2 * lane;
+            const float d0 = t0 < s1 ? softplus_series(r0 + bias) : 0.0f;
+            const float d1 = t0 + 1 < s1 ? softplus_series(r1 + bias) : 0.0f;
+            r0 = raw(t0 + kTurn * kL);        // (the next chunk's, in flight meanwhile)
+            r1 = raw(t0 + kTurn * kL + 1);
+            // The sums up to and including a token, and those behind it, are both summed:
+            // neither is a difference of long sums.
+            // (a decay below 2^-150 is zero in fp32; without the bound one such token would cost
+            // the sums behind it their precision)
+            const float a0 = fmaxf(negA2 * d0, -160.0f), a1 = fmaxf(negA2 * d1, -160.0f);
+            float up = a0 + a1, down = up;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {
-                const float u0 = __shfl_up_sync(0xffffffffu, p0, m), u1 = __shfl_up_sync(0xffffffffu, p1, m);
-                const float v0 = __shfl_down_sync(0xffffffffu, q0, m), v1 = __shfl_down_sync(0xffffffffu, q1, m);
-                if (lane >= m) {
-                    p0 += u0;
-                    p1 += u1;
-                }
-                if (lane + m < 32) {
-                    q0 += v0;
-                    q1 += v1;
-                }
+                const float u = __shfl_up_sync(0xffffffffu, up, m), v = __shfl_down_sync(0xffffffffu, down, m);
+                up += lane >= m ? u : 0.0f;
+                down += lane + m < 32 ? v : 0.0f;
             }
-            const float t0 = __shfl_sync(0xffffffffu, p0, 31), t1 = __shfl_sync(0xffffffffu, p1, 31);
-            q0 = __shfl_down_sync(0xffffffffu, q0, 1);
-            q1 = __shfl_down_sync(0xffffffffu, q1, 1);
-            if (lane == 31) q0 = q1 = 0.0f;
-            if (c >= 2 && !wait.warp(bar(bars.ydone[c & 1]), ((c - 2) >> 1) & 1, kSsmY)) break;
+            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+            before = lane > 0 ? before : 0.0f;
+            behind = lane < 31 ? behind : 0.0f;
+            const float l0 = before + a0, l1 = up;
+            // from a token to the end of its 8-token block
+            const float n1 = __shfl_down_sync(0xffffffffu, a0 + a1, 1, 4), n2 = __shfl_down_sync(0xffffffffu, a0 + a1, 2, 4),
+                        n3 = __shfl_down_sync(0xffffffffu, a0 + a1, 3, 4);
+            const int q = lane & 3;
+            const float rest = (q < 3 ? n1 : 0.0f) + (q < 2 ? n2 : 0.0f) + (q < 1 ? n3 : 0.0f);
+            if (c >= kGateStages &&
+                !wait.warp(bar(bars.ydone[c & (kGateStages - 1)]), c / kGateStages - 1, kSsmY)) break;
             Gates *o = gates_of(c, head);
-            o->la[lane] = p0;
-            o->la[lane + 32] = p1;
-            o->dt[lane] = d0;
-            o->dt[lane + 32] = d1;
-            o->e[lane] = exp2f(p0);
-            o->e[lane + 32] = exp2f(t0 + p1);
-            o->w[lane] = exp2f(q0 + t1) * d0;
-            o->w[lane + 32] = exp2f(q1) * d1;
-            o->cf[lane] = exp2f(q0) * d0;
-            o->rf[lane] = exp2f(p1);
-            if (lane == 0) o->total = exp2f(t0 + t1);
-            warp_arrive(bar(bars.gates[c & 1]), lane);
-            if (c + 1 < nch) {
-                const int64_t t = s0 + static_cast<int64_t>(c + 1) * kL + lane;
-                d0 = step_of(t);
-                d1 = step_of(t + 32);
-            }
+            auto put = [&](float *to, float v0, float v1) { reinterpret_cast<float2 *>(to)[lane] = make_float2(v0, v1); };
+            put(o->la, l0, l1);
+            put(o->lb, l0 - __log2f(d0), l1 - __log2f(d1));
+            put(o->cf, ex2(rest + a1) * d0, ex2(rest) * d1);
+            put(o->e, ex2(l0), ex2(l1));
+            split2_bf16(ex2(behind + a1) * d0, ex2(behind) * d1, o->wh[lane], o->wl[lane]);
+            if (lane == 31) o->total = ex2(l1);
+            warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
         }
     } else if (warp >= 4 && warp < 8) {
         // -------------------------------------------------------------- state path
@@ -423,42 +524,51 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 r[j] = __float_as_uint(x.x); r[j + 1] = __float_as_uint(x.y);
                 r[j + 2] = __float_as_uint(x.z); r[j + 3] = __float_as_uint(x.w);
             }
-            tmem_st32(tmem_addr(tm, lane_base, TM_S + 32 * q), r);
+            tmem_st32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
         }
         tmem_wait_st();
         bool ok = true;
         for (int c = 0; c < nch; ++c) {
-            if (!(ok = wait.warp(bar(bars.gates[c & 1]), (c >> 1) & 1, kSsmGates))) break;
+            if (!(ok = gates_full(c))) break;
             const float decay = gates_of(c, hrow)->total;
-            if (c >= 2 && !(ok = wait.warp(bar(bars.cs[c & 1]), ((c - 2) >> 1) & 1, kSsmCS))) break;
-            if (c >= 1 && !(ok = wait.warp(bar(bars.s), (c - 1) & 1, kSsmS))) break;
+            // the state is up to date, and so has Yi of two chunks before (of the one before,
+            // with one copy) read bf16(S): it went out earlier
+            if (c >= 1 && !(ok = wait.warp(bar(bars.s), c - 1, kSsmS))) break;
+            const uint32_t sb = TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0);
             const uint64_t d2 = f2(decay, decay);
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
-                uint32_t r[32], b[16];
-                tmem_ld32(tmem_addr(tm, lane_base, TM_S + 32 * q), r);
-                tmem_wait_ld_dep(r);
+            for (int q = 0; q < 4; q += 2) {
+                uint32_t r[2][32];
+                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r[0]);
+                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q + 32), r[1]);
+                tmem_wait_ld_dep(r[0]);
+                tmem_wait_ld_dep(r[1]);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                tmem_st16(tmem_addr(tm, lane_base, TM_SB + (c & 1) * 64 + 16 * q), b);
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t b[16];
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    float v0, v1;
-                    unf2(mul_f2(f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), d2), v0, v1);
-                    r[j] = __float_as_uint(v0);
-                    r[j + 1] = __float_as_uint(v1);
+                    for (int j = 0; j < 16; ++j)
+                        b[j] = pack_bf16x2(__uint_as_float(r[k][2 * j]), __uint_as_float(r[k][2 * j + 1]));
+                    tmem_st16(tmem_addr(tm, lane_base, sb + 16 * (q + k)), b);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float v0, v1;
+                        unf2(mul_f2(bits2(r[k][j], r[k][j + 1]), d2), v0, v1);
+                        r[k][j] = __float_as_uint(v0);
+                        r[k][j + 1] = __float_as_uint(v1);
+                    }
+                    tmem_st32(tmem_addr(tm, lane_base, TM::S + 32 * (q + k)), r[k]);
                 }
-                tmem_st32(tmem_addr(tm, lane_base, TM_S + 32 * q), r);
             }
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(bar(bars.sready), lane);
+            warp_arrive(bar(bars.update), lane);
         }
-        if (ok && wait.warp(bar(bars.s), (nch - 1) & 1, kSsmS)) {
+        if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS)) {
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
                 uint32_t r[32];
-                tmem_ld32(tmem_addr(tm, lane_base, TM_S + 32 * q), r);
+                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
                 tmem_wait_ld_dep(r);
                 if (!dead) {
 #pragma unroll
@@ -472,145 +582,170 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         }
     } else if (warp >= 8 && warp < 12) {
         // -------------------------------------------------------------- outputs
-        const int yw = warp - 8, l16 = lane & 15, half = lane >> 4;
-        const uint32_t ya = TM_YA + (PAIR ? hrow * 64 : 0);
-        uint16_t *so = reinterpret_cast<uint16_t *>(sm + OFF_Y);
-        auto *out = static_cast<__nv_bfloat16 *>(p.out) + static_cast<int64_t>(h0) * p.head_size + l16 * 8;
-        const bool stores = !lone || l16 < 8;
+        // A fragment's registers hold two neighbouring tokens of one state row; stmatrix
+        // writes eight rows' worth of them transposed, as 16 bytes of each token's row.
+        const uint32_t ya = TM::YA + (PAIR ? hrow * 64 : 0);
+        const int mi = lane >> 3, r8 = lane & 7, q2 = 2 * (lane & 3);
         for (int c = 0; c < nch; ++c) {
-            const int st = c & 1;
-            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
-            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
-            const float *e = gates_of(c, hrow)->e;
-            if (gated && !wait.warp(bar(bars.zfull[st]), (c >> 1) & 1, kSsmZ)) break;
-            if (!wait.warp(bar(bars.cs[c & 1]), (c >> 1) & 1, kSsmCS)) break;
-            if (!wait.warp(bar(bars.mx), c & 1, kSsmMX)) break;
-            // the stores of the chunk before have read the staging rows
-            if (c > 0 && !wait.warp(bar(bars.yfree), (c - 1) & 1, kSsmStage)) break;
-            const uint8_t *zt = sm + OFF_Z + st * kTile + (row >> 6) * 8192 + (row & 7) * 2;
-            const int zc = (row & 63) >> 3;
-#pragma unroll 1
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t yi[32], yo[32];
-                tmem_ld32(tmem_addr(tm, lane_base, TM_YI + 32 * hf), yi);
-                tmem_ld32(tmem_addr(tm, lane_base, ya + 32 * hf), yo);
+            const float *e = gates_of(c, hrow)->e + q2;
+            if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
+            // the stores two chunks before have read the staging rows (z's copy waited for them)
+            if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
+            if (!wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX)) break;      // (Yi went out before Ya)
+            const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
+#pragma unroll 2
+            for (int u = 0; u < 8; ++u) {          // 16 state rows x 16 tokens
+                const int lh = u & 1, h = u >> 1;
+                uint32_t yi[8], yo[8], zr[4], y[4];
+                tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, TM::YI + 16 * h), yi);
+                tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, ya + 16 * h), yo);
+                const int p0 = static_cast<int>(lane_base) + 16 * lh + 8 * (mi & 1);
+                const uint32_t to = tile + (p0 >> 6) * 8192 + sw128(16 * h + 8 * (mi >> 1) + r8, (p0 & 63) >> 3);
+                const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * h), eb = *reinterpret_cast<const float2 *>(e + 16 * h + 8);
+                if (gated) ldsm_x4_t(zr, to);
                 tmem_wait_ld_dep(yi);
                 tmem_wait_ld_dep(yo);
-                if (hf == 1) {
-                    tc_fence_before();
-                    warp_arrive(bar(bars.yread), lane);
-                }
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const int i = 32 * hf + j;
+                for (int k = 0; k < 4; ++k) {
                     float y0, y1;
-                    unf2(fma_f2(f2(__uint_as_float(yi[j]), __uint_as_float(yi[j + 1])), f2(e[i], e[i + 1]),
-                                f2(__uint_as_float(yo[j]), __uint_as_float(yo[j + 1]))), y0, y1);
+                    unf2(fma_f2(bits2(yi[2 * k], yi[2 * k + 1]), k < 2 ? f2(ea.x, ea.y) : f2(eb.x, eb.y),
+                                bits2(yo[2 * k], yo[2 * k + 1])), y0, y1);
                     if (gated) {
-                        y0 *= ssm_silu(__bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(zt + sw128(i, zc))));
-                        y1 *= ssm_silu(__bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(zt + sw128(i + 1, zc))));
+                        y0 *= ssm_silu(bf16_lo(zr[k]));
+                        y1 *= ssm_silu(bf16_hi(zr[k]));
                     }
-                    const uint32_t pk = pack_bf16x2(y0, y1);
-                    so[i * kRows + row] = static_cast<uint16_t>(pk);
-                    so[(i + 1) * kRows + row] = static_cast<uint16_t>(pk >> 16);
+                    y[k] = pack_bf16x2(y0, y1);
                 }
+                if (gated) __syncwarp();
+                stsm_x4_t(to, y);
             }
-            warp_arrive(bar(bars.ydone[st]), lane);     // (gates and z read)
-            warp_arrive(bar(bars.yst), lane);
-            if (!wait.warp(bar(bars.yst), c & 1, kSsmStage)) break;
-#pragma unroll 2
-            for (int u = 0; u < 8; ++u) {
-                const int i = 16 * yw + 2 * u + half;
-                const uint4 v = *reinterpret_cast<const uint4 *>(so + i * kRows + l16 * 8);
-                if (i < nt && stores)
-                    *reinterpret_cast<uint4 *>(out + (t0 + i) * p.heads * p.head_size) = v;
-            }
-            warp_arrive(bar(bars.yfree), lane);
-        }
-    } else if (warp == 12 || warp == 13 || warp == 17) {
-        // -------------------------------------------------------------- M
-        // warp 12: rows and columns 0..31; 13: rows 32..63, columns 0..31; 17: rows and
-        // columns 32..63.
-        const bool diag = warp != 13;
-        const int i = row, j0 = warp == 17 ? 32 : 0;
-        float D[kHeads];
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) D[k] = p.D ? load_scalar(p.D, lone ? h0 : h0 + k, p.param_dtype) : 0.0f;
-        for (int c = 0; c < nch; ++c) {
-            if (!wait.warp(bar(bars.gates[c & 1]), (c >> 1) & 1, kSsmGates)) break;
-            if (!wait.warp(bar(bars.g), c & 1, kSsmG)) break;
-            uint32_t r[32];
-            tmem_ld32(tmem_addr(tm, lane_base, TM_G + j0), r);
-            tmem_wait_ld_dep(r);
             tc_fence_before();
-            warp_arrive(bar(bars.mread), lane);
-            if (c >= 1 && !wait.warp(bar(bars.mx), (c - 1) & 1, kSsmMX)) break;
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k) {
-                const Gates *o = gates_of(c, k);
-                const float lai = o->la[i], rfi = o->rf[lane];
-                uint8_t *dst = sm + OFF_M + k * 8192;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t b[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = 8 * q + 2 * e;
-                        float v[2];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const float gv = __uint_as_float(r[j + u]);
-                            if (diag) {
-                                const float m = gv * (exp2f(lai - o->la[j0 + j + u]) * o->dt[j0 + j + u]);
-                                v[u] = j + u < lane ? m : (j + u == lane ? m + D[k] : 0.0f);
-                            } else {
-                                v[u] = gv * (rfi * o->cf[j + u]);
-                            }
-                        }
-                        b[e] = pack_bf16x2(v[0], v[1]);
-                    }
-                    *reinterpret_cast<uint4 *>(dst + sw128(i, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
-                }
-            }
+            warp_arrive(bar(bars.yread), lane);
+            warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
             fence_proxy_async_smem();
-            warp_arrive(bar(bars.mready), lane);
+            warp_arrive(bar(bars.yst[c & 1]), lane);
         }
-    } else if (warp == 14 || warp == 15 || warp == 18 || warp == 19) {
-        // -------------------------------------------------------------- w x, hi and lo
-        const int t = (warp < 16 ? warp - 14 : warp - 16) * 32 + lane;     // 0..127
+    } else if (warp == 19) {
+        // -------------------------------------------------------------- output rows
         for (int c = 0; c < nch; ++c) {
-            const int st = c & 1;
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
             const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
-            if (!wait.warp(bar(bars.gates[st]), (c >> 1) & 1, kSsmGates)) break;
-            if (!wait.warp(bar(bars.full[st]), (c >> 1) & 1, kSsmTma)) break;
-            if (c >= 1 && !wait.warp(bar(bars.s), (c - 1) & 1, kSsmS)) break;
-            uint8_t *xs = sm + OFF_STAGE + st * STAGE + ST_X, *bs = sm + OFF_STAGE + st * STAGE + ST_B;
-#pragma unroll 2
-            for (int u = 0; u < 8; ++u) {
-                const int at = u * 128 + t, j = (at >> 3) & 63;     // 16-byte word; atom at >> 9, token j
-                const float w = gates_of(c, PAIR ? at >> 9 : 0)->w[j];
-                uint32_t hi[4] = {}, lo[4] = {};
-                if (j < nt) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(xs + at * 16);
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                    const uint64_t w2 = f2(w, w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v0, v1;
-                        unf2(mul_f2(f2(bf16_lo(x[e]), bf16_hi(x[e])), w2), v0, v1);
-                        split2_bf16_f2(v0, v1, hi[e], lo[e]);
-                    }
-                } else {
-                    // rows behind the last token: other sequences' or none
-                    *reinterpret_cast<uint4 *>(xs + at * 16) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(bs + at * 16) = make_uint4(0, 0, 0, 0);
+            if (!wait.warp(bar(bars.yst[c & 1]), c >> 1, kSsmStage)) break;
+            const uint32_t off = OFF_Y + (c & 1) * kTile;
+            if (nt == kL) {
+                if (lane == 0) {
+                    tma_store_2d(&ymap, sbase + off, xc0, static_cast<int>(t0));
+                    if (!lone) tma_store_2d(&ymap, sbase + off + 8192, xc1, static_cast<int>(t0));
+                    bulk_commit();
+                    bulk_wait_read();
                 }
-                *reinterpret_cast<uint4 *>(sm + OFF_WX + at * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(sm + OFF_WX + kTile + at * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+                // the rows behind belong to the next sequence
+                const int l16 = lane & 15;
+                auto *out = static_cast<__nv_bfloat16 *>(p.out) + xc0 + l16 * 8;
+                for (int i = lane >> 4; i < nt; i += 2)
+                    if (!lone || l16 < 8)
+                        *reinterpret_cast<uint4 *>(out + (t0 + i) * p.heads * p.head_size) =
+                            *reinterpret_cast<const uint4 *>(sm + off + (l16 >> 3) * 8192 + sw128(i, l16 & 7));
             }
+            warp_arrive(bar(bars.yfree[c & 1]), lane);
+        }
+        if (lane == 0) bulk_wait_all();
+        __syncwarp();
+    } else if (warp == 16 || warp == 17 || warp == 1) {
+        // -------------------------------------------------------------- M
+        // warp 16: rows and columns 0..31; 17: rows 32..63, columns 0..31; 1: rows and
+        // columns 32..63.
+        const int j0 = warp == 1 ? 32 : 0;
+        const int reach = warp == 17 ? 31 : lane;          // last column of the row on or below the diagonal
+        const float D0 = p.D && warp != 17 ? load_scalar(p.D, h0, p.param_dtype) : 0.0f;
+        const float D1 = p.D && warp != 17 && PAIR && !lone ? load_scalar(p.D, h0 + 1, p.param_dtype) : D0;
+        const int block = warp == 17 ? 4 : lane >> 3;      // the 8 columns that hold the row's diagonal entry
+        for (int c = 0; c < nch; ++c) {
+            if (!gates_full(c)) break;
+            // the tile has been read by Ya two chunks before (one, with one buffer)
+            if (c >= kMBuffers &&
+                !wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers - 1, kSsmMX)) break;
+            if (!wait.warp(bar(bars.g), c, kSsmG)) break;
+#pragma unroll 1
+            for (int k = 0; k < kHeads; ++k) {
+                const Gates *o = gates_of(c, k);
+                uint8_t *dst = sm + OFF_M + (PAIR ? k : c & 1) * 8192;
+                const float lai = o->la[row];
+                float own[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) own[j] = ex2(lai - o->lb[(row & ~7) + j]);
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {              // 8 columns
+                    uint32_t r[8], b[4];
+                    tmem_ld8(tmem_addr(tm, lane_base, TM::G + j0 + 8 * q), r);
+                    const float4 *col = reinterpret_cast<const float4 *>(o->cf + j0 + 8 * q);
+                    const float4 v0 = col[0], v1 = col[1];
+                    const float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                    const float rf = ex2(lai - o->la[j0 + 8 * q + 7]);
+                    tmem_wait_ld_dep(r);
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        float m0, m1;
+                        unf2(mul_f2(bits2(r[j], r[j + 1]), f2(q == block ? own[j] : rf * f[j], q == block ? own[j + 1] : rf * f[j + 1])),
+                             m0, m1);
+                        if (8 * q + j == lane) m0 += k ? D1 : D0;
+                        if (8 * q + j + 1 == lane) m1 += k ? D1 : D0;
+                        b[j / 2] = pack_bf16x2(8 * q + j <= reach ? m0 : 0.0f, 8 * q + j + 1 <= reach ? m1 : 0.0f);
+                    }
+                    *reinterpret_cast<uint4 *>(dst + sw128(row, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
+                }
+            }
+            tc_fence_before();
+            warp_arrive(bar(bars.mread), lane);
             fence_proxy_async_smem();
-            warp_arrive(bar(bars.split), lane);
+            warp_arrive(bar(bars.mready[c & (kMBuffers - 1)]), lane);
+        }
+    } else if (warp >= 12 && warp < 16) {
+        // -------------------------------------------------------------- w x, hi and lo
+        // ldmatrix.trans reads the x tile [token][row] as fragments [row][token pair], the
+        // layout of the TMEM operand's 32-bit columns.
+        const int mi = lane >> 3, r8 = lane & 7, q1 = lane & 3;
+        for (int c = 0; c < nch; ++c) {
+            const int st = c % kStages;
+            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
+            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
+            if (!gates_full(c)) break;
+            if (!wait.warp(bar(bars.full[st]), c / kStages, kSsmTma)) break;
+            if (c >= 1 && !wait.warp(bar(bars.s), c - 1, kSsmS)) break;
+            const uint32_t xs = sbase + OFF_STAGE + st * STAGE + ST_X;
+            const Gates *o = gates_of(c, hrow);
+            if (nt < kL) {
+                // Rows behind the last token, which may hold anything: zero in this warp's 32
+                // columns of x and of B.
+                uint8_t *bt = sm + OFF_STAGE + st * STAGE + ST_B + (warp >> 1 & 1) * 8192;
+                for (int i = nt * 4 + lane; i < kL * 4; i += 32) {
+                    const uint32_t at = sw128(i >> 2, (warp & 1) * 4 + (i & 3));
+                    *reinterpret_cast<uint4 *>(bt + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(bt + (ST_X - ST_B) + at) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+#pragma unroll 1
+            for (int lh = 0; lh < 2; ++lh) {       // 16 state rows
+                const int p0 = static_cast<int>(lane_base) + 16 * lh + 8 * (mi & 1);
+                const uint32_t from = xs + (p0 >> 6) * 8192 + sw128(8 * (mi >> 1) + r8, (p0 & 63) >> 3);
+                uint32_t x[16], hi[16], lo[16];
+#pragma unroll
+                for (int gp = 0; gp < 4; ++gp) ldsm_x4_t(*reinterpret_cast<uint32_t(*)[4]>(x + 4 * gp), from + gp * 2048);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t wh = o->wh[4 * (k >> 1) + q1], wl = o->wl[4 * (k >> 1) + q1];
+                    hi[k] = mul_bf2(x[k], wh);
+                    lo[k] = fma_bf2(x[k], wl, fma_bf2(x[k], wh, hi[k] ^ 0x80008000u));
+                }
+                tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W), hi);
+                tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W + 32), lo);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(bar(bars.update), lane);
         }
     }
     tc_fence_before();
@@ -620,7 +755,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         tmem_dealloc(tm, 512);
     }
 }
-
 bool is_sm100() {
     int dev = 0, major = 0, minor = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -649,19 +783,19 @@ cudaError_t launch_ssm_prefill_tc(const SsmArgs &p, cudaStream_t stream) {
     const int64_t ctas = p.num_seqs * a.slabs;
     if (ctas == 0) return cudaSuccess;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    CUtensorMap maps[4];
+    CUtensorMap maps[5];
     std::memset(maps, 0, sizeof(maps));
     const int64_t wide = static_cast<int64_t>(p.heads) * p.head_size, bc = static_cast<int64_t>(p.groups) * kSsmState;
     if (!make_tmap_rows_bf16(&maps[0], p.x, p.rows, wide, p.x_stride) ||
         !make_tmap_rows_bf16(&maps[1], p.B, p.rows, bc, p.B_stride) ||
         !make_tmap_rows_bf16(&maps[2], p.C, p.rows, bc, p.C_stride) ||
-        (p.z && !make_tmap_rows_bf16(&maps[3], p.z, p.rows, wide, p.z_stride)))
+        (p.z && !make_tmap_rows_bf16(&maps[3], p.z, p.rows, wide, p.z_stride)) ||
+        !make_tmap_rows_bf16(&maps[4], p.out, p.rows, wide, wide))
         return cudaErrorInvalidValue;
     const auto kernel = pair ? ssm_tc_kernel<true> : ssm_tc_kernel<false>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_GATED);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES + sizeof(WaitControl));
     if (e != cudaSuccess) return e;
-    kernel<<<static_cast<unsigned>(ctas), kThreads, p.z ? SMEM_GATED : SMEM_PLAIN, stream>>>(maps[0], maps[1], maps[2],
-                                                                                             maps[3], a);
+    kernel<<<static_cast<unsigned>(ctas), kThreads, SMEM_BYTES + sizeof(WaitControl), stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
     return cudaGetLastError();
 }
 

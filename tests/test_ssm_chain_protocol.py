@@ -16,120 +16,133 @@ Q4 = range(4)
 M_WARPS, SPLIT_WARPS = 3, 4
 
 
+STAGES, GATE_STAGES = 3, 4
+
+
 def counts(heads):
-    one = dict(g=1, mread=M_WARPS, mready=M_WARPS, mx=1, s=1, sready=4, split=SPLIT_WARPS, yread=4, yst=4, yfree=4)
-    two = dict(full=1, empty=1, zfull=1, gates=heads, ydone=4, cs=1)
-    return {**one, **{f"{k}{i}": v for k, v in two.items() for i in (0, 1)}}
+    c = dict(g=1, mread=M_WARPS, s=1, update=4 + SPLIT_WARPS, yread=4, last=1)
+    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, 4),
+                    ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, 4), ("yfree", 2, 1)):
+        c.update({f"{k}{i}": v for i in range(n)})
+    return c
 
 
 class Scan(Sim):
     def __init__(self, nch, heads, gated, plant=None):
         super().__init__(nch, plant)
-        self.heads, self.gated = heads, gated
+        self.heads, self.gated, self.copies_of_s, self.m_buffers = heads, gated, 3 - heads, 3 - heads
         self.b = {k: Bar(k, v) for k, v in counts(heads).items()}
 
 
 def issuer(sim):
-    who, nch = "issuer", sim.nch
-    ng = nmx = ncs = ns = nfree = 0
+    nch, ok = sim.nch, True
+    issued = dict(g=0, s=0, mx=0)
 
-    def seen(bar, k):
-        return sim.b[bar].test(k, who)
+    def scores(c):
+        if not (yield ("wait", f"full{c % STAGES}", c // STAGES)):
+            return False
+        if c >= 1 and sim.plant != "no_mread" and not (yield ("wait", "mread", c - 1)):
+            return False
+        sim.mma({("C", c % STAGES): c, ("B", c % STAGES): c}, {("G",): (None, c)}, f"G({c})")
+        sim.commit("g")
+        issued["g"] += 1
+        return True
 
-    while nfree < nch:
-        sim.progress = False
-        if ns < ng and seen("sready", ns) and seen("split", ns):
-            sim.mma({("B", ns & 1): ns, **{("WX", w): ns for w in range(SPLIT_WARPS)}},
-                    {("S", q): (("dec", ns), ("S", ns + 1)) for q in Q4}, f"S update({ns})")
-            sim.commit("s")
-            ns += 1
-            sim.progress = True
-        if (ncs < ng and (ncs < ns or seen("sready", ncs))
-                and (ncs == 0 or sim.plant == "no_yread" or seen("yread", ncs - 1))):
-            sim.mma({("C", ncs & 1): ncs, **{("SB", ncs & 1, q): ncs for q in Q4}},
-                    {("YI", q): (None, ncs) for q in Q4}, f"Yi({ncs})")
-            sim.commit(f"cs{ncs & 1}")
-            ncs += 1
-            sim.progress = True
-        if (nmx < ng and seen("mready", nmx) and (nmx < ns or seen("split", nmx))
-                and (nmx == 0 or seen("yread", nmx - 1))):
-            sim.mma({("X", nmx & 1): nmx, **{("M", w): nmx for w in range(M_WARPS)}},
-                    {("YA", q): (None, nmx) for q in Q4}, f"Ya({nmx})")
-            sim.commit("mx")
-            nmx += 1
-            sim.progress = True
-        if (ng < nch and ng <= nfree + 1 and seen(f"full{ng & 1}", ng >> 1)
-                and (ng == 0 or sim.plant == "no_mread" or seen("mread", ng - 1))):
-            sim.mma({("C", ng & 1): ng, ("B", ng & 1): ng}, {("G",): (None, ng)}, f"G({ng})")
-            sim.commit("g")
-            ng += 1
-            sim.progress = True
-        if nfree < min(ns, ncs, nmx):
-            sim.commit(f"empty{nfree & 1}")
-            nfree += 1
-            sim.progress = True
-        if not sim.progress and sim.abort:
+    def from_state(c):
+        if c >= 1 and sim.plant != "no_yread" and not (yield ("wait", "yread", c - 1)):
+            return False
+        sim.mma({("C", c % STAGES): c, **{("SB", c % sim.copies_of_s, q): c for q in Q4}},
+                {("YI", q): (None, c) for q in Q4}, f"Yi({c})")
+        return True
+
+    ok = yield from scores(0)
+    for c in range(nch):
+        if not ok or not (ok := (yield ("wait", "update", c))):
             break
+        if sim.copies_of_s == 1 and sim.plant != "late_yi" and not (ok := (yield from from_state(c))):
+            break
+        sim.mma({("B", c % STAGES): c, **{("W", q): c for q in Q4}},
+                {("S", q): (("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
+        sim.commit("s")
+        issued["s"] += 1
+        if c + 1 < nch and not (ok := (yield from scores(c + 1))):
+            break
+        if (sim.copies_of_s == 2 or sim.plant == "late_yi") and not (ok := (yield from from_state(c))):
+            break
+        if not (ok := (yield ("wait", f"mready{c % sim.m_buffers}", c // sim.m_buffers))):
+            break
+        sim.mma({("X", c % STAGES): c, **{("M", c % sim.m_buffers, w): c for w in range(M_WARPS)}},
+                {("YA", q): (None, c) for q in Q4}, f"Ya({c})")
+        sim.commit(f"mx{c % sim.m_buffers}")
+        sim.commit(f"empty{c % STAGES}")
+        issued["mx"] += 1
         yield None
-    for bar, k in (("g", ng - 1), ("mx", nmx - 1), ("s", ns - 1)):
-        if k >= 0:
-            yield ("drain", bar, k)
-    for c in range(max(0, ncs - 2), ncs):
-        yield ("drain", f"cs{c & 1}", c >> 1)
-    for c in range(max(0, nfree - 2), nfree):
-        yield ("drain", f"empty{c & 1}", c >> 1)
+    for bar in ("g", "s"):
+        if issued[bar]:
+            yield ("drain", bar, issued[bar] - 1)
+    for c in range(max(0, issued["mx"] - sim.m_buffers), issued["mx"]):
+        yield ("drain", f"mx{c % sim.m_buffers}", c // sim.m_buffers)
+    sim.commit("last")
+    yield ("drain", "last", 0)
+    for c in range(max(0, issued["mx"] - STAGES), issued["mx"]):
+        yield ("drain", f"empty{c % STAGES}", c // STAGES)
 
 
 def copier(sim):
     issued = z = 0
     for c in range(sim.nch):
-        st = c & 1
-        if c >= 2 and sim.plant != "no_empty" and not (yield ("wait", f"empty{st}", (c - 2) >> 1)):
+        st = c % STAGES
+        if c >= STAGES and sim.plant != "no_empty" and not (yield ("wait", f"empty{st}", c // STAGES - 1)):
             break
         sim.copy([("C", st), ("B", st), ("X", st)], c, f"full{st}", "copier")
         issued += 1
         if sim.gated:
-            if c >= 2 and not (yield ("wait", f"ydone{st}", (c - 2) >> 1)):
+            if c >= 2 and sim.plant != "no_yfree" and not (yield ("wait", f"yfree{c & 1}", (c >> 1) - 1)):
                 break
-            sim.copy([("Z", st)], c, f"zfull{st}", "copier")
+            sim.copy([("ZY", c & 1, k) for k in Q4], ("z", c), f"zfull{c & 1}", "copier")
             z += 1
-    for c in range(max(0, issued - 2), issued):
-        yield ("drain", f"full{c & 1}", c >> 1)
+    for c in range(max(0, issued - STAGES), issued):
+        yield ("drain", f"full{c % STAGES}", c // STAGES)
     for c in range(max(0, z - 2), z):
         yield ("drain", f"zfull{c & 1}", c >> 1)
 
 
-def gates(sim, head):
-    for c in range(sim.nch):
-        if c >= 2 and not (yield ("wait", f"ydone{c & 1}", (c - 2) >> 1)):
+def gates(sim, w):
+    """A warp per head, or two taking one head's chunks in turn."""
+    head, turn = (w, 1) if sim.heads == 2 else (0, 2)
+    for c in range(0 if sim.heads == 2 else w, sim.nch, turn):
+        gs = c % GATE_STAGES
+        if c >= GATE_STAGES and not (yield ("wait", f"ydone{gs}", c // GATE_STAGES - 1)):
             return
-        sim.write(("GT", c & 1, head), c, f"gates{head}")
+        sim.write(("GT", gs, head), c, f"gates{w}")
         yield None
-        sim.b[f"gates{c & 1}"].arrive()
+        sim.b[f"gates{gs}"].arrive()
+
+
+def gates_full(c):
+    return ("wait", f"gates{c % GATE_STAGES}", c // GATE_STAGES)
 
 
 def read_gates(sim, c, who):
     for h in range(sim.heads):
-        sim.read(("GT", c & 1, h), c, who)
+        sim.read(("GT", c % GATE_STAGES, h), c, who)
 
 
 def state(sim, q):
     who, ok = f"state{q}", True
     sim.write(("S", q), ("S", 0), who)
     for c in range(sim.nch):
-        if not (ok := (yield ("wait", f"gates{c & 1}", c >> 1))):
+        if not (ok := (yield gates_full(c))):
             break
         read_gates(sim, c, who)
-        if c >= 2 and not (ok := (yield ("wait", f"cs{c & 1}", (c - 2) >> 1))):
-            break
         if c >= 1 and not (ok := (yield ("wait", "s", c - 1))):
             break
         sim.read(("S", q), ("S", c), who)
         yield None
-        sim.write(("SB", c & 1, q), c, who)
+        sim.write(("SB", c % sim.copies_of_s, q), c, who)
         sim.write(("S", q), ("dec", c), who)
         yield None
-        sim.b["sready"].arrive()
+        sim.b["update"].arrive()
     if ok and (yield ("wait", "s", sim.nch - 1)):
         sim.read(("S", q), ("S", sim.nch), who)
 
@@ -137,77 +150,82 @@ def state(sim, q):
 def outputs(sim, q):
     who = f"out{q}"
     for c in range(sim.nch):
-        st = c & 1
-        if sim.gated and not (yield ("wait", f"zfull{st}", c >> 1)):
+        if sim.gated and not (yield ("wait", f"zfull{c & 1}", c >> 1)):
             return
-        if not (yield ("wait", f"cs{st}", c >> 1)) or not (yield ("wait", "mx", c)):
+        if not (yield ("wait", f"mx{c % sim.m_buffers}", c // sim.m_buffers)):
             return
-        if c > 0 and sim.plant != "no_yfree" and not (yield ("wait", "yfree", c - 1)):
+        if not sim.gated and c >= 2 and sim.plant != "no_yfree" and not (yield ("wait", f"yfree{c & 1}", (c >> 1) - 1)):
             return
-        for half in (0, 1):
+        for part in range(4):
             sim.read(("YI", q), c, who)
             sim.read(("YA", q), c, who)
             read_gates(sim, c, who)
             yield None
-            if half == 1:
+            if part == 3:
                 sim.b["yread"].arrive()
-            if sim.gated:
-                sim.read(("Z", st), c, who)
-            sim.write(("STG", q), c, who)
+            if sim.gated and part == 0:
+                sim.read(("ZY", c & 1, q), ("z", c), who)
+            sim.write(("ZY", c & 1, q), c, who)
         yield None
-        sim.b[f"ydone{st}"].arrive()
-        sim.b["yst"].arrive()
-        if not (yield ("wait", "yst", c)):
+        sim.b[f"ydone{c % GATE_STAGES}"].arrive()
+        sim.b[f"yst{c & 1}"].arrive()
+
+
+def rows(sim):
+    """The output rows' stores (the bulk store's reads end before yfree)."""
+    for c in range(sim.nch):
+        if not (yield ("wait", f"yst{c & 1}", c >> 1)):
             return
         for _ in range(2):
             for k in Q4:
-                sim.read(("STG", k), c, who)
+                sim.read(("ZY", c & 1, k), c, "rows")
             yield None
-        sim.b["yfree"].arrive()
+        sim.b[f"yfree{c & 1}"].arrive()
 
 
 def scores(sim, w):
     who = f"m{w}"
     for c in range(sim.nch):
-        if not (yield ("wait", f"gates{c & 1}", c >> 1)) or not (yield ("wait", "g", c)):
+        if not (yield gates_full(c)) or not (yield ("wait", "g", c)):
             return
-        sim.read(("G",), c, who)
-        yield None
+        m = c % sim.m_buffers
+        if c >= sim.m_buffers and sim.plant != "no_mx" and not (yield ("wait", f"mx{m}", c // sim.m_buffers - 1)):
+            return
+        for _ in range(2):
+            sim.read(("G",), c, who)
+            read_gates(sim, c, who)
+            sim.write(("M", m, w), c, who)
+            yield None
         sim.b["mread"].arrive()
-        if c >= 1 and sim.plant != "no_mx" and not (yield ("wait", "mx", c - 1)):
-            return
-        read_gates(sim, c, who)
-        sim.write(("M", w), c, who)
-        yield None
-        sim.b["mready"].arrive()
+        sim.b[f"mready{m}"].arrive()
 
 
-def split(sim, w):
-    who = f"split{w}"
+def split(sim, q):
+    who = f"split{q}"
     for c in range(sim.nch):
-        st = c & 1
-        if not (yield ("wait", f"gates{st}", c >> 1)) or not (yield ("wait", f"full{st}", c >> 1)):
+        st = c % STAGES
+        if not (yield gates_full(c)) or not (yield ("wait", f"full{st}", c // STAGES)):
             return
-        if c >= 1 and not (yield ("wait", "s", c - 1)):
+        if c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
             return
         read_gates(sim, c, who)
         sim.read(("X", st), c, who)
         yield None
-        sim.write(("WX", w), c, who)
+        sim.write(("W", q), c, who)
         yield None
-        sim.b["split"].arrive()
+        sim.b["update"].arrive()
 
 
 def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=300000):
     sim = Scan(nch, heads, gated, plant)
     rng = random.Random(seed)
-    sim.progress, sim.timeouts = False, timeouts
     roles = {"issuer": issuer(sim), "copier": copier(sim)}
-    roles.update({f"gates{h}": gates(sim, h) for h in range(heads)})
+    roles.update({f"gates{w}": gates(sim, w) for w in (0, 1)})
     roles.update({f"state{q}": state(sim, q) for q in Q4})
     roles.update({f"out{q}": outputs(sim, q) for q in Q4})
     roles.update({f"m{w}": scores(sim, w) for w in range(M_WARPS)})
-    roles.update({f"split{w}": split(sim, w) for w in range(SPLIT_WARPS)})
+    roles.update({f"split{q}": split(sim, q) for q in Q4})
+    roles["rows"] = rows(sim)
     waiting, done = {}, set()
 
     def step(name, value=None):
@@ -221,7 +239,6 @@ def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=30
 
     for name in roles:
         step(name)
-    idle = 0
     for _ in range(max_steps):
         live = [n for n in roles if n not in done]
         if not live:
@@ -241,13 +258,8 @@ def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=30
         if sim.pipe:
             ready.append(("pipe", None))
         ready += [("copy", i) for i in range(len(sim.copies))]
-        # (the polling issuer is always ready; a schedule in which nothing else is and it
-        # makes no progress is a deadlock)
-        idle = idle + 1 if ready == [("issuer", None)] and not sim.progress else 0
-        if not ready or (idle > 3 and not timeouts):
+        if not ready:
             raise ProtocolError(f"deadlock: waiting {waiting}")
-        if idle > 50:
-            sim.abort = True        # the issuing thread's own limit
         name, val = ready[rng.randrange(len(ready))]
         if name == "pipe":
             sim.retire_pipe()
@@ -269,11 +281,11 @@ def test_random_schedules(nch, heads, gated):
         assert all(sim.tags[("S", q)] == ("S", nch) for q in Q4)
 
 
-@pytest.mark.parametrize("plant", ["no_yread", "no_mread", "no_empty", "no_yfree", "no_mx"])
+@pytest.mark.parametrize("plant", ["no_yread", "no_mread", "no_empty", "no_yfree", "no_mx", "no_s", "late_yi"])
 def test_planted_mistakes_are_caught(plant):
     with pytest.raises(ProtocolError):
         for seed in range(300):
-            run(5, seed, plant=plant)
+            run(5, seed, gated=plant != "no_empty", plant=plant)
 
 
 @pytest.mark.parametrize("nch", [1, 2, 3, 6])
@@ -286,7 +298,13 @@ def test_barrier_counts_match_the_kernel():
     src = open(KERNEL).read()
     consts = {k: int(v) for k, v in re.findall(r"\b(k\w+Warps) = (\d+)", src)}
     found = {}
-    for name, two, n in re.findall(r"mbar_init\(bar\(bars\.(\w+?)(\[i\])?\), (\w+)\)", src):
+    sizes = {k: int(v) for k, v in re.findall(r"constexpr int (k\w*Stages) = (\d+)", src)}
+    loop = None
+    for bound, name, many, n in re.findall(r"for \(int i = 0; i < (kStages|kGateStages|2); \+\+i\) \{|mbar_init\(bar\(bars\.(\w+?)(\[i\])?\), (\w+)\)",
+                                           src):
+        if bound:
+            loop = sizes.get(bound) or int(bound)
+            continue
         v = {"kHeads": 2}.get(n) or (int(n) if n.isdigit() else consts[n])
-        found.update({name + i: v for i in (("0", "1") if two else ("",))})
+        found.update({name + i: v for i in (map(str, range(loop)) if many else ("",))})
     assert found == counts(2)
