@@ -28,17 +28,17 @@
 // block; the 8 rows of the block itself take one exponential per element.  So a row of 32
 // columns takes 12 exponentials, and none overflows however strong the decays are.
 //
-// Roles (20 warps), handing chunks to each other through mbarriers:
-//   warp 0        allocates TMEM and issues the MMAs in a fixed order per chunk c: the state
-//                 update(c), G(c + 1), Yi(c), Ya(c)
+// Roles (25 of 28 warps), handing chunks to each other through mbarriers:
+//   warp 0        issues the state update(c), then G(c + 1); allocates TMEM
+//   warp 27       issues Yi(c), Ya(c) (one thread alone could not keep the tensor pipe busy)
 //   warp 18       copies (TMA): three stages of C, B and x, two of z, and boxes further ahead
 //                 into L2
 //   warps 2, 3    the chunk's gates: one head each, or one head's chunks in turn
 //   warps 4-7     state path: S -> bf16 copy (TMEM operand of Yi) and the decay of S
 //   warps 12-15   w x hi / lo into TMEM; the rows behind the last token set to zero
 //   warps 16, 17, 1   M, a 32 x 32 block each
-//   warps 8-11    outputs: Yi, Ya from TMEM as accumulator fragments, the gate z, transposed
-//                 into bf16 rows in shared memory (stmatrix)
+//   warps 8-11, 20-23   outputs, 32 tokens each: Yi, Ya from TMEM as accumulator fragments, the
+//                 gate z, transposed into bf16 rows in shared memory (stmatrix)
 //   warp 19       output rows to global memory (TMA; the last, partial chunk by hand)
 // The loops are kept rolled and the waits out of line: together they have to fit the SM's
 // instruction caches (with everything unrolled a chunk took 7,200 cycles, two thirds of the
@@ -64,12 +64,12 @@ using msync::ldsm_x4_t;
 using msync::stsm_x4_t;
 
 constexpr int kL = 64;              // tokens of a chunk
-constexpr int kThreads = 640;
+constexpr int kThreads = 896;
 constexpr int kRows = 128;          // state rows of a CTA
 constexpr int kStages = 3;          // of C, B, x
 constexpr int kGateStages = 4;
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
-constexpr int kMWarps = 3;
+constexpr int kMWarps = 3, kYWarps = 8;
 constexpr int kUpdateWarps = 8;      // of the state path and the split
 
 // Shared memory (bytes from the 1024-aligned base).  Tiles are 64 rows of 64 bf16 (one
@@ -90,7 +90,9 @@ struct alignas(16) Gates {
     float lb[64];         // la_j - log2(dt'_j): 2^(la_i - lb_j) = exp(la_i - la_j) dt'_j
     float cf[64];         // exp(la_r - la_j) dt'_j, r = j | 7
     float e[64];          // exp(la_i)
-    uint32_t wh[32], wl[32];   // w_j = exp(la_63 - la_j) dt'_j as bf16 hi + lo, two tokens a word
+    // w_j = exp(la_63 - la_j) dt'_j as bf16 hi + lo, two tokens a word, word (j / 2) % 4 of all
+    // 8-token blocks side by side: what one lane of a fragment needs
+    uint32_t wh[4][8], wl[4][8];
     float total;          // exp(la_63)
 };
 static_assert(sizeof(Gates) <= GATE, "gate block");
@@ -110,7 +112,7 @@ struct Tm {
 };
 
 enum WaitSite { kSsmTma = 41, kSsmZ = 42, kSsmGates = 43, kSsmG = 44, kSsmM = 45, kSsmS = 46,
-                kSsmMX = 48, kSsmUpdate = 47, kSsmIssue = 49, kSsmY = 50, kSsmStage = 51, kSsmFree = 52,
+                kSsmMX = 48, kSsmUpdate = 47, kSsmCS = 53, kSsmIssue = 49, kSsmY = 50, kSsmStage = 51, kSsmFree = 52,
                 kSsmRead = 54 };
 constexpr uint64_t kDrainNs = 2000000000ull;
 constexpr uint32_t kMaxSuspendNs = 1000000;
@@ -123,8 +125,8 @@ struct TcArgs {
 
 struct Bars {
     uint64_t full[kStages], empty[kStages], gates[kGateStages], ydone[kGateStages];
-    uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2];
-    uint64_t g, mread, s, update, yread, last;
+    uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2], update[2], last[2];
+    uint64_t g, mread, s, cs, yread;
 };
 
 // What a wait looks at besides its barrier, at the end of the dynamic shared memory.
@@ -288,25 +290,26 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         if (lane == 0) {
             for (int i = 0; i < kStages; ++i) {
                 mbar_init(bar(bars.full[i]), 1);
-                mbar_init(bar(bars.empty[i]), 1);
+                mbar_init(bar(bars.empty[i]), 2);
             }
             for (int i = 0; i < kGateStages; ++i) {
                 mbar_init(bar(bars.gates[i]), kHeads);
-                mbar_init(bar(bars.ydone[i]), 4);
+                mbar_init(bar(bars.ydone[i]), kYWarps);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(bar(bars.zfull[i]), 1);
-                mbar_init(bar(bars.yst[i]), 4);
+                mbar_init(bar(bars.yst[i]), kYWarps);
                 mbar_init(bar(bars.yfree[i]), 1);
                 mbar_init(bar(bars.mx[i]), 1);
                 mbar_init(bar(bars.mready[i]), kMWarps);
+                mbar_init(bar(bars.update[i]), kUpdateWarps);
+                mbar_init(bar(bars.last[i]), 1);
             }
             mbar_init(bar(bars.g), 1);
             mbar_init(bar(bars.mread), kMWarps);
             mbar_init(bar(bars.s), 1);
-            mbar_init(bar(bars.update), kUpdateWarps);
-            mbar_init(bar(bars.yread), 4);
-            mbar_init(bar(bars.last), 1);
+            mbar_init(bar(bars.cs), 1);
+            mbar_init(bar(bars.yread), kYWarps);
             WaitControl *ctl = wait_control();
             ctl->limit = args.wait_ns;
             ctl->status = p.status;
@@ -331,19 +334,16 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     auto gates_full = [&](int c) { return wait.warp(bar(bars.gates[c & (kGateStages - 1)]), c / kGateStages, kSsmGates); };
 
     if (warp == 0) {
-        // -------------------------------------------------------------- MMA issue
-        // The whole warp runs this loop, so that its control flow and the descriptors stay
+        // -------------------------------------------------------------- state update and G
+        // The whole warp runs the loop, so that its control flow and the descriptors stay
         // uniform; one elected lane issues.
         const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
         const uint64_t dBk = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 16, 1024);     // K-major
         const uint64_t dBm = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 8192, 1024);   // MN-major
-        const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
-        const uint64_t dM = smem_desc_sw128(sbase + OFF_M, 16, 1024);                 // K-major
         constexpr int kAtom = 8192 >> 4, kStep = 2048 >> 4, kSt = STAGE >> 4;
         constexpr uint32_t id_g = idesc_bf16_f32(128, 64, false, false);
         constexpr uint32_t id_s = idesc_bf16_f32(128, 128, false, true);
-        constexpr uint32_t id_m = idesc_bf16_f32(128, 64 * kHeads, true, false);
-        int ng = 0, nmx = 0, ns = 0;
+        int ng = 0, ns = 0;
         auto scores = [&](int c) -> bool {      // G(c)
             const uint32_t st = (c % kStages) * kSt;
             if (!wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) return false;
@@ -359,58 +359,68 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             ++ng;
             return true;
         };
-        auto from_state = [&](int c) -> bool {  // Yi(c)
-            const uint32_t st = (c % kStages) * kSt;
-            if (c >= 1 && !wait.warp(bar(bars.yread), c - 1, kSsmRead)) return false;
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_ts(tm + TM::YI, tm + TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0) + 8 * k,
-                           dC + st + (k >> 2) * kAtom + 2 * (k & 3), id_g, k > 0);
-            }
-            __syncwarp();
-            return true;
-        };
         bool ok = scores(0);
         for (int c = 0; ok && c < nch; ++c) {
             const uint32_t st = (c % kStages) * kSt;
             // (the state path's and the split's warps)
-            if (!(ok = wait.warp(bar(bars.update), c, kSsmUpdate))) break;
-            // (with one copy of bf16(S), Yi has to read it before the state path goes on)
-            if (TM::kCopies == 1 && !(ok = from_state(c))) break;
+            if (!(ok = wait.warp(bar(bars.update[c & 1]), c >> 1, kSsmUpdate))) break;
             if (elect_one()) {                  // S += (w x)^T B: hi, then lo against the same B
 #pragma unroll
                 for (int k = 0; k < 8; ++k) mma_ts(tm + TM::S, tm + TM::W + 8 * k, dBm + st + (k & 3) * kStep, id_s, 1);
                 mma_commit(bar(bars.s));
+                mma_commit(bar(bars.empty[c % kStages]));
             }
             __syncwarp();
             ++ns;
-            if (c + 1 < nch && !(ok = scores(c + 1))) break;
-            if (TM::kCopies == 2 && !(ok = from_state(c))) break;
-            if (!(ok = wait.warp(bar(bars.mready[c & (kMBuffers - 1)]), c / kMBuffers, kSsmM))) break;
-            if (elect_one()) {                  // Ya(c)
+            if (c + 1 < nch) ok = scores(c + 1);
+        }
+        // No MMA or barrier arrive is in flight when the CTA leaves (after a give-up some may
+        // have gone out without a commit of their own).
+        if (elect_one()) mma_commit(bar(bars.last[0]));
+        __syncwarp();
+        wait.drain(bar(bars.last[0]), 0, kSsmIssue);
+        if (ng) wait.drain(bar(bars.g), ng - 1, kSsmG);
+        if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
+        __syncwarp();
+    } else if (warp == 27) {
+        // -------------------------------------------------------------- Yi and Ya
+        const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
+        const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
+        const uint64_t dM = smem_desc_sw128(sbase + OFF_M, 16, 1024);                 // K-major
+        constexpr int kAtom = 8192 >> 4, kStep = 2048 >> 4, kSt = STAGE >> 4;
+        constexpr uint32_t id_y = idesc_bf16_f32(128, 64, false, false);
+        constexpr uint32_t id_m = idesc_bf16_f32(128, 64 * kHeads, true, false);
+        int nmx = 0;
+        for (int c = 0; c < nch; ++c) {
+            const uint32_t st = (c % kStages) * kSt;
+            if (!wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) break;
+            if (!wait.warp(bar(bars.update[c & 1]), c >> 1, kSsmUpdate)) break;       // (bf16(S) is there)
+            if (c >= 1 && !wait.warp(bar(bars.yread), c - 1, kSsmRead)) break;
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tm + TM::YI, tm + TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0) + 8 * k,
+                           dC + st + (k >> 2) * kAtom + 2 * (k & 3), id_y, k > 0);
+                if (TM::kCopies == 1) mma_commit(bar(bars.cs));
+            }
+            __syncwarp();
+            if (!wait.warp(bar(bars.mready[c & (kMBuffers - 1)]), c / kMBuffers, kSsmM)) break;
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     mma_ss(tm + TM::YA, dX + st + k * kStep, dM + (PAIR ? 0 : (c & 1) * kAtom) + 2 * k, id_m, k > 0);
                 mma_commit(bar(bars.mx[c & (kMBuffers - 1)]));
-                mma_commit(bar(bars.empty[c % kStages]));   // (the chunk's last product)
+                mma_commit(bar(bars.empty[c % kStages]));
             }
             __syncwarp();
             ++nmx;
         }
-        // No MMA or barrier arrive is in flight when the CTA leaves (after a give-up some may
-        // have gone out without a commit of their own).
-        if (elect_one()) mma_commit(bar(bars.last));
+        if (elect_one()) mma_commit(bar(bars.last[1]));
         __syncwarp();
-        wait.drain(bar(bars.last), 0, kSsmIssue);
-        if (ng) wait.drain(bar(bars.g), ng - 1, kSsmG);
-        if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
+        wait.drain(bar(bars.last[1]), 0, kSsmIssue);
 #pragma unroll 1
         for (int c = nmx > kMBuffers ? nmx - kMBuffers : 0; c < nmx; ++c)
             wait.drain(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX);
-#pragma unroll 1
-        for (int c = nmx > kStages ? nmx - kStages : 0; c < nmx; ++c)
-            wait.drain(bar(bars.empty[c % kStages]), c / kStages, kSsmFree);
         __syncwarp();
     } else if (warp == 18) {
         // -------------------------------------------------------------- copies
@@ -508,7 +518,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             put(o->lb, l0 - __log2f(d0), l1 - __log2f(d1));
             put(o->cf, ex2(rest + a1) * d0, ex2(rest) * d1);
             put(o->e, ex2(l0), ex2(l1));
-            split2_bf16(ex2(behind + a1) * d0, ex2(behind) * d1, o->wh[lane], o->wl[lane]);
+            split2_bf16(ex2(behind + a1) * d0, ex2(behind) * d1, o->wh[lane & 3][lane >> 2], o->wl[lane & 3][lane >> 2]);
             if (lane == 31) o->total = ex2(l1);
             warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
         }
@@ -531,38 +541,35 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         for (int c = 0; c < nch; ++c) {
             if (!(ok = gates_full(c))) break;
             const float decay = gates_of(c, hrow)->total;
-            // the state is up to date, and so has Yi of two chunks before (of the one before,
-            // with one copy) read bf16(S): it went out earlier
+            // Yi has read the copy (two chunks before, or one), the state is up to date
+            if (TM::kCopies == 2) {
+                if (c >= 2 && !(ok = wait.warp(bar(bars.mx[c & 1]), (c >> 1) - 1, kSsmMX))) break;
+            } else {
+                if (c >= 1 && !(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
+            }
             if (c >= 1 && !(ok = wait.warp(bar(bars.s), c - 1, kSsmS))) break;
             const uint32_t sb = TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0);
             const uint64_t d2 = f2(decay, decay);
 #pragma unroll 1
-            for (int q = 0; q < 4; q += 2) {
-                uint32_t r[2][32];
-                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r[0]);
-                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q + 32), r[1]);
-                tmem_wait_ld_dep(r[0]);
-                tmem_wait_ld_dep(r[1]);
+            for (int q = 0; q < 4; ++q) {
+                uint32_t r[32], b[16];
+                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
+                tmem_wait_ld_dep(r);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t b[16];
+                for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                tmem_st16(tmem_addr(tm, lane_base, sb + 16 * q), b);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        b[j] = pack_bf16x2(__uint_as_float(r[k][2 * j]), __uint_as_float(r[k][2 * j + 1]));
-                    tmem_st16(tmem_addr(tm, lane_base, sb + 16 * (q + k)), b);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float v0, v1;
-                        unf2(mul_f2(bits2(r[k][j], r[k][j + 1]), d2), v0, v1);
-                        r[k][j] = __float_as_uint(v0);
-                        r[k][j + 1] = __float_as_uint(v1);
-                    }
-                    tmem_st32(tmem_addr(tm, lane_base, TM::S + 32 * (q + k)), r[k]);
+                for (int j = 0; j < 32; j += 2) {
+                    float v0, v1;
+                    unf2(mul_f2(bits2(r[j], r[j + 1]), d2), v0, v1);
+                    r[j] = __float_as_uint(v0);
+                    r[j + 1] = __float_as_uint(v1);
                 }
+                tmem_st32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
             }
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(bar(bars.update), lane);
+            warp_arrive(bar(bars.update[c & 1]), lane);
         }
         if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS)) {
 #pragma unroll 1
@@ -580,7 +587,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 __syncwarp();
             }
         }
-    } else if (warp >= 8 && warp < 12) {
+    } else if ((warp >= 8 && warp < 12) || (warp >= 20 && warp < 24)) {
         // -------------------------------------------------------------- outputs
         // A fragment's registers hold two neighbouring tokens of one state row; stmatrix
         // writes eight rows' worth of them transposed, as 16 bytes of each token's row.
@@ -594,8 +601,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (!wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX)) break;      // (Yi went out before Ya)
             const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
 #pragma unroll 2
-            for (int u = 0; u < 8; ++u) {          // 16 state rows x 16 tokens
-                const int lh = u & 1, h = u >> 1;
+            for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
+                const int lh = u & 1, h = (u >> 1) + (warp >= 20 ? 2 : 0);
                 uint32_t yi[8], yo[8], zr[4], y[4];
                 tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, TM::YI + 16 * h), yi);
                 tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, ya + 16 * h), yo);
@@ -657,11 +664,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // warp 16: rows and columns 0..31; 17: rows 32..63, columns 0..31; 1: rows and
         // columns 32..63.
         const int j0 = warp == 1 ? 32 : 0;
-        const int reach = warp == 17 ? 31 : lane;          // last column of the row on or below the diagonal
+        const int block = (row - j0) >> 3;      // the 8 of its columns that hold the row's diagonal entry
         const float D0 = p.D && warp != 17 ? load_scalar(p.D, h0, p.param_dtype) : 0.0f;
         const float D1 = p.D && warp != 17 && PAIR && !lone ? load_scalar(p.D, h0 + 1, p.param_dtype) : D0;
-        const int block = warp == 17 ? 4 : lane >> 3;      // the 8 columns that hold the row's diagonal entry
         for (int c = 0; c < nch; ++c) {
+            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
+            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
             if (!gates_full(c)) break;
             // the tile has been read by Ya two chunks before (one, with one buffer)
             if (c >= kMBuffers &&
@@ -672,9 +680,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 const Gates *o = gates_of(c, k);
                 uint8_t *dst = sm + OFF_M + (PAIR ? k : c & 1) * 8192;
                 const float lai = o->la[row];
-                float own[8];
+                float own[8];                              // the diagonal block's factors, zero above it
 #pragma unroll
-                for (int j = 0; j < 8; ++j) own[j] = ex2(lai - o->lb[(row & ~7) + j]);
+                for (int j = 0; j < 8; ++j) own[j] = j <= (row & 7) ? ex2(lai - o->lb[(row & ~7) + j]) : 0.0f;
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {              // 8 columns
                     uint32_t r[8], b[4];
@@ -682,18 +690,25 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                     const float4 *col = reinterpret_cast<const float4 *>(o->cf + j0 + 8 * q);
                     const float4 v0 = col[0], v1 = col[1];
                     const float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                    const float rf = ex2(lai - o->la[j0 + 8 * q + 7]);
+                    const float rf = q < block ? ex2(lai - o->la[j0 + 8 * q + 7]) : 0.0f;
+                    const uint64_t rf2 = f2(rf, rf);
                     tmem_wait_ld_dep(r);
+                    if (nt < kL) {                         // scores with rows behind the last token: zero, not x 0
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) r[j] = j0 + 8 * q + j < nt ? r[j] : 0u;
+                    }
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        float m0, m1;
-                        unf2(mul_f2(bits2(r[j], r[j + 1]), f2(q == block ? own[j] : rf * f[j], q == block ? own[j + 1] : rf * f[j + 1])),
-                             m0, m1);
-                        if (8 * q + j == lane) m0 += k ? D1 : D0;
-                        if (8 * q + j + 1 == lane) m1 += k ? D1 : D0;
-                        b[j / 2] = pack_bf16x2(8 * q + j <= reach ? m0 : 0.0f, 8 * q + j + 1 <= reach ? m1 : 0.0f);
+                        float f0, f1, m0, m1;
+                        unf2(mul_f2(f2(f[j], f[j + 1]), rf2), f0, f1);
+                        unf2(mul_f2(bits2(r[j], r[j + 1]), f2(q == block ? own[j] : f0, q == block ? own[j + 1] : f1)), m0, m1);
+                        b[j / 2] = pack_bf16x2(m0, m1);
                     }
                     *reinterpret_cast<uint4 *>(dst + sw128(row, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
+                }
+                if (warp != 17) {                          // D on the diagonal: onto the rounded entry, rounded again
+                    auto *d = reinterpret_cast<__nv_bfloat16 *>(dst + sw128(row, row >> 3) + (row & 7) * 2);
+                    *d = __float2bfloat16_rn(__bfloat162float(*d) + (k ? D1 : D0));
                 }
             }
             tc_fence_before();
@@ -714,7 +729,16 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (!wait.warp(bar(bars.full[st]), c / kStages, kSsmTma)) break;
             if (c >= 1 && !wait.warp(bar(bars.s), c - 1, kSsmS)) break;
             const uint32_t xs = sbase + OFF_STAGE + st * STAGE + ST_X;
-            const Gates *o = gates_of(c, hrow);
+            uint32_t wh[8], wl[8];
+            {
+                const Gates *o = gates_of(c, hrow);
+#pragma unroll
+                for (int k = 0; k < 8; k += 4) {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(&o->wh[q1][k]), b = *reinterpret_cast<const uint4 *>(&o->wl[q1][k]);
+                    wh[k] = a.x; wh[k + 1] = a.y; wh[k + 2] = a.z; wh[k + 3] = a.w;
+                    wl[k] = b.x; wl[k + 1] = b.y; wl[k + 2] = b.z; wl[k + 3] = b.w;
+                }
+            }
             if (nt < kL) {
                 // Rows behind the last token, which may hold anything: zero in this warp's 32
                 // columns of x and of B.
@@ -736,16 +760,15 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 for (int gp = 0; gp < 4; ++gp) ldsm_x4_t(*reinterpret_cast<uint32_t(*)[4]>(x + 4 * gp), from + gp * 2048);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const uint32_t wh = o->wh[4 * (k >> 1) + q1], wl = o->wl[4 * (k >> 1) + q1];
-                    hi[k] = mul_bf2(x[k], wh);
-                    lo[k] = fma_bf2(x[k], wl, fma_bf2(x[k], wh, hi[k] ^ 0x80008000u));
+                    hi[k] = mul_bf2(x[k], wh[k >> 1]);
+                    lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
                 }
                 tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W), hi);
                 tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W + 32), lo);
             }
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(bar(bars.update), lane);
+            warp_arrive(bar(bars.update[c & 1]), lane);
         }
     }
     tc_fence_before();

@@ -13,16 +13,16 @@ from test_tc_chain_protocol import Bar, ProtocolError, Sim
 
 KERNEL = os.path.join(os.path.dirname(__file__), "..", "fastaf_kernel_b200", "csrc", "gdn_ssm_tc.cu")
 Q4 = range(4)
-M_WARPS, SPLIT_WARPS = 3, 4
+M_WARPS, SPLIT_WARPS, Y_WARPS = 3, 4, 8
 
 
 STAGES, GATE_STAGES = 3, 4
 
 
 def counts(heads):
-    c = dict(g=1, mread=M_WARPS, s=1, update=4 + SPLIT_WARPS, yread=4, last=1)
-    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, 4),
-                    ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, 4), ("yfree", 2, 1)):
+    c = dict(g=1, mread=M_WARPS, s=1, cs=1, yread=Y_WARPS)
+    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, Y_WARPS),
+                    ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, Y_WARPS), ("yfree", 2, 1)):
         c.update({f"{k}{i}": v for i in range(n)})
     return c
 
@@ -34,9 +34,11 @@ class Scan(Sim):
         self.b = {k: Bar(k, v) for k, v in counts(heads).items()}
 
 
-def issuer(sim):
-    nch, ok = sim.nch, True
-    issued = dict(g=0, s=0, mx=0)
+# The tensor pipe is modelled in order over both issuing threads; a commit arrives when its own
+# thread's products are done, which in order is no later.
+def issue_state(sim):
+    """S update(c), then G(c + 1)."""
+    nch, ng, ns = sim.nch, 0, 0
 
     def scores(c):
         if not (yield ("wait", f"full{c % STAGES}", c // STAGES)):
@@ -45,47 +47,54 @@ def issuer(sim):
             return False
         sim.mma({("C", c % STAGES): c, ("B", c % STAGES): c}, {("G",): (None, c)}, f"G({c})")
         sim.commit("g")
-        issued["g"] += 1
-        return True
-
-    def from_state(c):
-        if c >= 1 and sim.plant != "no_yread" and not (yield ("wait", "yread", c - 1)):
-            return False
-        sim.mma({("C", c % STAGES): c, **{("SB", c % sim.copies_of_s, q): c for q in Q4}},
-                {("YI", q): (None, c) for q in Q4}, f"Yi({c})")
         return True
 
     ok = yield from scores(0)
+    ng += ok
     for c in range(nch):
-        if not ok or not (ok := (yield ("wait", "update", c))):
-            break
-        if sim.copies_of_s == 1 and sim.plant != "late_yi" and not (ok := (yield from from_state(c))):
+        if not ok or not (yield ("wait", f"update{c & 1}", c >> 1)):
             break
         sim.mma({("B", c % STAGES): c, **{("W", q): c for q in Q4}},
                 {("S", q): (("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
         sim.commit("s")
-        issued["s"] += 1
-        if c + 1 < nch and not (ok := (yield from scores(c + 1))):
+        sim.commit(f"empty{c % STAGES}")
+        ns += 1
+        yield None
+        if c + 1 < nch:
+            ok = yield from scores(c + 1)
+            ng += ok
+    sim.commit("last0")
+    yield ("drain", "last0", 0)
+    if ng:
+        yield ("drain", "g", ng - 1)
+    if ns:
+        yield ("drain", "s", ns - 1)
+
+
+def issue_outputs(sim):
+    """Yi(c), Ya(c)."""
+    nmx = 0
+    for c in range(sim.nch):
+        if not (yield ("wait", f"full{c % STAGES}", c // STAGES)) or not (yield ("wait", f"update{c & 1}", c >> 1)):
             break
-        if (sim.copies_of_s == 2 or sim.plant == "late_yi") and not (ok := (yield from from_state(c))):
+        if c >= 1 and sim.plant != "no_yread" and not (yield ("wait", "yread", c - 1)):
             break
-        if not (ok := (yield ("wait", f"mready{c % sim.m_buffers}", c // sim.m_buffers))):
+        sim.mma({("C", c % STAGES): c, **{("SB", c % sim.copies_of_s, q): c for q in Q4}},
+                {("YI", q): (None, c) for q in Q4}, f"Yi({c})")
+        if sim.copies_of_s == 1:
+            sim.commit("cs")
+        if not (yield ("wait", f"mready{c % sim.m_buffers}", c // sim.m_buffers)):
             break
         sim.mma({("X", c % STAGES): c, **{("M", c % sim.m_buffers, w): c for w in range(M_WARPS)}},
                 {("YA", q): (None, c) for q in Q4}, f"Ya({c})")
         sim.commit(f"mx{c % sim.m_buffers}")
         sim.commit(f"empty{c % STAGES}")
-        issued["mx"] += 1
+        nmx += 1
         yield None
-    for bar in ("g", "s"):
-        if issued[bar]:
-            yield ("drain", bar, issued[bar] - 1)
-    for c in range(max(0, issued["mx"] - sim.m_buffers), issued["mx"]):
+    sim.commit("last1")
+    yield ("drain", "last1", 0)
+    for c in range(max(0, nmx - sim.m_buffers), nmx):
         yield ("drain", f"mx{c % sim.m_buffers}", c // sim.m_buffers)
-    sim.commit("last")
-    yield ("drain", "last", 0)
-    for c in range(max(0, issued["mx"] - STAGES), issued["mx"]):
-        yield ("drain", f"empty{c % STAGES}", c // STAGES)
 
 
 def copier(sim):
@@ -99,7 +108,7 @@ def copier(sim):
         if sim.gated:
             if c >= 2 and sim.plant != "no_yfree" and not (yield ("wait", f"yfree{c & 1}", (c >> 1) - 1)):
                 break
-            sim.copy([("ZY", c & 1, k) for k in Q4], ("z", c), f"zfull{c & 1}", "copier")
+            sim.copy([("ZY", c & 1, k) for k in range(Y_WARPS)], ("z", c), f"zfull{c & 1}", "copier")
             z += 1
     for c in range(max(0, issued - STAGES), issued):
         yield ("drain", f"full{c % STAGES}", c // STAGES)
@@ -135,6 +144,13 @@ def state(sim, q):
         if not (ok := (yield gates_full(c))):
             break
         read_gates(sim, c, who)
+        if sim.plant == "late_copy":
+            pass
+        elif sim.copies_of_s == 2:
+            if c >= 2 and not (ok := (yield ("wait", f"mx{c & 1}", (c >> 1) - 1))):
+                break
+        elif c >= 1 and not (ok := (yield ("wait", "cs", c - 1))):
+            break
         if c >= 1 and not (ok := (yield ("wait", "s", c - 1))):
             break
         sim.read(("S", q), ("S", c), who)
@@ -142,13 +158,13 @@ def state(sim, q):
         sim.write(("SB", c % sim.copies_of_s, q), c, who)
         sim.write(("S", q), ("dec", c), who)
         yield None
-        sim.b["update"].arrive()
+        sim.b[f"update{c & 1}"].arrive()
     if ok and (yield ("wait", "s", sim.nch - 1)):
         sim.read(("S", q), ("S", sim.nch), who)
 
 
-def outputs(sim, q):
-    who = f"out{q}"
+def outputs(sim, w):
+    who, q = f"out{w}", w % 4
     for c in range(sim.nch):
         if sim.gated and not (yield ("wait", f"zfull{c & 1}", c >> 1)):
             return
@@ -164,8 +180,8 @@ def outputs(sim, q):
             if part == 3:
                 sim.b["yread"].arrive()
             if sim.gated and part == 0:
-                sim.read(("ZY", c & 1, q), ("z", c), who)
-            sim.write(("ZY", c & 1, q), c, who)
+                sim.read(("ZY", c & 1, w), ("z", c), who)
+            sim.write(("ZY", c & 1, w), c, who)
         yield None
         sim.b[f"ydone{c % GATE_STAGES}"].arrive()
         sim.b[f"yst{c & 1}"].arrive()
@@ -177,7 +193,7 @@ def rows(sim):
         if not (yield ("wait", f"yst{c & 1}", c >> 1)):
             return
         for _ in range(2):
-            for k in Q4:
+            for k in range(Y_WARPS):
                 sim.read(("ZY", c & 1, k), c, "rows")
             yield None
         sim.b[f"yfree{c & 1}"].arrive()
@@ -213,16 +229,16 @@ def split(sim, q):
         yield None
         sim.write(("W", q), c, who)
         yield None
-        sim.b["update"].arrive()
+        sim.b[f"update{c & 1}"].arrive()
 
 
 def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=300000):
     sim = Scan(nch, heads, gated, plant)
     rng = random.Random(seed)
-    roles = {"issuer": issuer(sim), "copier": copier(sim)}
+    roles = {"state issue": issue_state(sim), "output issue": issue_outputs(sim), "copier": copier(sim)}
     roles.update({f"gates{w}": gates(sim, w) for w in (0, 1)})
     roles.update({f"state{q}": state(sim, q) for q in Q4})
-    roles.update({f"out{q}": outputs(sim, q) for q in Q4})
+    roles.update({f"out{w}": outputs(sim, w) for w in range(Y_WARPS)})
     roles.update({f"m{w}": scores(sim, w) for w in range(M_WARPS)})
     roles.update({f"split{q}": split(sim, q) for q in Q4})
     roles["rows"] = rows(sim)
@@ -281,7 +297,7 @@ def test_random_schedules(nch, heads, gated):
         assert all(sim.tags[("S", q)] == ("S", nch) for q in Q4)
 
 
-@pytest.mark.parametrize("plant", ["no_yread", "no_mread", "no_empty", "no_yfree", "no_mx", "no_s", "late_yi"])
+@pytest.mark.parametrize("plant", ["no_yread", "no_mread", "no_empty", "no_yfree", "no_mx", "no_s", "late_copy"])
 def test_planted_mistakes_are_caught(plant):
     with pytest.raises(ProtocolError):
         for seed in range(300):
