@@ -68,6 +68,7 @@ constexpr int kThreads = 896;
 constexpr int kRows = 128;          // state rows of a CTA
 constexpr int kStages = 3;          // of C, B, x
 constexpr int kGateStages = 4;
+constexpr int64_t kMinSegment = 512;    // tokens a sequence is cut into at least
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
 constexpr int kMWarps = 3, kYWarps = 8;
 constexpr int kUpdateWarps = 8;      // of the state path and the split
@@ -117,11 +118,37 @@ enum WaitSite { kSsmTma = 41, kSsmZ = 42, kSsmGates = 43, kSsmG = 44, kSsmM = 45
 constexpr uint64_t kDrainNs = 2000000000ull;
 constexpr uint32_t kMaxSuspendNs = 1000000;
 
+// Sequences may be cut into segments of `segment` tokens (a multiple of 64; as many as there
+// are, without cuts) that run side by side.  Segment j of sequence n has slot
+// cu_seqlens[n] / segment + n + j, so that the slots of different sequences are distinct
+// whatever their lengths; a first pass (LOCAL) leaves in `ends` what every segment but a
+// sequence's last adds to the state (the first one: the state behind it) and in `decays` its
+// decay, ssm_combine_kernel turns `ends` into the states behind the segments, and the main
+// pass starts every segment from the one in front of it.
 struct TcArgs {
     SsmArgs a;
-    int slabs, per_group;    // CTAs per sequence, per group
+    int slabs, per_group;    // CTAs per segment, per group
     uint64_t wait_ns;
+    int64_t segment;
+    float *ends;             // [slot][slab][128][128]
+    float *decays;           // [slot][slab][128], one per state row
 };
+
+// The tokens of sequence n, clamped to [0, T].
+__device__ __forceinline__ void sequence_of(const SsmArgs &p, int64_t n, int64_t &s0, int64_t &s1) {
+    s0 = p.cu_seqlens[n];
+    s1 = p.cu_seqlens[n + 1];
+    s0 = s0 < 0 ? 0 : (s0 > p.rows ? p.rows : s0);
+    s1 = s1 < s0 ? s0 : (s1 > p.rows ? p.rows : s1);
+}
+__device__ __forceinline__ int64_t first_slot(const TcArgs &a, int64_t n) {
+    int64_t s0 = a.a.cu_seqlens[n];
+    s0 = s0 < 0 ? 0 : (s0 > a.a.rows ? a.a.rows : s0);
+    return s0 / a.segment + n;
+}
+__device__ __forceinline__ int64_t segments_of(const TcArgs &a, int64_t tokens) {
+    return tokens > 0 ? (tokens + a.segment - 1) / a.segment : 1;
+}
 
 struct Bars {
     uint64_t full[kStages], empty[kStages], gates[kGateStages], ydone[kGateStages];
@@ -172,9 +199,6 @@ __device__ __noinline__ void wait_own(uint32_t bar, uint32_t key) {
 // look while phase k + 1 cannot be complete; tests/test_ssm_chain_protocol.py models it.
 struct Waiter {
     static __device__ __forceinline__ uint32_t key(uint32_t phase, int site) { return (phase & 1u) | (site << 1); }
-    __device__ __forceinline__ bool one(uint32_t bar, uint32_t phase, int site) const {
-        return mbar_try_wait(bar, phase & 1) || wait_slow(bar, key(phase, site));
-    }
     // The whole warp; it stays converged for the next .aligned tcgen05 instruction.
     __device__ __forceinline__ bool warp(uint32_t bar, uint32_t phase, int site) const {
         bool ok = mbar_try_wait(bar, phase & 1);
@@ -235,8 +259,8 @@ __device__ __forceinline__ float softplus_series(float x) {
     return fmaxf(x, 0.0f) + 2.0f * v;
 }
 
-// PAIR: two heads of 64 rows; else one head of 128.
-template <bool PAIR>
+// PAIR: two heads of 64 rows; else one head of 128.  LOCAL: the state path alone (see TcArgs).
+template <bool PAIR, bool LOCAL>
 __global__ void __launch_bounds__(kThreads, 1)
 ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap bmap,
               const __grid_constant__ CUtensorMap cmap, const __grid_constant__ CUtensorMap zmap,
@@ -247,24 +271,41 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     using TM = Tm<PAIR>;
     const SsmArgs &p = args.a;
     constexpr int kHeads = PAIR ? 2 : 1;
+    constexpr int kGateReaders = LOCAL ? kUpdateWarps : kYWarps;    // the last to read a chunk's gates
     constexpr int kMBuffers = PAIR ? 1 : 2;    // M tiles: one of both heads, or two of the one
 
     // (warp-uniform for the compiler too, so that the MMA warp's loop and descriptors are)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) * 32;
     const int row = static_cast<int>(lane_base) + lane;    // this thread's TMEM lane
-    const int64_t n = blockIdx.x / args.slabs;
+    const int64_t slot = blockIdx.x / args.slabs;
+    int64_t n = slot;
+    if (args.ends != nullptr) {
+        // the last sequence whose first slot is not behind this one
+        int64_t lo = 0, hi = p.num_seqs - 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (first_slot(args, mid) <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        n = lo;
+    }
     const int slab = static_cast<int>(blockIdx.x % args.slabs);
     const int g = slab / args.per_group, R = p.heads / p.groups;
     const int h0 = g * R + (slab % args.per_group) * kHeads;
     const bool lone = PAIR && (slab % args.per_group) * 2 + 1 >= R;   // a pair's second head is missing
-    const int64_t T = p.rows;
-    if (tid == 0 && slab == 0) check_seq_bounds(p.cu_seqlens, n, p.num_seqs, T, p.status);
-    int64_t s0 = p.cu_seqlens[n], s1 = p.cu_seqlens[n + 1];
-    s0 = s0 < 0 ? 0 : (s0 > T ? T : s0);
-    s1 = s1 < s0 ? s0 : (s1 > T ? T : s1);
+    // (there are at least as many slots as sequences)
+    if (!LOCAL && tid == 0 && slab == 0 && slot < p.num_seqs)
+        check_seq_bounds(p.cu_seqlens, slot, p.num_seqs, p.rows, p.status);
+    int64_t s0, s1;
+    sequence_of(p, n, s0, s1);
+    const int64_t segments = args.ends ? segments_of(args, s1 - s0) : 1, seg = args.ends ? slot - first_slot(args, n) : 0;
+    const bool last = seg == segments - 1;
+    if (seg < 0 || seg >= segments || (LOCAL && last)) return;      // (no such segment, or none needed)
+    s0 += seg * args.segment;
+    s1 = last ? s1 : s0 + args.segment;
     const int nch = static_cast<int>((s1 - s0 + kL - 1) / kL);
-    const bool gated = p.z != nullptr;
+    const bool gated = !LOCAL && p.z != nullptr;
     const uint32_t sbase = smem_u32(sm);
     auto bar = [&](const uint64_t &b) { return smem_u32(&b); };
     const Waiter wait;
@@ -274,6 +315,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     const bool dead = lone && hrow == 1;
     const int64_t state_at =
         ((n * p.heads + h0 + hrow) * p.head_size + (PAIR ? row & 63 : row)) * static_cast<int64_t>(kSsmState);
+    const int64_t end_at = (slot * args.slabs + slab) * kRows + row;      // the row in the segments' workspace
     // the slab's columns in the rows of x, z and y (a lone head's twice: the copy is not stored)
     const int xc0 = h0 * p.head_size, xc1 = lone ? xc0 : xc0 + 64;
 
@@ -294,7 +336,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             }
             for (int i = 0; i < kGateStages; ++i) {
                 mbar_init(bar(bars.gates[i]), kHeads);
-                mbar_init(bar(bars.ydone[i]), kYWarps);
+                mbar_init(bar(bars.ydone[i]), kGateReaders);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(bar(bars.zfull[i]), 1);
@@ -359,9 +401,11 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             ++ng;
             return true;
         };
-        bool ok = scores(0);
+        bool ok = LOCAL || scores(0);
+#pragma unroll 1
         for (int c = 0; ok && c < nch; ++c) {
             const uint32_t st = (c % kStages) * kSt;
+            if (LOCAL && !(ok = wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma))) break;
             // (the state path's and the split's warps)
             if (!(ok = wait.warp(bar(bars.update[c & 1]), c >> 1, kSsmUpdate))) break;
             if (elect_one()) {                  // S += (w x)^T B: hi, then lo against the same B
@@ -369,10 +413,11 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 for (int k = 0; k < 8; ++k) mma_ts(tm + TM::S, tm + TM::W + 8 * k, dBm + st + (k & 3) * kStep, id_s, 1);
                 mma_commit(bar(bars.s));
                 mma_commit(bar(bars.empty[c % kStages]));
+                if (LOCAL) mma_commit(bar(bars.empty[c % kStages]));   // (for the other issuing warp)
             }
             __syncwarp();
             ++ns;
-            if (c + 1 < nch) ok = scores(c + 1);
+            if (!LOCAL && c + 1 < nch) ok = scores(c + 1);
         }
         // No MMA or barrier arrive is in flight when the CTA leaves (after a give-up some may
         // have gone out without a commit of their own).
@@ -382,7 +427,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         if (ng) wait.drain(bar(bars.g), ng - 1, kSsmG);
         if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
         __syncwarp();
-    } else if (warp == 27) {
+    } else if (!LOCAL && warp == 27) {
         // -------------------------------------------------------------- Yi and Ya
         const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
         const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
@@ -391,6 +436,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         constexpr uint32_t id_y = idesc_bf16_f32(128, 64, false, false);
         constexpr uint32_t id_m = idesc_bf16_f32(128, 64 * kHeads, true, false);
         int nmx = 0;
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const uint32_t st = (c % kStages) * kSt;
             if (!wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) break;
@@ -424,52 +470,41 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         __syncwarp();
     } else if (warp == 18) {
         // -------------------------------------------------------------- copies
-        if (lane == 0) {
-            auto token = [&](int c) { return static_cast<int>(s0 + static_cast<int64_t>(c) * kL); };
-            auto ahead = [&](int c) {
-                const int t = token(c);
-                tma_prefetch_2d(&cmap, g * 128, t);
-                tma_prefetch_2d(&cmap, g * 128 + 64, t);
-                tma_prefetch_2d(&bmap, g * 128, t);
-                tma_prefetch_2d(&bmap, g * 128 + 64, t);
-                tma_prefetch_2d(&xmap, xc0, t);
-                if (xc1 != xc0) tma_prefetch_2d(&xmap, xc1, t);
-                if (gated) {
-                    tma_prefetch_2d(&zmap, xc0, t);
-                    if (xc1 != xc0) tma_prefetch_2d(&zmap, xc1, t);
-                }
-            };
-            int issued = 0, zissued = 0;
-            for (int c = 0; c < nch; ++c) {
-                const int st = c % kStages, t = token(c);
-                if (c >= kStages && !wait.one(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
-                const uint32_t base = sbase + OFF_STAGE + st * STAGE, b = bar(bars.full[st]);
-                mbar_arrive_expect_tx(b, STAGE);
-                tma_load_2d(base + ST_C, &cmap, b, g * 128, t);
-                tma_load_2d(base + ST_C + 8192, &cmap, b, g * 128 + 64, t);
-                tma_load_2d(base + ST_B, &bmap, b, g * 128, t);
-                tma_load_2d(base + ST_B + 8192, &bmap, b, g * 128 + 64, t);
-                tma_load_2d(base + ST_X, &xmap, b, xc0, t);
-                tma_load_2d(base + ST_X + 8192, &xmap, b, xc1, t);
-                ++issued;
-                if (c + kPrefetch < nch) ahead(c + kPrefetch);
-                if (gated) {
-                    // (into the staging rows that the stores two chunks before have read)
-                    if (c >= 2 && !wait.one(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
-                    const uint32_t zb = bar(bars.zfull[c & 1]), dst = sbase + OFF_Y + (c & 1) * kTile;
-                    mbar_arrive_expect_tx(zb, kTile);
-                    tma_load_2d(dst, &zmap, zb, xc0, t);
-                    tma_load_2d(dst + 8192, &zmap, zb, xc1, t);
-                    ++zissued;
-                }
+        // Lanes 0..7 take a box each -- C, B, x and z, two of 64 columns -- so that the loop holds
+        // one copy and one prefetch: fourteen of them in a row, fetched once a chunk, slowed
+        // every other role down.
+        const CUtensorMap *map = lane < 2 ? &cmap : lane < 4 ? &bmap : lane < 6 ? &xmap : &zmap;
+        const int x = lane < 4 ? g * 128 + (lane & 1) * 64 : (lane & 1) ? xc1 : xc0;
+        const bool staged = lane < 6 && !(LOCAL && lane < 2);
+        const bool fetched = lane < (gated ? 8 : 6) && !(LOCAL && lane < 2);
+        int issued = 0, zissued = 0;
+#pragma unroll 1
+ #pragma unroll 1
+       for (int c = 0; c < nch; ++c) {
+            const int t = static_cast<int>(s0) + c * kL;
+            const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
+            if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
+            if (lane == 0) mbar_arrive_expect_tx(b, LOCAL ? STAGE - kTile : STAGE);
+            __syncwarp();
+            if (staged) tma_load_2d(sbase + OFF_STAGE + st * STAGE + lane * 8192, map, b, x, t);
+            if (fetched && c + kPrefetch < nch) tma_prefetch_2d(map, x, t + kPrefetch * kL);
+            ++issued;
+            if (gated) {
+                // (into the staging rows that the stores two chunks before have read)
+                if (c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
+                const uint32_t zb = bar(bars.zfull[c & 1]);
+                if (lane == 0) mbar_arrive_expect_tx(zb, kTile);
+                __syncwarp();
+                if (lane == 6 || lane == 7) tma_load_2d(sbase + OFF_Y + (c & 1) * kTile + (lane - 6) * 8192, map, zb, x, t);
+                ++zissued;
             }
-#pragma unroll 1
-            for (int c = issued > kStages ? issued - kStages : 0; c < issued; ++c)
-                wait.drain(bar(bars.full[c % kStages]), c / kStages, kSsmTma);
-#pragma unroll 1
-            for (int c = zissued > 2 ? zissued - 2 : 0; c < zissued; ++c)
-                wait.drain(bar(bars.zfull[c & 1]), c >> 1, kSsmZ);
         }
+#pragma unroll 1
+        for (int c = issued > kStages ? issued - kStages : 0; c < issued; ++c)
+            wait.drain(bar(bars.full[c % kStages]), c / kStages, kSsmTma);
+#pragma unroll 1
+        for (int c = zissued > 2 ? zissued - 2 : 0; c < zissued; ++c)
+            wait.drain(bar(bars.zfull[c & 1]), c >> 1, kSsmZ);
         __syncwarp();
     } else if (warp == 2 || warp == 3) {
         // -------------------------------------------------------------- gates
@@ -483,6 +518,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // a lane holds tokens 2 lane and 2 lane + 1
         const int c0 = PAIR ? 0 : warp - 2;
         float r0 = raw(s0 + c0 * kL + 2 * lane), r1 = raw(s0 + c0 * kL + 2 * lane + 1);
+#pragma unroll 1
         for (int c = c0; c < nch; c += kTurn) {
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL + 2 * lane;
             const float d0 = t0 < s1 ? softplus_series(r0 + bias) : 0.0f;
@@ -524,13 +560,18 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         }
     } else if (warp >= 4 && warp < 8) {
         // -------------------------------------------------------------- state path
+        const float *first = seg == 0 ? (p.state && !dead ? p.state + state_at : nullptr)
+                             : LOCAL  ? nullptr
+                                      : args.ends + (end_at - static_cast<int64_t>(args.slabs) * kRows) * kSsmState;
+        float *const after = LOCAL ? args.ends + end_at * kSsmState : (last && !dead ? p.new_state + state_at : nullptr);
+        float product = 1.0f;           // of the segment's decays
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
             uint32_t r[32];
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
-                const float4 x = p.state && !dead ? *reinterpret_cast<const float4 *>(p.state + state_at + 32 * q + j)
-                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 x = first ? *reinterpret_cast<const float4 *>(first + 32 * q + j)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
                 r[j] = __float_as_uint(x.x); r[j + 1] = __float_as_uint(x.y);
                 r[j + 2] = __float_as_uint(x.z); r[j + 3] = __float_as_uint(x.w);
             }
@@ -538,15 +579,20 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         }
         tmem_wait_st();
         bool ok = true;
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             if (!(ok = gates_full(c))) break;
             const float decay = gates_of(c, hrow)->total;
-            // Yi has read the copy (two chunks before, or one), the state is up to date
-            if (TM::kCopies == 2) {
+            if (LOCAL) {
+                product *= decay;
+                warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
+            } else if (TM::kCopies == 2) {
+                // Yi of two chunks before has read the copy (of the one before, with one copy)
                 if (c >= 2 && !(ok = wait.warp(bar(bars.mx[c & 1]), (c >> 1) - 1, kSsmMX))) break;
             } else {
                 if (c >= 1 && !(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
             }
+            // the state is up to date
             if (c >= 1 && !(ok = wait.warp(bar(bars.s), c - 1, kSsmS))) break;
             const uint32_t sb = TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0);
             const uint64_t d2 = f2(decay, decay);
@@ -555,9 +601,11 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 uint32_t r[32], b[16];
                 tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
                 tmem_wait_ld_dep(r);
+                if (!LOCAL) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                tmem_st16(tmem_addr(tm, lane_base, sb + 16 * q), b);
+                    for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    tmem_st16(tmem_addr(tm, lane_base, sb + 16 * q), b);
+                }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     float v0, v1;
@@ -571,28 +619,30 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);
         }
+        if (LOCAL) args.decays[end_at] = product;
         if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS)) {
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
                 uint32_t r[32];
                 tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
                 tmem_wait_ld_dep(r);
-                if (!dead) {
+                if (after) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4 *>(p.new_state + state_at + 32 * q + j) =
+                        *reinterpret_cast<float4 *>(after + 32 * q + j) =
                             make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
                                         __uint_as_float(r[j + 3]));
                 }
                 __syncwarp();
             }
         }
-    } else if ((warp >= 8 && warp < 12) || (warp >= 20 && warp < 24)) {
+    } else if (!LOCAL && ((warp >= 8 && warp < 12) || (warp >= 20 && warp < 24))) {
         // -------------------------------------------------------------- outputs
         // A fragment's registers hold two neighbouring tokens of one state row; stmatrix
         // writes eight rows' worth of them transposed, as 16 bytes of each token's row.
         const uint32_t ya = TM::YA + (PAIR ? hrow * 64 : 0);
         const int mi = lane >> 3, r8 = lane & 7, q2 = 2 * (lane & 3);
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const float *e = gates_of(c, hrow)->e + q2;
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
@@ -632,17 +682,17 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             fence_proxy_async_smem();
             warp_arrive(bar(bars.yst[c & 1]), lane);
         }
-    } else if (warp == 19) {
+    } else if (!LOCAL && warp == 19) {
         // -------------------------------------------------------------- output rows
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
             const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
             if (!wait.warp(bar(bars.yst[c & 1]), c >> 1, kSsmStage)) break;
             const uint32_t off = OFF_Y + (c & 1) * kTile;
             if (nt == kL) {
-                if (lane == 0) {
-                    tma_store_2d(&ymap, sbase + off, xc0, static_cast<int>(t0));
-                    if (!lone) tma_store_2d(&ymap, sbase + off + 8192, xc1, static_cast<int>(t0));
+                if (lane < (lone ? 1 : 2)) {
+                    tma_store_2d(&ymap, sbase + off + lane * 8192, xc0 + lane * 64, static_cast<int>(t0));
                     bulk_commit();
                     bulk_wait_read();
                 }
@@ -650,6 +700,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 // the rows behind belong to the next sequence
                 const int l16 = lane & 15;
                 auto *out = static_cast<__nv_bfloat16 *>(p.out) + xc0 + l16 * 8;
+#pragma unroll 1
                 for (int i = lane >> 4; i < nt; i += 2)
                     if (!lone || l16 < 8)
                         *reinterpret_cast<uint4 *>(out + (t0 + i) * p.heads * p.head_size) =
@@ -657,9 +708,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             }
             warp_arrive(bar(bars.yfree[c & 1]), lane);
         }
-        if (lane == 0) bulk_wait_all();
+        if (lane < 2) bulk_wait_all();
         __syncwarp();
-    } else if (warp == 16 || warp == 17 || warp == 1) {
+    } else if (!LOCAL && (warp == 16 || warp == 17 || warp == 1)) {
         // -------------------------------------------------------------- M
         // warp 16: rows and columns 0..31; 17: rows 32..63, columns 0..31; 1: rows and
         // columns 32..63.
@@ -667,6 +718,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const int block = (row - j0) >> 3;      // the 8 of its columns that hold the row's diagonal entry
         const float D0 = p.D && warp != 17 ? load_scalar(p.D, h0, p.param_dtype) : 0.0f;
         const float D1 = p.D && warp != 17 && PAIR && !lone ? load_scalar(p.D, h0 + 1, p.param_dtype) : D0;
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
             const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
@@ -721,6 +773,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // ldmatrix.trans reads the x tile [token][row] as fragments [row][token pair], the
         // layout of the TMEM operand's 32-bit columns.
         const int mi = lane >> 3, r8 = lane & 7, q1 = lane & 3;
+#pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int st = c % kStages;
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
@@ -738,6 +791,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                     wh[k] = a.x; wh[k + 1] = a.y; wh[k + 2] = a.z; wh[k + 3] = a.w;
                     wl[k] = b.x; wl[k + 1] = b.y; wl[k + 2] = b.z; wl[k + 3] = b.w;
                 }
+                if (LOCAL) warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);
             }
             if (nt < kL) {
                 // Rows behind the last token, which may hold anything: zero in this warp's 32
@@ -778,6 +832,35 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         tmem_dealloc(tm, 512);
     }
 }
+// ends[slot of segment j] <- the state behind segment j, for all but a sequence's last: what
+// the segment added, plus the state in front of it times the segment's decay.  One thread per
+// four state elements; nothing to do for the first segment, whose local pass started from
+// the sequence's state.
+constexpr int kCombineThreads = 256, kCombineCtas = kRows * kSsmState / 4 / kCombineThreads;
+__global__ void __launch_bounds__(kCombineThreads) ssm_combine_kernel(const TcArgs args) {
+    const int64_t chain = blockIdx.x / kCombineCtas, n = chain / args.slabs;
+    const int slab = static_cast<int>(chain % args.slabs);
+    const int at = static_cast<int>(blockIdx.x % kCombineCtas) * kCombineThreads + threadIdx.x;   // float4 of the block
+    const int row = at / (kSsmState / 4);
+    int64_t s0, s1;
+    sequence_of(args.a, n, s0, s1);
+    const int64_t segments = segments_of(args, s1 - s0), slot = first_slot(args, n);
+    if (segments < 3) return;
+    auto block = [&](int64_t j) { return (slot + j) * args.slabs + slab; };
+    auto *ends = reinterpret_cast<float4 *>(args.ends);
+    constexpr int kVecs = kRows * kSsmState / 4;
+    float4 state = ends[block(0) * kVecs + at];
+    for (int64_t j = 1; j < segments - 1; ++j) {
+        float4 e = ends[block(j) * kVecs + at];
+        const float d = args.decays[block(j) * kRows + row];
+        e.x = fmaf(d, state.x, e.x);
+        e.y = fmaf(d, state.y, e.y);
+        e.z = fmaf(d, state.z, e.z);
+        e.w = fmaf(d, state.w, e.w);
+        ends[block(j) * kVecs + at] = state = e;
+    }
+}
+
 bool is_sm100() {
     int dev = 0, major = 0, minor = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -796,6 +879,53 @@ bool ssm_prefill_tc_supported(int64_t total_tokens) {
     return total_tokens >= kL && total_tokens < (int64_t(1) << 31) && is_sm100();
 }
 
+namespace {
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return sms;
+}
+
+template <bool PAIR, bool LOCAL>
+cudaError_t launch_pass(const CUtensorMap *maps, const TcArgs &a, int64_t slots, cudaStream_t stream) {
+    const auto kernel = ssm_tc_kernel<PAIR, LOCAL>;
+    const uint32_t smem = SMEM_BYTES + sizeof(WaitControl);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<static_cast<unsigned>(slots * a.slabs), kThreads, smem, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
+    return cudaGetLastError();
+}
+
+template <bool PAIR>
+cudaError_t launch_passes(const CUtensorMap *maps, const TcArgs &a, int64_t slots, cudaStream_t stream) {
+    if (a.ends != nullptr) {
+        cudaError_t e = launch_pass<PAIR, true>(maps, a, slots, stream);
+        if (e != cudaSuccess) return e;
+        ssm_combine_kernel<<<static_cast<unsigned>(a.a.num_seqs * a.slabs * kCombineCtas), kCombineThreads, 0, stream>>>(a);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    return launch_pass<PAIR, false>(maps, a, slots, stream);
+}
+
+// Tokens of a segment, or 0 for no cuts, of a call with `chains` (sequence, slab) pairs: as
+// many segments of a sequence of mean length as fill the SMs once, so that few long prompts
+// use all of them.  With more chains than half the SMs the local pass costs more than the
+// idle SMs.
+int64_t segment_tokens(int64_t tokens, int64_t num_seqs, int64_t chains, int sms) {
+    const int64_t cuts = sms / chains;
+    if (cuts < 2) return 0;
+    int64_t s = (tokens + num_seqs * cuts - 1) / (num_seqs * cuts);
+    s = (s + kL - 1) / kL * kL;
+    return s < kMinSegment ? kMinSegment : s;
+}
+
+}  // namespace
+
 cudaError_t launch_ssm_prefill_tc(const SsmArgs &p, cudaStream_t stream) {
     const bool pair = p.head_size == 64;
     const int R = p.heads / p.groups;
@@ -803,9 +933,13 @@ cudaError_t launch_ssm_prefill_tc(const SsmArgs &p, cudaStream_t stream) {
     a.per_group = pair ? (R + 1) / 2 : R;
     a.slabs = p.groups * a.per_group;
     a.wait_ns = wait_limit_ns();
-    const int64_t ctas = p.num_seqs * a.slabs;
-    if (ctas == 0) return cudaSuccess;
-    if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    const int64_t chains = p.num_seqs * a.slabs;
+    if (chains == 0) return cudaSuccess;
+    const int sms = sm_count();
+    a.segment = sms > 0 ? segment_tokens(p.rows, p.num_seqs, chains, sms) : 0;
+    const bool cut = a.segment > 0 && a.segment < p.rows;
+    const int64_t slots = cut ? p.rows / a.segment + p.num_seqs : p.num_seqs;
+    if (slots * a.slabs > 0x7fffffffLL || chains * kCombineCtas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     CUtensorMap maps[5];
     std::memset(maps, 0, sizeof(maps));
     const int64_t wide = static_cast<int64_t>(p.heads) * p.head_size, bc = static_cast<int64_t>(p.groups) * kSsmState;
@@ -815,11 +949,17 @@ cudaError_t launch_ssm_prefill_tc(const SsmArgs &p, cudaStream_t stream) {
         (p.z && !make_tmap_rows_bf16(&maps[3], p.z, p.rows, wide, p.z_stride)) ||
         !make_tmap_rows_bf16(&maps[4], p.out, p.rows, wide, wide))
         return cudaErrorInvalidValue;
-    const auto kernel = pair ? ssm_tc_kernel<true> : ssm_tc_kernel<false>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES + sizeof(WaitControl));
-    if (e != cudaSuccess) return e;
-    kernel<<<static_cast<unsigned>(ctas), kThreads, SMEM_BYTES + sizeof(WaitControl), stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
-    return cudaGetLastError();
+    cudaError_t e = cudaSuccess, ef = cudaSuccess;
+    if (cut) {
+        void *ws = nullptr;
+        const size_t blocks = static_cast<size_t>(slots) * a.slabs;
+        if ((e = pool_alloc(&ws, blocks * (kRows * kSsmState + kRows) * sizeof(float), stream)) != cudaSuccess) return e;
+        a.ends = static_cast<float *>(ws);
+        a.decays = a.ends + blocks * kRows * kSsmState;
+    }
+    e = pair ? launch_passes<true>(maps, a, slots, stream) : launch_passes<false>(maps, a, slots, stream);
+    if (cut) ef = cudaFreeAsync(a.ends, stream);
+    return e != cudaSuccess ? e : ef;
 }
 
 }  // namespace gdn

@@ -19,19 +19,20 @@ M_WARPS, SPLIT_WARPS, Y_WARPS = 3, 4, 8
 STAGES, GATE_STAGES = 3, 4
 
 
-def counts(heads):
+def counts(heads, local=False):
     c = dict(g=1, mread=M_WARPS, s=1, cs=1, yread=Y_WARPS)
-    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, Y_WARPS),
+    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, 4 + SPLIT_WARPS if local else Y_WARPS),
                     ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, Y_WARPS), ("yfree", 2, 1)):
         c.update({f"{k}{i}": v for i in range(n)})
     return c
 
 
 class Scan(Sim):
-    def __init__(self, nch, heads, gated, plant=None):
+    def __init__(self, nch, heads, gated, plant=None, local=False):
         super().__init__(nch, plant)
         self.heads, self.gated, self.copies_of_s, self.m_buffers = heads, gated, 3 - heads, 3 - heads
-        self.b = {k: Bar(k, v) for k, v in counts(heads).items()}
+        self.b = {k: Bar(k, v) for k, v in counts(heads, local).items()}
+        self.local = local     # the state path alone
 
 
 # The tensor pipe is modelled in order over both issuing threads; a commit arrives when its own
@@ -49,18 +50,21 @@ def issue_state(sim):
         sim.commit("g")
         return True
 
-    ok = yield from scores(0)
-    ng += ok
+    ok = sim.local or (yield from scores(0))
+    ng += ok and not sim.local
     for c in range(nch):
-        if not ok or not (yield ("wait", f"update{c & 1}", c >> 1)):
+        if not ok or (sim.local and not (yield ("wait", f"full{c % STAGES}", c // STAGES))):
+            break
+        if not (yield ("wait", f"update{c & 1}", c >> 1)):
             break
         sim.mma({("B", c % STAGES): c, **{("W", q): c for q in Q4}},
                 {("S", q): (("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
         sim.commit("s")
-        sim.commit(f"empty{c % STAGES}")
+        for _ in range(2 if sim.local else 1):
+            sim.commit(f"empty{c % STAGES}")
         ns += 1
         yield None
-        if c + 1 < nch:
+        if c + 1 < nch and not sim.local:
             ok = yield from scores(c + 1)
             ng += ok
     sim.commit("last0")
@@ -103,7 +107,7 @@ def copier(sim):
         st = c % STAGES
         if c >= STAGES and sim.plant != "no_empty" and not (yield ("wait", f"empty{st}", c // STAGES - 1)):
             break
-        sim.copy([("C", st), ("B", st), ("X", st)], c, f"full{st}", "copier")
+        sim.copy(([] if sim.local else [("C", st)]) + [("B", st), ("X", st)], c, f"full{st}", "copier")
         issued += 1
         if sim.gated:
             if c >= 2 and sim.plant != "no_yfree" and not (yield ("wait", f"yfree{c & 1}", (c >> 1) - 1)):
@@ -144,7 +148,9 @@ def state(sim, q):
         if not (ok := (yield gates_full(c))):
             break
         read_gates(sim, c, who)
-        if sim.plant == "late_copy":
+        if sim.local:
+            sim.b[f"ydone{c % GATE_STAGES}"].arrive()
+        elif sim.plant == "late_copy":
             pass
         elif sim.copies_of_s == 2:
             if c >= 2 and not (ok := (yield ("wait", f"mx{c & 1}", (c >> 1) - 1))):
@@ -155,7 +161,8 @@ def state(sim, q):
             break
         sim.read(("S", q), ("S", c), who)
         yield None
-        sim.write(("SB", c % sim.copies_of_s, q), c, who)
+        if not sim.local:
+            sim.write(("SB", c % sim.copies_of_s, q), c, who)
         sim.write(("S", q), ("dec", c), who)
         yield None
         sim.b[f"update{c & 1}"].arrive()
@@ -225,6 +232,8 @@ def split(sim, q):
         if c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
             return
         read_gates(sim, c, who)
+        if sim.local:
+            sim.b[f"ydone{c % GATE_STAGES}"].arrive()
         sim.read(("X", st), c, who)
         yield None
         sim.write(("W", q), c, who)
@@ -232,8 +241,8 @@ def split(sim, q):
         sim.b[f"update{c & 1}"].arrive()
 
 
-def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=300000):
-    sim = Scan(nch, heads, gated, plant)
+def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, local=False, max_steps=300000):
+    sim = Scan(nch, heads, gated, plant, local)
     rng = random.Random(seed)
     roles = {"state issue": issue_state(sim), "output issue": issue_outputs(sim), "copier": copier(sim)}
     roles.update({f"gates{w}": gates(sim, w) for w in (0, 1)})
@@ -242,6 +251,8 @@ def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, max_steps=30
     roles.update({f"m{w}": scores(sim, w) for w in range(M_WARPS)})
     roles.update({f"split{q}": split(sim, q) for q in Q4})
     roles["rows"] = rows(sim)
+    if local:
+        roles = {k: v for k, v in roles.items() if k in ("state issue", "copier") or k.startswith(("gates", "state", "split"))}
     waiting, done = {}, set()
 
     def step(name, value=None):
@@ -297,6 +308,15 @@ def test_random_schedules(nch, heads, gated):
         assert all(sim.tags[("S", q)] == ("S", nch) for q in Q4)
 
 
+@pytest.mark.parametrize("heads", [1, 2])
+@pytest.mark.parametrize("nch", [1, 2, 5, 9])
+def test_random_schedules_of_the_local_pass(nch, heads):
+    for seed in range(40):
+        sim = run(nch, 100 * nch + seed, heads, False, local=True)
+        assert all(sim.tags[("S", q)] == ("S", nch) for q in Q4)
+        run(nch, 700 * nch + seed, heads, False, timeouts=True, local=True)
+
+
 @pytest.mark.parametrize("plant", ["no_yread", "no_mread", "no_empty", "no_yfree", "no_mx", "no_s", "late_copy"])
 def test_planted_mistakes_are_caught(plant):
     with pytest.raises(ProtocolError):
@@ -321,6 +341,6 @@ def test_barrier_counts_match_the_kernel():
         if bound:
             loop = sizes.get(bound) or int(bound)
             continue
-        v = {"kHeads": 2}.get(n) or (int(n) if n.isdigit() else consts[n])
+        v = {"kHeads": 2, "kGateReaders": Y_WARPS}.get(n) or (int(n) if n.isdigit() else consts[n])
         found.update({name + i: v for i in (map(str, range(loop)) if many else ("",))})
     assert found == counts(2)
