@@ -7,10 +7,13 @@
 // without one), act is the identity or silu(y) = y / (1 + exp(-y)), and the new state is
 // the last W-1 rows of [state; x].  fp32 arithmetic from bf16 rows, one rounding of y.
 //
-// Both kernels are HBM-bound (4 bytes a token and channel against 2 W flops and one silu).
-// A thread owns 8 channels (one 16-byte word of a row) and a run of consecutive tokens, so
-// the window slides through its registers: every row is read from HBM once, plus W-1 rows
-// of overlap per run that mostly hit in L2.
+// Both kernels are HBM-bound (4 bytes a token and channel against 2 W flops and one silu, of
+// whose two hardware functions an SM does 16 a cycle: 0.24 of the 0.33 ms that 65,536 x 8192
+// take to read and write).  A thread owns 4 channels (8 bytes of a row) and a run of
+// consecutive tokens, so the window slides through its registers: every row is read from HBM
+// once, plus W-1 rows of overlap per run that mostly hit in L2.  Four channels and not eight,
+// whose weights and window alone took 96 registers: with 12 warps an SM the loads in flight
+// covered half of HBM's latency (0.68 ms).
 #include "gdn_common.cuh"
 #include "gdn_launch.h"
 
@@ -18,53 +21,76 @@ namespace gdn {
 
 namespace {
 
-constexpr int kVec = 8;            // channels of a thread
+constexpr int kVec = 4;            // channels of a thread
 constexpr int kConvThreads = 128;
-constexpr int kBatchRows = 4;      // rows a thread has in flight
+constexpr int kBatchRows = 8;      // rows a thread loads at once
 
 // silu from the hardware exponential and division (a few units of 2^-22 relative, far below
 // the bf16 rounding of the result); -> 0 for large negative y.
 __device__ __forceinline__ float silu_fast(float y) { return __fdividef(y, 1.0f + __expf(-y)); }
 
-struct Row {                       // 8 channels as packed fp32 pairs
-    uint64_t v[4];
+struct Row {                       // 4 channels as packed fp32 pairs
+    uint64_t v[2];
 };
 
-__device__ __forceinline__ Row unpack_row(uint4 w) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ Row unpack_row(uint2 w) {
     Row r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r.v[e] = f2(bf16_lo(u[e]), bf16_hi(u[e]));
+    r.v[0] = f2(bf16_lo(w.x), bf16_hi(w.x));
+    r.v[1] = f2(bf16_lo(w.y), bf16_hi(w.y));
     return r;
 }
 
-__device__ __forceinline__ uint4 load_row(const __nv_bfloat16 *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
+__device__ __forceinline__ uint2 load_row(const __nv_bfloat16 *p) { return __ldg(reinterpret_cast<const uint2 *>(p)); }
 
-// The 8 channels' weights, tap by tap, and bias.
+// The 4 channels' weights, tap by tap, and bias.
 template <int W>
 struct Taps {
     Row w[W], b;
     __device__ __forceinline__ void load(const ConvArgs &p, int64_t c) {
-        float t[kVec * W];
+        float t[kVec * W], u[kVec] = {};
+        if (!p.weights_aligned) {
 #pragma unroll
-        for (int i = 0; i < kVec * W; ++i) t[i] = load_scalar(p.weight, c * W + i, p.weight_dtype);
+            for (int i = 0; i < kVec * W; ++i) t[i] = load_scalar(p.weight, c * W + i, p.weight_dtype);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+                if (p.bias) u[i] = load_scalar(p.bias, c + i, p.weight_dtype);
+        } else if (p.weight_dtype == 1) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p.weight) + c * W) + i);
+                t[4 * i] = bf16_lo(v.x); t[4 * i + 1] = bf16_hi(v.x);
+                t[4 * i + 2] = bf16_lo(v.y); t[4 * i + 3] = bf16_hi(v.y);
+            }
+            if (p.bias) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p.bias) + c));
+                u[0] = bf16_lo(v.x); u[1] = bf16_hi(v.x); u[2] = bf16_lo(v.y); u[3] = bf16_hi(v.y);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + c * W) + i);
+                t[4 * i] = v.x; t[4 * i + 1] = v.y; t[4 * i + 2] = v.z; t[4 * i + 3] = v.w;
+            }
+            if (p.bias) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.bias) + c));
+                u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < W; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[k].v[e] = f2(t[(2 * e) * W + k], t[(2 * e + 1) * W + k]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            b.v[e] = p.bias ? f2(load_scalar(p.bias, c + 2 * e, p.weight_dtype), load_scalar(p.bias, c + 2 * e + 1, p.weight_dtype))
-                            : f2(0.0f, 0.0f);
+            for (int e = 0; e < 2; ++e) w[k].v[e] = f2(t[(2 * e) * W + k], t[(2 * e + 1) * W + k]);
+        b.v[0] = f2(u[0], u[1]);
+        b.v[1] = f2(u[2], u[3]);
     }
 };
 
-// One output row's 8 channels from the window (win[0] oldest) and the current row.
+// One output row's 4 channels from the window (win[0] oldest) and the current row.
 template <int W>
-__device__ __forceinline__ uint4 conv_row(const Taps<W> &k, const Row (&win)[W - 1], const Row &x, bool silu) {
-    uint32_t r[4];
+__device__ __forceinline__ uint2 conv_row(const Taps<W> &k, const Row (&win)[W - 1], const Row &x, bool silu) {
+    uint32_t r[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
         uint64_t acc = k.b.v[e];
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) acc = fma_f2(k.w[i].v[e], win[i].v[e], acc);
@@ -77,7 +103,7 @@ __device__ __forceinline__ uint4 conv_row(const Taps<W> &k, const Row (&win)[W -
         }
         r[e] = pack_bf16x2(y0, y1);
     }
-    return make_uint4(r[0], r[1], r[2], r[3]);
+    return make_uint2(r[0], r[1]);
 }
 
 // Where channel c goes: the output tensor that holds it, as a pointer to its first row and
@@ -118,19 +144,22 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
 #pragma unroll
         for (int r = 0; r < W - 1; ++r) {
             const int64_t e = s1 - s0 + r;
-            uint4 v = make_uint4(0, 0, 0, 0);
+            uint2 v = make_uint2(0, 0);
             if (e >= W - 1) v = load_row(x + (s0 + e - (W - 1)) * p.x_stride);
             else if (state) v = load_row(state + (n * (W - 1) + e) * C);
-            *reinterpret_cast<uint4 *>(dst + r * C) = v;
+            *reinterpret_cast<uint2 *>(dst + r * C) = v;
         }
         return;
     }
     const int64_t t0 = tile * run;
     const int64_t t1 = t0 + run < T ? t0 + run : T;
-    uint4 raw[kBatchRows];
+    uint2 raw[kBatchRows];
+    auto load_batch = [&](int64_t t) {
 #pragma unroll
-    for (int u = 0; u < kBatchRows; ++u)
-        raw[u] = t0 + u < t1 ? load_row(x + (t0 + u) * p.x_stride) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < kBatchRows; ++u)
+            raw[u] = t + u < t1 ? load_row(x + (t + u) * p.x_stride) : make_uint2(0, 0);
+    };
+    load_batch(t0);
     Taps<W> taps;
     taps.load(p, c);
     int64_t width;
@@ -145,22 +174,23 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
     int64_t n = lo;
     int64_t s0 = cu[n];
     s0 = s0 < 0 ? 0 : (s0 > t0 ? t0 : s0);
-    int64_t next = cu[n + 1];
-    // row `back` rows in front of token t of sequence n that starts at s0
-    auto before = [&](int64_t t, int back) -> Row {
-        const int64_t at = t - back - s0;
-        if (at >= 0) return unpack_row(load_row(x + (t - back) * p.x_stride));
-        if (state) return unpack_row(load_row(state + (n * (W - 1) + (W - 1) + at) * C));
-        return unpack_row(make_uint4(0, 0, 0, 0));
-    };
+    int64_t next = n + 1 < N ? cu[n + 1] : T;      // (behind the last sequence there is none to go on to)
+    // the rows in front of token t of sequence n that starts at s0
     Row win[W - 1];
+    auto window = [&](int64_t t) {
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) win[i] = before(t0, W - 1 - i);
+        for (int i = 0; i < W - 1; ++i) {
+            const int back = W - 1 - i;
+            const int64_t at = t - back - s0;
+            uint2 v = make_uint2(0, 0);
+            if (at >= 0) v = load_row(x + (t - back) * p.x_stride);
+            else if (state) v = load_row(state + (n * (W - 1) + (W - 1) + at) * C);
+            win[i] = unpack_row(v);
+        }
+    };
+    window(t0);
     for (int64_t t = t0; t < t1; t += kBatchRows) {
-        uint4 nxt[kBatchRows];
-#pragma unroll
-        for (int u = 0; u < kBatchRows; ++u)
-            nxt[u] = t + kBatchRows + u < t1 ? load_row(x + (t + kBatchRows + u) * p.x_stride) : make_uint4(0, 0, 0, 0);
+        if (t > t0) load_batch(t);
 #pragma unroll
         for (int u = 0; u < kBatchRows; ++u) {
             const int64_t tt = t + u;
@@ -168,21 +198,18 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
                 if (tt >= next && n + 1 < N) {     // the next sequence that has tokens starts here
                     do {
                         ++n;
-                        next = cu[n + 1];
+                        next = n + 1 < N ? cu[n + 1] : T;
                     } while (tt >= next && n + 1 < N);
                     s0 = tt;
-#pragma unroll
-                    for (int i = 0; i < W - 1; ++i) win[i] = before(tt, W - 1 - i);
+                    window(tt);
                 }
                 const Row cur = unpack_row(raw[u]);
-                *reinterpret_cast<uint4 *>(out + tt * width) = conv_row<W>(taps, win, cur, p.silu);
+                *reinterpret_cast<uint2 *>(out + tt * width) = conv_row<W>(taps, win, cur, p.silu);
 #pragma unroll
                 for (int i = 0; i + 1 < W - 1; ++i) win[i] = win[i + 1];
                 win[W - 2] = cur;
             }
         }
-#pragma unroll
-        for (int u = 0; u < kBatchRows; ++u) raw[u] = nxt[u];
     }
 }
 
@@ -204,18 +231,18 @@ conv_decode_kernel(const ConvArgs p, int run, int64_t runs) {
     __nv_bfloat16 *out = out_of(p, c, width);
     const int64_t b1 = (tile + 1) * run < p.rows ? (tile + 1) * run : p.rows;
     for (int64_t b = tile * run; b < b1; ++b) {
-        uint4 raw[W];
+        uint2 raw[W];
 #pragma unroll
         for (int i = 0; i < W - 1; ++i)
-            raw[i] = state ? *reinterpret_cast<const uint4 *>(state + (b * (W - 1) + i) * C + c) : make_uint4(0, 0, 0, 0);
+            raw[i] = state ? *reinterpret_cast<const uint2 *>(state + (b * (W - 1) + i) * C + c) : make_uint2(0, 0);
         raw[W - 1] = load_row(x + b * p.x_stride);
         Row win[W - 1];
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) win[i] = unpack_row(raw[i]);
-        *reinterpret_cast<uint4 *>(out + b * width) = conv_row<W>(taps, win, unpack_row(raw[W - 1]), p.silu);
+        *reinterpret_cast<uint2 *>(out + b * width) = conv_row<W>(taps, win, unpack_row(raw[W - 1]), p.silu);
 #pragma unroll
         for (int i = 0; i < W - 1; ++i)
-            *reinterpret_cast<uint4 *>(new_state + (b * (W - 1) + i) * C + c) = raw[i + 1];
+            *reinterpret_cast<uint2 *>(new_state + (b * (W - 1) + i) * C + c) = raw[i + 1];
     }
 }
 

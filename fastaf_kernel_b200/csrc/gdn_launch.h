@@ -57,6 +57,7 @@ struct ConvArgs {
     int64_t x_stride;
     const void *weight, *bias;   // [channels][width], [channels] or nullptr (weight_dtype)
     int weight_dtype;
+    int weights_aligned;         // weight and bias start on 16-byte boundaries
     const void *state;           // bf16 [num_seqs][width - 1][channels] or nullptr (zero)
     const int32_t *cu_seqlens;   // [num_seqs + 1], device (prefill only)
     int64_t num_seqs, rows;      // rows: tokens (prefill) or sequences (decode)

@@ -93,6 +93,7 @@ int conv_args(gdn::ConvArgs &p, const void *x, int64_t x_row_stride, const void 
     p.weight = weight;
     p.bias = bias;
     p.weight_dtype = weight_dtype;
+    p.weights_aligned = aligned16(weight) && aligned16(bias);
     p.state = state;
     p.num_seqs = num_seqs;
     p.rows = rows;

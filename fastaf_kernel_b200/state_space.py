@@ -14,12 +14,12 @@ The reference has neither operator; its entry points start at q, k and v.
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .api import _GATE_DTYPES, _check_cu_seqlens_host, _gate, _on_device, _ptr
+from .api import _GATE_DTYPES, _check_cu_seqlens_host, _gate
 
 __all__ = ["conv_prefill", "conv_decode", "ssm_prefill", "ssm_decode", "ssm_method"]
 
@@ -31,38 +31,62 @@ _BF16, _F32 = torch.bfloat16, torch.float32
 
 Outputs = Union[torch.Tensor, Tuple[torch.Tensor, ...]]
 
+# (single-token calls take a few microseconds of GPU time: the checks below look at each
+# tensor once and build no torch objects on the way)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _on(device: torch.device, named) -> None:
-    """Every given tensor is a CUDA tensor on ``device``."""
+
+def _on(index: int, named) -> None:
+    """Every given tensor is a CUDA tensor on device ``index``."""
     for name, t in named:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got {t.device}")
-        if t.get_device() != device.index:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index or index < 0):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if not t.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got {t.device}")
+            raise ValueError(f"{name} is on {t.device}, expected the device of x (cuda:{index})")
 
 
-def _rows(name: str, t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+def _index(x) -> int:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    return x.get_device()
+
+
+def _call(fn, index: int, args) -> None:
+    """One C call on the current stream of device ``index``."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _rows(name: str, t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int, int]:
     """bf16 rows of ``width`` elements (the last dimensions of ``t``, packed among
-    themselves) as the kernels read them: the tensor and its row stride in elements.  Rows
-    that do not start on a 16-byte boundary or are not packed become a packed copy."""
+    themselves) as the kernels read them: the tensor, its address and its row stride in
+    elements.  Rows that do not start on a 16-byte boundary or are not packed become a
+    packed copy."""
     if t.dtype != _BF16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    at = t.data_ptr()
     if t.is_contiguous():
-        # (a contiguous slice may still start off a 16-byte boundary)
-        return (t if t.data_ptr() % 16 == 0 else t.clone()), width
-    rows, shape, strides = t.shape[0], t.shape[1:], t.stride()
-    step, packed = 1, True
-    for n, st in zip(reversed(shape), reversed(strides[1:])):
+        if at % 16:      # (a contiguous slice may still start off a 16-byte boundary)
+            t = t.clone()
+            at = t.data_ptr()
+        return t, at, width
+    strides, step, packed = t.stride(), 1, True
+    for n, st in zip(reversed(t.shape[1:]), reversed(strides[1:])):
         packed = packed and (n == 1 or st == step)
         step *= n
-    stride = strides[0] if rows > 1 else width
-    if packed and stride >= width and stride % 8 == 0 and stride < 1 << 31 and t.data_ptr() % 16 == 0:
-        return t, stride
-    return t.contiguous(), width
+    stride = strides[0] if t.shape[0] > 1 else width
+    if packed and stride >= width and stride % 8 == 0 and stride < 1 << 31 and at % 16 == 0:
+        return t, at, stride
+    t = t.contiguous()
+    return t, t.data_ptr(), width
 
 
 def _dt_rows(t: torch.Tensor, heads: int) -> Tuple[torch.Tensor, int]:
@@ -78,13 +102,15 @@ def _dt_rows(t: torch.Tensor, heads: int) -> Tuple[torch.Tensor, int]:
     return t.contiguous(), heads
 
 
-def _destination(name: str, t: Optional[torch.Tensor], shape, dtype, device) -> torch.Tensor:
+def _destination(name: str, t: Optional[torch.Tensor], shape, dtype, like: torch.Tensor) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        if like.shape == shape and like.dtype == dtype and like.is_contiguous():
+            return torch.empty_like(like)
+        return torch.empty(shape, dtype=dtype, device=like.device)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != like.device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
     return t
 
 
@@ -93,7 +119,7 @@ def _state(state: Optional[torch.Tensor], new_state: Optional[torch.Tensor], sha
     readable as it is: a converted copy would leave it half old."""
     if state is None:
         return None
-    if tuple(state.shape) != tuple(shape):
+    if state.shape != shape:
         raise ValueError(f"state must have shape {tuple(shape)}, got {tuple(state.shape)}")
     if state.dtype == dtype and state.is_contiguous() and state.data_ptr() % 16 == 0:
         return state
@@ -102,18 +128,18 @@ def _state(state: Optional[torch.Tensor], new_state: Optional[torch.Tensor], sha
     return state.to(dtype).contiguous().clone()
 
 
-def _cu(cu_seqlens: torch.Tensor, T: int, device: torch.device, validate: bool) -> Tuple[torch.Tensor, int]:
+def _cu(cu_seqlens: torch.Tensor, T: int, x: torch.Tensor, validate: bool) -> Tuple[torch.Tensor, int]:
     if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of at least one entry")
     if cu_seqlens.is_cuda:
-        if cu_seqlens.get_device() != device.index:
-            raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, expected {device}")
+        if cu_seqlens.get_device() != x.get_device():
+            raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, expected {x.device}")
     elif validate:
         _check_cu_seqlens_host(cu_seqlens.detach().to(torch.int64), T)
     if cu_seqlens.shape[0] == 1 and T:
         raise ValueError("cu_seqlens names no sequence but there are tokens")
     if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_cuda or not cu_seqlens.is_contiguous():
-        cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+        cu_seqlens = cu_seqlens.to(device=x.device, dtype=torch.int32).contiguous()
     return cu_seqlens, cu_seqlens.shape[0] - 1
 
 
@@ -122,7 +148,6 @@ def _cu(cu_seqlens: torch.Tensor, T: int, device: torch.device, validate: bool) 
 def _conv(x, weight, bias, state, num_seqs, activation, split, output, new_state):
     """The checks and conversions of both convolution calls: the C call's arguments (without
     cu_seqlens and sizes that only prefill has), the outputs and the new state."""
-    device = x.device
     if x.dim() != 2:
         raise ValueError("x must be [rows, channels]")
     T, C = x.shape
@@ -135,33 +160,36 @@ def _conv(x, weight, bias, state, num_seqs, activation, split, output, new_state
         raise ValueError(f"channels={C} must be a positive multiple of 8")
     if activation not in _ACTIVATIONS:
         raise ValueError("activation must be None or 'silu'")
-    if bias is not None and tuple(bias.shape) != (C,):
+    if bias is not None and bias.shape != (C,):
         raise ValueError(f"bias must be [{C}]")
     weight = _gate(weight)
     if bias is not None:
         bias = _gate(bias)
         if bias.dtype != weight.dtype:
             weight, bias = weight.float(), bias.float()
-    x, stride = _rows("x", x, C)
-    widths: Sequence[int] = (C,) if split is None else tuple(int(n) for n in split)
-    if not 1 <= len(widths) <= _MAX_OUTPUTS or any(n <= 0 or n % 8 for n in widths) or sum(widths) != C:
-        raise ValueError(f"split must be 1 to {_MAX_OUTPUTS} positive multiples of 8 that add up to {C} channels")
+    x, at, stride = _rows("x", x, C)
     if split is None:
-        outs: List[torch.Tensor] = [_destination("output", output, (T, C), _BF16, device)]
+        y = _destination("output", output, (T, C), _BF16, x)
+        outs: Sequence[torch.Tensor] = (y,)
+        widths: Sequence[int] = (C,)
     else:
+        widths = tuple(int(n) for n in split)
+        if not 1 <= len(widths) <= _MAX_OUTPUTS or any(n <= 0 or n % 8 for n in widths) or sum(widths) != C:
+            raise ValueError(f"split must be 1 to {_MAX_OUTPUTS} positive multiples of 8 that add up to {C} channels")
         if output is not None and len(output) != len(widths):
             raise ValueError("output must hold one tensor per split")
-        outs = [_destination("output", None if output is None else output[j], (T, n), _BF16, device)
-                for j, n in enumerate(widths)]
+        y = outs = tuple([_destination("output", None if output is None else output[j], (T, n), _BF16, x)
+                          for j, n in enumerate(widths)])
     shape = (num_seqs, W - 1, C)
-    new_state = _destination("new_state", new_state, shape, _BF16, device)
+    new_state = _destination("new_state", new_state, shape, _BF16, x if state is None else state)
     state = _state(state, new_state, shape, _BF16)
     n = len(widths)
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
-    head = (_ptr(x), stride, _ptr(weight), _ptr(bias), _GATE_DTYPES[weight.dtype], _ptr(state))
-    tail = (_ACTIVATIONS[activation], ptrs, (ctypes.c_int64 * n)(*widths), n, _ptr(new_state))
+    head = (at, stride, weight.data_ptr(), None if bias is None else bias.data_ptr(), _GATE_DTYPES[weight.dtype],
+            None if state is None else state.data_ptr())
+    tail = (_ACTIVATIONS[activation], (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs]),
+            (ctypes.c_int64 * n)(*widths), n, new_state.data_ptr())
     # (the converted copies live until the call has been enqueued)
-    return head, tail, (T, C, W), outs[0] if split is None else tuple(outs), new_state, (x, weight, bias, state)
+    return head, tail, (T, C, W), y, new_state, (x, weight, bias, state)
 
 
 def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
@@ -182,16 +210,13 @@ def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     side, such as q, k and v for ``kernel`` or x, B and C for ``ssm_prefill``; y (and
     ``output``) is then a tuple of [T, width] tensors.  new_state must not overlap state.
     """
-    device = x.device
-    _on(device, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    index = _index(x)
+    _on(index, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
     if x.dim() != 2:
         raise ValueError("x must be [T, channels]")
-    cu, N = _cu(cu_seqlens, x.shape[0], device, validate)
-    head, tail, (T, C, W), y, new_state, held = _conv(x, weight, bias, state, N, activation, split, output, new_state)
-    lib = _lib.load()
-    ctx, stream = _on_device(device)
-    with ctx:
-        _lib.check(lib.gdn_conv_prefill(*head, _ptr(cu), N, T, C, W, *tail, stream))
+    cu, N = _cu(cu_seqlens, x.shape[0], x, validate)
+    head, tail, sizes, y, new_state, held = _conv(x, weight, bias, state, N, activation, split, output, new_state)
+    _call(_lib.load().gdn_conv_prefill, index, (*head, cu.data_ptr(), N, *sizes, *tail))
     return y, new_state
 
 
@@ -201,14 +226,13 @@ def conv_decode(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 new_state: Optional[torch.Tensor] = None) -> Tuple[Outputs, torch.Tensor]:
     """``conv_prefill`` for one token of each sequence: x [B, C], state [B, W-1, C] bf16 or
     None.  Returns (y [B, C], new_state); pass ``new_state=state`` to update it in place."""
-    device = x.device
-    _on(device, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
-    head, tail, (B, C, W), y, new_state, held = _conv(x, weight, bias, state, x.shape[0], activation, split, output,
-                                                      new_state)
-    lib = _lib.load()
-    ctx, stream = _on_device(device)
-    with ctx:
-        _lib.check(lib.gdn_conv_decode(*head, B, C, W, *tail, stream))
+    index = _index(x)
+    _on(index, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    if x.dim() != 2:
+        raise ValueError("x must be [B, channels]")
+    head, tail, sizes, y, new_state, held = _conv(x, weight, bias, state, x.shape[0], activation, split, output,
+                                                  new_state)
+    _call(_lib.load().gdn_conv_decode, index, (*head, *sizes, *tail))
     return y, new_state
 
 
@@ -225,34 +249,32 @@ def ssm_method(total_tokens: int, method: str = "auto", num_seqs: int = 1) -> st
 
 def _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, num_seqs, output, new_state):
     """The checks and conversions of both scan calls."""
-    device = x.device
-    lead = tuple(x.shape[:-2])
-    H, P = x.shape[-2:]
+    *lead, H, P = x.shape
     if P != 64 and P != 128:
         raise NotImplementedError(f"head_size={P} is not supported (64 or 128)")
-    if B.dim() != x.dim() or tuple(B.shape[:-2]) != lead:
-        raise ValueError(f"B must be [..., groups, state_size] with x's leading shape {lead}, got {tuple(B.shape)}")
+    if B.dim() != x.dim() or B.shape[:-2] != x.shape[:-2]:
+        raise ValueError(f"B must be [..., groups, state_size] with x's leading shape {lead}, got {list(B.shape)}")
     G, S = B.shape[-2:]
     if S != 128:
         raise NotImplementedError(f"state_size={S} is not supported (only 128)")
     if C.shape != B.shape:
-        raise ValueError(f"C shape {tuple(C.shape)} must equal B shape {tuple(B.shape)}")
+        raise ValueError(f"C shape {list(C.shape)} must equal B shape {list(B.shape)}")
     if H == 0 or G == 0 or H % G:
         raise ValueError(f"{H} heads must be a positive multiple of {G} groups")
-    if tuple(dt.shape) != lead + (H,):
-        raise ValueError(f"dt must be {list(lead + (H,))}, got {list(dt.shape)}")
+    if dt.shape != x.shape[:-1]:
+        raise ValueError(f"dt must be {list(x.shape[:-1])}, got {list(dt.shape)}")
     for name, t in (("A_log", A_log), ("D", D), ("dt_bias", dt_bias)):
-        if t is not None and tuple(t.shape) != (H,):
+        if t is not None and t.shape != (H,):
             raise ValueError(f"{name} must be [heads] = [{H}]")
     if z is not None and z.shape != x.shape:
-        raise ValueError(f"z shape {tuple(z.shape)} must equal x shape {tuple(x.shape)}")
-    x, sx = _rows("x", x, H * P)
-    B, sB = _rows("B", B, G * S)
-    C, sC = _rows("C", C, G * S)
+        raise ValueError(f"z shape {list(z.shape)} must equal x shape {list(x.shape)}")
+    shape = x.shape
+    x, xp, sx = _rows("x", x, H * P)
+    B, Bp, sB = _rows("B", B, G * S)
+    C, Cp, sC = _rows("C", C, G * S)
+    zp, sz = None, 0
     if z is not None:
-        z, sz = _rows("z", z, H * P)
-    else:
-        sz = 0
+        z, zp, sz = _rows("z", z, H * P)
     dt, sdt = _dt_rows(dt, H)
     A_log = _gate(A_log)
     D = None if D is None else _gate(D)
@@ -261,13 +283,13 @@ def _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, num_seqs, output, new_state):
         A_log = A_log.float()
         D = None if D is None else D.float()
         dt_bias = None if dt_bias is None else dt_bias.float()
-    output = _destination("output", output, lead + (H, P), _BF16, device)
-    shape = (num_seqs, H, P, S)
-    new_state = _destination("new_state", new_state, shape, _F32, device)
-    state = _state(state, new_state, shape, _F32)
-    head = (_ptr(x), sx, _ptr(dt), sdt, _ptr(A_log), _ptr(B), sB, _ptr(C), sC, _ptr(D), _ptr(dt_bias), _ptr(z), sz,
-            _ptr(state))
-    tail = (H, G, P, S, _GATE_DTYPES[dt.dtype], _GATE_DTYPES[A_log.dtype], _ptr(output), _ptr(new_state))
+    output = _destination("output", output, shape, _BF16, x)
+    state_shape = (num_seqs, H, P, S)
+    new_state = _destination("new_state", new_state, state_shape, _F32, x if state is None else state)
+    state = _state(state, new_state, state_shape, _F32)
+    head = (xp, sx, dt.data_ptr(), sdt, A_log.data_ptr(), Bp, sB, Cp, sC, None if D is None else D.data_ptr(),
+            None if dt_bias is None else dt_bias.data_ptr(), zp, sz, None if state is None else state.data_ptr())
+    tail = (H, G, P, S, _GATE_DTYPES[dt.dtype], _GATE_DTYPES[A_log.dtype], output.data_ptr(), new_state.data_ptr())
     # (the converted copies live until the call has been enqueued)
     return head, tail, output, new_state, (x, dt, A_log, B, C, D, dt_bias, z, state)
 
@@ -292,20 +314,17 @@ def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch
     tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what
     ``ssm_method`` reports).
     """
-    device = x.device
-    _on(device, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
-                 ("state", state), ("z", z)))
+    index = _index(x)
+    _on(index, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
+                ("state", state), ("z", z)))
     if x.dim() != 3:
         raise ValueError("x must be [T, heads, head_size]")
     if method not in _METHODS:
         raise ValueError(f"method must be one of {sorted(_METHODS)}")
     T = x.shape[0]
-    cu, N = _cu(cu_seqlens, T, device, validate)
+    cu, N = _cu(cu_seqlens, T, x, validate)
     head, tail, output, new_state, held = _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, N, output, new_state)
-    lib = _lib.load()
-    ctx, stream = _on_device(device)
-    with ctx:
-        _lib.check(lib.gdn_ssm_prefill(*head, _ptr(cu), N, T, *tail, _METHODS[method], stream))
+    _call(_lib.load().gdn_ssm_prefill, index, (*head, cu.data_ptr(), N, T, *tail, _METHODS[method]))
     return output, new_state
 
 
@@ -316,15 +335,12 @@ def ssm_decode(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.
     """One step of ``ssm_prefill``'s scan for each sequence: x, z [B, 1, H, P]; dt [B, 1, H];
     B, C [B, 1, G, 128]; state [B, H, P, 128] fp32 or None.  Returns (y [B, 1, H, P] bf16,
     new_state); pass ``new_state=state`` to update the state in place."""
-    device = x.device
-    _on(device, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
-                 ("state", state), ("z", z)))
+    index = _index(x)
+    _on(index, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
+                ("state", state), ("z", z)))
     if x.dim() != 4 or x.shape[1] != 1:
         raise ValueError("x must be [B, 1, heads, head_size]")
     batch = x.shape[0]
     head, tail, output, new_state, held = _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, batch, output, new_state)
-    lib = _lib.load()
-    ctx, stream = _on_device(device)
-    with ctx:
-        _lib.check(lib.gdn_ssm_decode(*head, batch, *tail, stream))
+    _call(_lib.load().gdn_ssm_decode, index, (*head, batch, *tail))
     return output, new_state
