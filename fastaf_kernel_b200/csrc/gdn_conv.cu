@@ -25,10 +25,6 @@ constexpr int kVec = 4;            // channels of a thread
 constexpr int kConvThreads = 128;
 constexpr int kBatchRows = 8;      // rows a thread loads at once
 
-// silu from the hardware exponential and division (a few units of 2^-22 relative, far below
-// the bf16 rounding of the result); -> 0 for large negative y.
-__device__ __forceinline__ float silu_fast(float y) { return __fdividef(y, 1.0f + __expf(-y)); }
-
 struct Row {                       // 4 channels as packed fp32 pairs
     uint64_t v[2];
 };
@@ -98,8 +94,8 @@ __device__ __forceinline__ uint2 conv_row(const Taps<W> &k, const Row (&win)[W -
         float y0, y1;
         unf2(acc, y0, y1);
         if (silu) {
-            y0 = silu_fast(y0);
-            y1 = silu_fast(y1);
+            y0 = silu_approx(y0);
+            y1 = silu_approx(y1);
         }
         r[e] = pack_bf16x2(y0, y1);
     }
@@ -151,65 +147,72 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
         }
         return;
     }
-    const int64_t t0 = tile * run;
-    const int64_t t1 = t0 + run < T ? t0 + run : T;
+    const int t0 = static_cast<int>(tile * run);
+    const int t1 = static_cast<int>(t0 + run < T ? t0 + run : T);
     uint2 raw[kBatchRows];
-    auto load_batch = [&](int64_t t) {
+    const __nv_bfloat16 *xt = x + t0 * p.x_stride;      // row t
+    auto load_batch = [&](int rows) {
 #pragma unroll
-        for (int u = 0; u < kBatchRows; ++u)
-            raw[u] = t + u < t1 ? load_row(x + (t + u) * p.x_stride) : make_uint2(0, 0);
+        for (int u = 0; u < kBatchRows; ++u) raw[u] = u < rows ? load_row(xt + u * p.x_stride) : make_uint2(0, 0);
     };
-    load_batch(t0);
+    load_batch(t1 - t0);
     Taps<W> taps;
     taps.load(p, c);
     int64_t width;
     __nv_bfloat16 *out = out_of(p, c, width);
+    out += t0 * width;
     // The sequence of token t0: the last one that starts at or before it.
-    int64_t lo = 0, hi = N - 1;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) >> 1;
-        if (cu[mid] <= t0) lo = mid;
+    int64_t n = 0;
+    for (int64_t hi = N - 1; n < hi;) {
+        const int64_t mid = (n + hi + 1) >> 1;
+        if (cu[mid] <= t0) n = mid;
         else hi = mid - 1;
     }
-    int64_t n = lo;
-    int64_t s0 = cu[n];
+    int s0 = cu[n];
     s0 = s0 < 0 ? 0 : (s0 > t0 ? t0 : s0);
-    int64_t next = n + 1 < N ? cu[n + 1] : T;      // (behind the last sequence there is none to go on to)
+    int next = n + 1 < N ? cu[n + 1] : 0x7fffffff;      // (behind the last sequence there is none to go on to)
     // the rows in front of token t of sequence n that starts at s0
     Row win[W - 1];
-    auto window = [&](int64_t t) {
+    auto window = [&](int t) {
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) {
-            const int back = W - 1 - i;
-            const int64_t at = t - back - s0;
+            const int back = W - 1 - i, at = t - back - s0;
             uint2 v = make_uint2(0, 0);
             if (at >= 0) v = load_row(x + (t - back) * p.x_stride);
             else if (state) v = load_row(state + (n * (W - 1) + (W - 1) + at) * C);
             win[i] = unpack_row(v);
         }
     };
-    window(t0);
-    for (int64_t t = t0; t < t1; t += kBatchRows) {
-        if (t > t0) load_batch(t);
+    auto put_row = [&](uint2 w) {
+        const Row cur = unpack_row(w);
+        *reinterpret_cast<uint2 *>(out) = conv_row<W>(taps, win, cur, p.silu);
+        out += width;
 #pragma unroll
-        for (int u = 0; u < kBatchRows; ++u) {
-            const int64_t tt = t + u;
-            if (tt < t1) {
-                if (tt >= next && n + 1 < N) {     // the next sequence that has tokens starts here
+        for (int i = 0; i + 1 < W - 1; ++i) win[i] = win[i + 1];
+        win[W - 2] = cur;
+    };
+    window(t0);
+    for (int t = t0; t < t1; t += kBatchRows) {
+        if (t > t0) load_batch(t1 - t);
+        if (t1 - t >= kBatchRows && next - t >= kBatchRows) {
+            // whole batches inside a sequence, nearly all of them: nothing to check per row
+#pragma unroll
+            for (int u = 0; u < kBatchRows; ++u) put_row(raw[u]);
+        } else {
+#pragma unroll 1
+            for (int tt = t; tt < t1 && tt < t + kBatchRows; ++tt) {
+                if (tt >= next) {       // the next sequence that has tokens starts here
                     do {
                         ++n;
-                        next = n + 1 < N ? cu[n + 1] : T;
-                    } while (tt >= next && n + 1 < N);
+                        next = n + 1 < N ? cu[n + 1] : 0x7fffffff;
+                    } while (tt >= next);
                     s0 = tt;
                     window(tt);
                 }
-                const Row cur = unpack_row(raw[u]);
-                *reinterpret_cast<uint2 *>(out + tt * width) = conv_row<W>(taps, win, cur, p.silu);
-#pragma unroll
-                for (int i = 0; i + 1 < W - 1; ++i) win[i] = win[i + 1];
-                win[W - 2] = cur;
+                put_row(load_row(xt + (tt - t) * p.x_stride));
             }
         }
+        xt += kBatchRows * p.x_stride;
     }
 }
 

@@ -40,7 +40,7 @@ __device__ __forceinline__ float bf16_at(const void *p, int64_t i) {
 // y of one row, gated and rounded.
 __device__ __forceinline__ void store_y(const SsmArgs &p, int64_t row, int h, int r, float y, float x, float D) {
     y = fmaf(D, x, y);
-    if (p.z) y *= ssm_silu(bf16_at(p.z, row * p.z_stride + h * p.head_size + r));
+    if (p.z) y *= silu_approx(bf16_at(p.z, row * p.z_stride + h * p.head_size + r));
     static_cast<__nv_bfloat16 *>(p.out)[(row * p.heads + h) * p.head_size + r] = __float2bfloat16_rn(y);
 }
 

@@ -21,7 +21,4 @@ __device__ __forceinline__ float ssm_step(const SsmArgs &p, int64_t row, int h) 
     return softplus_torch(v);
 }
 
-// silu from the hardware exponential and division (a few units of 2^-22 relative).
-__device__ __forceinline__ float ssm_silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
-
 }  // namespace gdn

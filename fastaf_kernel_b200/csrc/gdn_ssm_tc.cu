@@ -668,8 +668,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                     unf2(fma_f2(bits2(yi[2 * k], yi[2 * k + 1]), k < 2 ? f2(ea.x, ea.y) : f2(eb.x, eb.y),
                                 bits2(yo[2 * k], yo[2 * k + 1])), y0, y1);
                     if (gated) {
-                        y0 *= ssm_silu(bf16_lo(zr[k]));
-                        y1 *= ssm_silu(bf16_hi(zr[k]));
+                        y0 *= silu_approx(bf16_lo(zr[k]));
+                        y1 *= silu_approx(bf16_hi(zr[k]));
                     }
                     y[k] = pack_bf16x2(y0, y1);
                 }
