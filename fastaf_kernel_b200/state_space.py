@@ -104,9 +104,7 @@ def _dt_rows(t: torch.Tensor, heads: int) -> Tuple[torch.Tensor, int]:
 
 def _destination(name: str, t: Optional[torch.Tensor], shape, dtype, like: torch.Tensor) -> torch.Tensor:
     if t is None:
-        if like.shape == shape and like.dtype == dtype and like.is_contiguous():
-            return torch.empty_like(like)
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape) if like.dtype == dtype else like.new_empty(shape, dtype=dtype)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != like.device:
@@ -173,13 +171,13 @@ def _conv(x, weight, bias, state, num_seqs, activation, split, output, new_state
         outs: Sequence[torch.Tensor] = (y,)
         widths: Sequence[int] = (C,)
     else:
-        widths = tuple(int(n) for n in split)
-        if not 1 <= len(widths) <= _MAX_OUTPUTS or any(n <= 0 or n % 8 for n in widths) or sum(widths) != C:
+        widths = split
+        if not 1 <= len(widths) <= _MAX_OUTPUTS or any([n <= 0 or n % 8 for n in widths]) or sum(widths) != C:
             raise ValueError(f"split must be 1 to {_MAX_OUTPUTS} positive multiples of 8 that add up to {C} channels")
         if output is not None and len(output) != len(widths):
             raise ValueError("output must hold one tensor per split")
-        y = outs = tuple([_destination("output", None if output is None else output[j], (T, n), _BF16, x)
-                          for j, n in enumerate(widths)])
+        y = outs = (tuple([x.new_empty((T, n)) for n in widths]) if output is None else
+                    tuple([_destination("output", t, (T, n), _BF16, x) for t, n in zip(output, widths)]))
     shape = (num_seqs, W - 1, C)
     new_state = _destination("new_state", new_state, shape, _BF16, x if state is None else state)
     state = _state(state, new_state, shape, _BF16)
