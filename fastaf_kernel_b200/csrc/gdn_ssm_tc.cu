@@ -28,14 +28,15 @@
 // block; the 8 rows of the block itself take one exponential per element.  So a row of 32
 // columns takes 12 exponentials, and none overflows however strong the decays are.
 //
-// Roles (25 of 28 warps), handing chunks to each other through mbarriers:
+// Roles (28 warps), handing chunks to each other through mbarriers:
 //   warp 0        issues the state update(c), then G(c + 1); allocates TMEM
-//   warp 27       issues Yi(c), Ya(c) (one thread alone could not keep the tensor pipe busy)
+//   warp 3        issues Yi(c), Ya(c) (one thread alone could not keep the tensor pipe busy)
 //   warp 18       copies (TMA): three stages of C, B and x, two of z, and boxes further ahead
 //                 into L2
-//   warps 2, 3    the chunk's gates: one head each, or one head's chunks in turn
+//   warp 2        the chunk's gates
 //   warps 4-7     state path: S -> bf16 copy (TMEM operand of Yi) and the decay of S
-//   warps 12-15   w x hi / lo into TMEM; the rows behind the last token set to zero
+//   warps 12-15, 24-27   w x hi / lo into TMEM, 16 state rows each; the rows behind the last
+//                 token set to zero
 //   warps 16, 17, 1   M, a 32 x 32 block each
 //   warps 8-11, 20-23   outputs, 32 tokens each: Yi, Ya from TMEM as accumulator fragments, the
 //                 gate z, transposed into bf16 rows in shared memory (stmatrix)
@@ -71,7 +72,7 @@ constexpr int kGateStages = 4;
 constexpr int64_t kMinSegment = 512;    // tokens a sequence is cut into at least
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
 constexpr int kMWarps = 3, kYWarps = 8;
-constexpr int kUpdateWarps = 8;      // of the state path and the split
+constexpr int kUpdateWarps = 12;     // of the state path and the split
 
 // Shared memory (bytes from the 1024-aligned base).  Tiles are 64 rows of 64 bf16 (one
 // 128-byte swizzled atom, 8 KB), two atoms side by side.
@@ -98,16 +99,16 @@ struct alignas(16) Gates {
 };
 static_assert(sizeof(Gates) <= GATE, "gate block");
 
-// TMEM columns (all 512 allocated).  One head: two copies of bf16(S), so that the state path
-// of a chunk need not wait for Yi of the one before; two heads: one copy, since Ya takes 64
-// columns per head (rows 0..63 use the first head's, rows 64..127 the second's).
+// TMEM columns (all 512 allocated).  One head: two buffers of G, so that the scores of a chunk
+// need not wait for M of the one before; two heads: one, since Ya takes 64 columns per head
+// (rows 0..63 use the first head's, rows 64..127 the second's).
 template <bool PAIR>
 struct Tm {
     static constexpr uint32_t S = 0;                         // [0, 128) fp32 state
-    static constexpr uint32_t SB = 128;                      // bf16x2, 64 columns a copy
-    static constexpr int kCopies = PAIR ? 1 : 2;
-    static constexpr uint32_t G = SB + 64 * kCopies;         // lanes 0..63
-    static constexpr uint32_t YI = G + 64, YA = YI + 64;
+    static constexpr uint32_t SB = 128;                      // [128, 192) bf16x2 copy of it
+    static constexpr uint32_t G = 192;                       // lanes 0..63, 64 columns a buffer
+    static constexpr int kG = PAIR ? 1 : 2;
+    static constexpr uint32_t YI = G + 64 * kG, YA = YI + 64;
     static constexpr uint32_t W = YA + (PAIR ? 128 : 64);    // bf16x2 w x: 32 columns hi, 32 lo
     static_assert(W + 64 == 512, "TMEM map");
 };
@@ -152,8 +153,8 @@ __device__ __forceinline__ int64_t segments_of(const TcArgs &a, int64_t tokens) 
 
 struct Bars {
     uint64_t full[kStages], empty[kStages], gates[kGateStages], ydone[kGateStages];
-    uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2], update[2], last[2];
-    uint64_t g, mread, s, cs, yread;
+    uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2], update[2], last[2], g[2], mread[2];
+    uint64_t s, cs, yread;
 };
 
 // What a wait looks at besides its barrier, at the end of the dynamic shared memory.
@@ -335,7 +336,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 mbar_init(bar(bars.empty[i]), 2);
             }
             for (int i = 0; i < kGateStages; ++i) {
-                mbar_init(bar(bars.gates[i]), kHeads);
+                mbar_init(bar(bars.gates[i]), 1);
                 mbar_init(bar(bars.ydone[i]), kGateReaders);
             }
             for (int i = 0; i < 2; ++i) {
@@ -346,9 +347,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 mbar_init(bar(bars.mready[i]), kMWarps);
                 mbar_init(bar(bars.update[i]), kUpdateWarps);
                 mbar_init(bar(bars.last[i]), 1);
+                mbar_init(bar(bars.g[i]), 1);
+                mbar_init(bar(bars.mread[i]), kMWarps);
             }
-            mbar_init(bar(bars.g), 1);
-            mbar_init(bar(bars.mread), kMWarps);
             mbar_init(bar(bars.s), 1);
             mbar_init(bar(bars.cs), 1);
             mbar_init(bar(bars.yread), kYWarps);
@@ -389,13 +390,13 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         auto scores = [&](int c) -> bool {      // G(c)
             const uint32_t st = (c % kStages) * kSt;
             if (!wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) return false;
-            if (c >= 1 && !wait.warp(bar(bars.mread), c - 1, kSsmM)) return false;
+            if (c >= TM::kG && !wait.warp(bar(bars.mread[c & (TM::kG - 1)]), c / TM::kG - 1, kSsmM)) return false;
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    mma_ss(tm + TM::G, dC + st + (k >> 2) * kAtom + 2 * (k & 3), dBk + st + (k >> 2) * kAtom + 2 * (k & 3),
+                    mma_ss(tm + TM::G + (c & (TM::kG - 1)) * 64, dC + st + (k >> 2) * kAtom + 2 * (k & 3), dBk + st + (k >> 2) * kAtom + 2 * (k & 3),
                            id_g, k > 0);
-                mma_commit(bar(bars.g));
+                mma_commit(bar(bars.g[c & (TM::kG - 1)]));
             }
             __syncwarp();
             ++ng;
@@ -424,10 +425,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         if (elect_one()) mma_commit(bar(bars.last[0]));
         __syncwarp();
         wait.drain(bar(bars.last[0]), 0, kSsmIssue);
-        if (ng) wait.drain(bar(bars.g), ng - 1, kSsmG);
+#pragma unroll 1
+        for (int c = ng > TM::kG ? ng - TM::kG : 0; c < ng; ++c)
+            wait.drain(bar(bars.g[c & (TM::kG - 1)]), c / TM::kG, kSsmG);
         if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
         __syncwarp();
-    } else if (!LOCAL && warp == 27) {
+    } else if (!LOCAL && warp == 3) {
         // -------------------------------------------------------------- Yi and Ya
         const uint64_t dC = smem_desc_sw128(sbase + OFF_STAGE + ST_C, 16, 1024);      // K-major
         const uint64_t dX = smem_desc_sw128(sbase + OFF_STAGE + ST_X, 8192, 1024);    // MN-major
@@ -445,9 +448,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    mma_ts(tm + TM::YI, tm + TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0) + 8 * k,
-                           dC + st + (k >> 2) * kAtom + 2 * (k & 3), id_y, k > 0);
-                if (TM::kCopies == 1) mma_commit(bar(bars.cs));
+                    mma_ts(tm + TM::YI, tm + TM::SB + 8 * k, dC + st + (k >> 2) * kAtom + 2 * (k & 3), id_y, k > 0);
+                mma_commit(bar(bars.cs));
             }
             __syncwarp();
             if (!wait.warp(bar(bars.mready[c & (kMBuffers - 1)]), c / kMBuffers, kSsmM)) break;
@@ -506,30 +508,55 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         for (int c = zissued > 2 ? zissued - 2 : 0; c < zissued; ++c)
             wait.drain(bar(bars.zfull[c & 1]), c >> 1, kSsmZ);
         __syncwarp();
-    } else if (warp == 2 || warp == 3) {
+    } else if (warp == 2) {
         // -------------------------------------------------------------- gates
-        // a warp for each of two heads, or two taking the one head's chunks in turn
-        const int head = PAIR ? warp - 2 : 0;
-        constexpr int kTurn = PAIR ? 1 : 2;
-        const int h = lone ? h0 : h0 + head;
-        const float negA2 = -expf(load_scalar(p.A_log, h, p.param_dtype)) * 1.4426950408889634f;   // log2 decays
-        const float bias = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
-        auto raw = [&](int64_t t) { return t < s1 ? load_scalar(p.dt, t * p.dt_stride + h, p.dt_dtype) : 0.0f; };
-        // a lane holds tokens 2 lane and 2 lane + 1
-        const int c0 = PAIR ? 0 : warp - 2;
-        float r0 = raw(s0 + c0 * kL + 2 * lane), r1 = raw(s0 + c0 * kL + 2 * lane + 1);
+        float negA2[kHeads], bias[kHeads];       // log2 decay of dt' = 1
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            const int h = lone ? h0 : h0 + k;
+            negA2[k] = -expf(load_scalar(p.A_log, h, p.param_dtype)) * 1.4426950408889634f;
+            bias[k] = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
+        }
+        // A lane holds tokens 2 lane and 2 lane + 1 of a chunk; one turn per chunk and head.  dt
+        // is loaded two turns ahead, and its lines are brought into L2 before that: with one turn
+        // between a load and its use, HBM's latency was every chunk's time.
+        float d[3][2];
+        auto fetch = [&](int i, float (&to)[2]) {
+            const int k = PAIR ? i & 1 : 0;
+            const int64_t t = s0 + static_cast<int64_t>(i / kHeads) * kL + 2 * lane;
+            const int64_t at = t * p.dt_stride + (lone ? h0 : h0 + k);
+            to[0] = t < s1 ? load_scalar(p.dt, at, p.dt_dtype) : 0.0f;
+            to[1] = t + 1 < s1 ? load_scalar(p.dt, at + p.dt_stride, p.dt_dtype) : 0.0f;
+        };
+        auto ahead = [&](int c) {
+            const int64_t t = s0 + static_cast<int64_t>(c) * kL + 2 * lane, at = t * p.dt_stride + h0;
+            const char *line = static_cast<const char *>(p.dt) + (p.dt_dtype == 1 ? 2 : 4) * at;
+            if (t < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            if (t + 1 < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (p.dt_dtype == 1 ? 2 : 4) * p.dt_stride));
+        };
+        fetch(0, d[0]);
+        fetch(1, d[1]);
+        for (int c = 1; c < kPrefetch; ++c) ahead(c);
 #pragma unroll 1
-        for (int c = c0; c < nch; c += kTurn) {
+        for (int i = 0; i < nch * kHeads; ++i) {
+            const int c = i / kHeads, head = PAIR ? i & 1 : 0;
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL + 2 * lane;
-            const float d0 = t0 < s1 ? softplus_series(r0 + bias) : 0.0f;
-            const float d1 = t0 + 1 < s1 ? softplus_series(r1 + bias) : 0.0f;
-            r0 = raw(t0 + kTurn * kL);        // (the next chunk's, in flight meanwhile)
-            r1 = raw(t0 + kTurn * kL + 1);
+            fetch(i + 2, d[2]);
+            if (head == 0) ahead(c + kPrefetch);
+            const float b0 = PAIR && head ? bias[kHeads - 1] : bias[0];
+            const float d0 = t0 < s1 ? softplus_series(d[0][0] + b0) : 0.0f;
+            const float d1 = t0 + 1 < s1 ? softplus_series(d[0][1] + b0) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                d[0][k] = d[1][k];
+                d[1][k] = d[2][k];
+            }
             // The sums up to and including a token, and those behind it, are both summed:
             // neither is a difference of long sums.
             // (a decay below 2^-150 is zero in fp32; without the bound one such token would cost
             // the sums behind it their precision)
-            const float a0 = fmaxf(negA2 * d0, -160.0f), a1 = fmaxf(negA2 * d1, -160.0f);
+            const float nA = PAIR && head ? negA2[kHeads - 1] : negA2[0];
+            const float a0 = fmaxf(nA * d0, -160.0f), a1 = fmaxf(nA * d1, -160.0f);
             float up = a0 + a1, down = up;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {
@@ -546,7 +573,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                         n3 = __shfl_down_sync(0xffffffffu, a0 + a1, 3, 4);
             const int q = lane & 3;
             const float rest = (q < 3 ? n1 : 0.0f) + (q < 2 ? n2 : 0.0f) + (q < 1 ? n3 : 0.0f);
-            if (c >= kGateStages &&
+            if (head == 0 && c >= kGateStages &&
                 !wait.warp(bar(bars.ydone[c & (kGateStages - 1)]), c / kGateStages - 1, kSsmY)) break;
             Gates *o = gates_of(c, head);
             auto put = [&](float *to, float v0, float v1) { reinterpret_cast<float2 *>(to)[lane] = make_float2(v0, v1); };
@@ -556,7 +583,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             put(o->e, ex2(l0), ex2(l1));
             split2_bf16(ex2(behind + a1) * d0, ex2(behind) * d1, o->wh[lane & 3][lane >> 2], o->wl[lane & 3][lane >> 2]);
             if (lane == 31) o->total = ex2(l1);
-            warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
+            if (head == kHeads - 1) warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
         }
     } else if (warp >= 4 && warp < 8) {
         // -------------------------------------------------------------- state path
@@ -586,15 +613,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (LOCAL) {
                 product *= decay;
                 warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
-            } else if (TM::kCopies == 2) {
-                // Yi of two chunks before has read the copy (of the one before, with one copy)
-                if (c >= 2 && !(ok = wait.warp(bar(bars.mx[c & 1]), (c >> 1) - 1, kSsmMX))) break;
-            } else {
-                if (c >= 1 && !(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
+            } else if (c >= 1) {
+                // Yi of the chunk before has read the copy
+                if (!(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
             }
             // the state is up to date
             if (c >= 1 && !(ok = wait.warp(bar(bars.s), c - 1, kSsmS))) break;
-            const uint32_t sb = TM::SB + (TM::kCopies == 2 ? (c & 1) * 64 : 0);
             const uint64_t d2 = f2(decay, decay);
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
@@ -604,7 +628,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 if (!LOCAL) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                    tmem_st16(tmem_addr(tm, lane_base, sb + 16 * q), b);
+                    tmem_st16(tmem_addr(tm, lane_base, TM::SB + 16 * q), b);
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
@@ -640,25 +664,26 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // -------------------------------------------------------------- outputs
         // A fragment's registers hold two neighbouring tokens of one state row; stmatrix
         // writes eight rows' worth of them transposed, as 16 bytes of each token's row.
-        const uint32_t ya = TM::YA + (PAIR ? hrow * 64 : 0);
-        const int mi = lane >> 3, r8 = lane & 7, q2 = 2 * (lane & 3);
+        const int mi = lane >> 3, r8 = lane & 7, i0 = warp >= 20 ? 32 : 0;      // the warp's first token
+        const uint32_t yi_at = tmem_addr(tm, lane_base, TM::YI + i0), ya_at = tmem_addr(tm, lane_base, TM::YA + (PAIR ? hrow * 64 : 0) + i0);
+        const uint32_t at = (lane_base >> 6) * 8192 + sw128(i0 + 8 * (mi >> 1) + r8, ((lane_base & 63) >> 3) + (mi & 1));
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
-            const float *e = gates_of(c, hrow)->e + q2;
+            const float *e = gates_of(c, hrow)->e + i0 + 2 * (lane & 3);
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
             // the stores two chunks before have read the staging rows (z's copy waited for them)
             if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
             if (!wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX)) break;      // (Yi went out before Ya)
             const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
-#pragma unroll 2
+#pragma unroll
             for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
-                const int lh = u & 1, h = (u >> 1) + (warp >= 20 ? 2 : 0);
+                const int lh = u & 1, hh = u >> 1;
                 uint32_t yi[8], yo[8], zr[4], y[4];
-                tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, TM::YI + 16 * h), yi);
-                tmem_ld_frag16(tmem_addr(tm, lane_base + 16 * lh, ya + 16 * h), yo);
-                const int p0 = static_cast<int>(lane_base) + 16 * lh + 8 * (mi & 1);
-                const uint32_t to = tile + (p0 >> 6) * 8192 + sw128(16 * h + 8 * (mi >> 1) + r8, (p0 & 63) >> 3);
-                const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * h), eb = *reinterpret_cast<const float2 *>(e + 16 * h + 8);
+                tmem_ld_frag16(yi_at + (16u * lh << 16) + 16 * hh, yi);
+                tmem_ld_frag16(ya_at + (16u * lh << 16) + 16 * hh, yo);
+                // (the second 16 rows are two 16-byte words on, under the swizzle)
+                const uint32_t to = tile + (lh ? at ^ 32u : at) + hh * 2048;
+                const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * hh), eb = *reinterpret_cast<const float2 *>(e + 16 * hh + 8);
                 if (gated) ldsm_x4_t(zr, to);
                 tmem_wait_ld_dep(yi);
                 tmem_wait_ld_dep(yo);
@@ -726,7 +751,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             // the tile has been read by Ya two chunks before (one, with one buffer)
             if (c >= kMBuffers &&
                 !wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers - 1, kSsmMX)) break;
-            if (!wait.warp(bar(bars.g), c, kSsmG)) break;
+            if (!wait.warp(bar(bars.g[c & (TM::kG - 1)]), c / TM::kG, kSsmG)) break;
 #pragma unroll 1
             for (int k = 0; k < kHeads; ++k) {
                 const Gates *o = gates_of(c, k);
@@ -738,7 +763,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {              // 8 columns
                     uint32_t r[8], b[4];
-                    tmem_ld8(tmem_addr(tm, lane_base, TM::G + j0 + 8 * q), r);
+                    tmem_ld8(tmem_addr(tm, lane_base, TM::G + (c & (TM::kG - 1)) * 64 + j0 + 8 * q), r);
                     const float4 *col = reinterpret_cast<const float4 *>(o->cf + j0 + 8 * q);
                     const float4 v0 = col[0], v1 = col[1];
                     const float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
@@ -764,15 +789,17 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 }
             }
             tc_fence_before();
-            warp_arrive(bar(bars.mread), lane);
+            warp_arrive(bar(bars.mread[c & (TM::kG - 1)]), lane);
             fence_proxy_async_smem();
             warp_arrive(bar(bars.mready[c & (kMBuffers - 1)]), lane);
         }
-    } else if (warp >= 12 && warp < 16) {
+    } else if ((warp >= 12 && warp < 16) || warp >= 24) {
         // -------------------------------------------------------------- w x, hi and lo
         // ldmatrix.trans reads the x tile [token][row] as fragments [row][token pair], the
         // layout of the TMEM operand's 32-bit columns.
         const int mi = lane >> 3, r8 = lane & 7, q1 = lane & 3;
+        const int p0 = static_cast<int>(lane_base) + (warp >= 24 ? 16 : 0);      // the warp's first state row
+        const uint32_t from = (p0 >> 6) * 8192 + sw128(8 * (mi >> 1) + r8, ((p0 & 63) >> 3) + (mi & 1));
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int st = c % kStages;
@@ -794,32 +821,29 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 if (LOCAL) warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);
             }
             if (nt < kL) {
-                // Rows behind the last token, which may hold anything: zero in this warp's 32
+                // Rows behind the last token, which may hold anything: zero in this warp's 16
                 // columns of x and of B.
-                uint8_t *bt = sm + OFF_STAGE + st * STAGE + ST_B + (warp >> 1 & 1) * 8192;
-                for (int i = nt * 4 + lane; i < kL * 4; i += 32) {
-                    const uint32_t at = sw128(i >> 2, (warp & 1) * 4 + (i & 3));
+                uint8_t *bt = sm + OFF_STAGE + st * STAGE + ST_B + (p0 >> 6) * 8192;
+#pragma unroll 1
+                for (int i = nt * 2 + lane; i < kL * 2; i += 32) {
+                    const uint32_t at = sw128(i >> 1, ((p0 & 63) >> 3) + (i & 1));
                     *reinterpret_cast<uint4 *>(bt + at) = make_uint4(0, 0, 0, 0);
                     *reinterpret_cast<uint4 *>(bt + (ST_X - ST_B) + at) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-#pragma unroll 1
-            for (int lh = 0; lh < 2; ++lh) {       // 16 state rows
-                const int p0 = static_cast<int>(lane_base) + 16 * lh + 8 * (mi & 1);
-                const uint32_t from = xs + (p0 >> 6) * 8192 + sw128(8 * (mi >> 1) + r8, (p0 & 63) >> 3);
-                uint32_t x[16], hi[16], lo[16];
+            uint32_t x[16], hi[16], lo[16];
 #pragma unroll
-                for (int gp = 0; gp < 4; ++gp) ldsm_x4_t(*reinterpret_cast<uint32_t(*)[4]>(x + 4 * gp), from + gp * 2048);
+            for (int gp = 0; gp < 4; ++gp)
+                ldsm_x4_t(*reinterpret_cast<uint32_t(*)[4]>(x + 4 * gp), xs + from + gp * 2048);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    hi[k] = mul_bf2(x[k], wh[k >> 1]);
-                    lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
-                }
-                tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W), hi);
-                tmem_st_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::W + 32), lo);
+            for (int k = 0; k < 16; ++k) {
+                hi[k] = mul_bf2(x[k], wh[k >> 1]);
+                lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
             }
+            tmem_st_frag32(tmem_addr(tm, p0, TM::W), hi);
+            tmem_st_frag32(tmem_addr(tm, p0, TM::W + 32), lo);
             tmem_wait_st();
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);

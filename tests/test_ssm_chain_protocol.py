@@ -13,15 +13,16 @@ from test_tc_chain_protocol import Bar, ProtocolError, Sim
 
 KERNEL = os.path.join(os.path.dirname(__file__), "..", "fastaf_kernel_b200", "csrc", "gdn_ssm_tc.cu")
 Q4 = range(4)
-M_WARPS, SPLIT_WARPS, Y_WARPS = 3, 4, 8
+M_WARPS, SPLIT_WARPS, Y_WARPS = 3, 8, 8
 
 
 STAGES, GATE_STAGES = 3, 4
 
 
 def counts(heads, local=False):
-    c = dict(g=1, mread=M_WARPS, s=1, cs=1, yread=Y_WARPS)
-    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1), ("gates", GATE_STAGES, heads), ("ydone", GATE_STAGES, 4 + SPLIT_WARPS if local else Y_WARPS),
+    c = dict(s=1, cs=1, yread=Y_WARPS)
+    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1),
+                    ("g", 2, 1), ("mread", 2, M_WARPS), ("gates", GATE_STAGES, 1), ("ydone", GATE_STAGES, 4 + SPLIT_WARPS if local else Y_WARPS),
                     ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, Y_WARPS), ("yfree", 2, 1)):
         c.update({f"{k}{i}": v for i in range(n)})
     return c
@@ -30,7 +31,7 @@ def counts(heads, local=False):
 class Scan(Sim):
     def __init__(self, nch, heads, gated, plant=None, local=False):
         super().__init__(nch, plant)
-        self.heads, self.gated, self.copies_of_s, self.m_buffers = heads, gated, 3 - heads, 3 - heads
+        self.heads, self.gated, self.m_buffers, self.g_buffers = heads, gated, 3 - heads, 3 - heads
         self.b = {k: Bar(k, v) for k, v in counts(heads, local).items()}
         self.local = local     # the state path alone
 
@@ -44,10 +45,11 @@ def issue_state(sim):
     def scores(c):
         if not (yield ("wait", f"full{c % STAGES}", c // STAGES)):
             return False
-        if c >= 1 and sim.plant != "no_mread" and not (yield ("wait", "mread", c - 1)):
+        n = sim.g_buffers
+        if c >= n and sim.plant != "no_mread" and not (yield ("wait", f"mread{c % n}", c // n - 1)):
             return False
-        sim.mma({("C", c % STAGES): c, ("B", c % STAGES): c}, {("G",): (None, c)}, f"G({c})")
-        sim.commit("g")
+        sim.mma({("C", c % STAGES): c, ("B", c % STAGES): c}, {("G", c % n): (None, c)}, f"G({c})")
+        sim.commit(f"g{c % n}")
         return True
 
     ok = sim.local or (yield from scores(0))
@@ -57,7 +59,7 @@ def issue_state(sim):
             break
         if not (yield ("wait", f"update{c & 1}", c >> 1)):
             break
-        sim.mma({("B", c % STAGES): c, **{("W", q): c for q in Q4}},
+        sim.mma({("B", c % STAGES): c, **{("W", w): c for w in range(SPLIT_WARPS)}},
                 {("S", q): (("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
         sim.commit("s")
         for _ in range(2 if sim.local else 1):
@@ -69,8 +71,8 @@ def issue_state(sim):
             ng += ok
     sim.commit("last0")
     yield ("drain", "last0", 0)
-    if ng:
-        yield ("drain", "g", ng - 1)
+    for c in range(max(0, ng - sim.g_buffers), ng):
+        yield ("drain", f"g{c % sim.g_buffers}", c // sim.g_buffers)
     if ns:
         yield ("drain", "s", ns - 1)
 
@@ -83,10 +85,9 @@ def issue_outputs(sim):
             break
         if c >= 1 and sim.plant != "no_yread" and not (yield ("wait", "yread", c - 1)):
             break
-        sim.mma({("C", c % STAGES): c, **{("SB", c % sim.copies_of_s, q): c for q in Q4}},
+        sim.mma({("C", c % STAGES): c, **{("SB", q): c for q in Q4}},
                 {("YI", q): (None, c) for q in Q4}, f"Yi({c})")
-        if sim.copies_of_s == 1:
-            sim.commit("cs")
+        sim.commit("cs")
         if not (yield ("wait", f"mready{c % sim.m_buffers}", c // sim.m_buffers)):
             break
         sim.mma({("X", c % STAGES): c, **{("M", c % sim.m_buffers, w): c for w in range(M_WARPS)}},
@@ -120,15 +121,14 @@ def copier(sim):
         yield ("drain", f"zfull{c & 1}", c >> 1)
 
 
-def gates(sim, w):
-    """A warp per head, or two taking one head's chunks in turn."""
-    head, turn = (w, 1) if sim.heads == 2 else (0, 2)
-    for c in range(0 if sim.heads == 2 else w, sim.nch, turn):
+def gates(sim):
+    for c in range(sim.nch):
         gs = c % GATE_STAGES
-        if c >= GATE_STAGES and not (yield ("wait", f"ydone{gs}", c // GATE_STAGES - 1)):
-            return
-        sim.write(("GT", gs, head), c, f"gates{w}")
-        yield None
+        for head in range(sim.heads):
+            if head == 0 and c >= GATE_STAGES and not (yield ("wait", f"ydone{gs}", c // GATE_STAGES - 1)):
+                return
+            sim.write(("GT", gs, head), c, "gates")
+            yield None
         sim.b[f"gates{gs}"].arrive()
 
 
@@ -150,19 +150,14 @@ def state(sim, q):
         read_gates(sim, c, who)
         if sim.local:
             sim.b[f"ydone{c % GATE_STAGES}"].arrive()
-        elif sim.plant == "late_copy":
-            pass
-        elif sim.copies_of_s == 2:
-            if c >= 2 and not (ok := (yield ("wait", f"mx{c & 1}", (c >> 1) - 1))):
-                break
-        elif c >= 1 and not (ok := (yield ("wait", "cs", c - 1))):
+        elif c >= 1 and sim.plant != "late_copy" and not (ok := (yield ("wait", "cs", c - 1))):
             break
         if c >= 1 and not (ok := (yield ("wait", "s", c - 1))):
             break
         sim.read(("S", q), ("S", c), who)
         yield None
         if not sim.local:
-            sim.write(("SB", c % sim.copies_of_s, q), c, who)
+            sim.write(("SB", q), c, who)
         sim.write(("S", q), ("dec", c), who)
         yield None
         sim.b[f"update{c & 1}"].arrive()
@@ -209,17 +204,17 @@ def rows(sim):
 def scores(sim, w):
     who = f"m{w}"
     for c in range(sim.nch):
-        if not (yield gates_full(c)) or not (yield ("wait", "g", c)):
+        if not (yield gates_full(c)) or not (yield ("wait", f"g{c % sim.g_buffers}", c // sim.g_buffers)):
             return
         m = c % sim.m_buffers
         if c >= sim.m_buffers and sim.plant != "no_mx" and not (yield ("wait", f"mx{m}", c // sim.m_buffers - 1)):
             return
         for _ in range(2):
-            sim.read(("G",), c, who)
+            sim.read(("G", c % sim.g_buffers), c, who)
             read_gates(sim, c, who)
             sim.write(("M", m, w), c, who)
             yield None
-        sim.b["mread"].arrive()
+        sim.b[f"mread{c % sim.g_buffers}"].arrive()
         sim.b[f"mready{m}"].arrive()
 
 
@@ -245,11 +240,11 @@ def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, local=False,
     sim = Scan(nch, heads, gated, plant, local)
     rng = random.Random(seed)
     roles = {"state issue": issue_state(sim), "output issue": issue_outputs(sim), "copier": copier(sim)}
-    roles.update({f"gates{w}": gates(sim, w) for w in (0, 1)})
+    roles["gates"] = gates(sim)
     roles.update({f"state{q}": state(sim, q) for q in Q4})
     roles.update({f"out{w}": outputs(sim, w) for w in range(Y_WARPS)})
     roles.update({f"m{w}": scores(sim, w) for w in range(M_WARPS)})
-    roles.update({f"split{q}": split(sim, q) for q in Q4})
+    roles.update({f"split{w}": split(sim, w) for w in range(SPLIT_WARPS)})
     roles["rows"] = rows(sim)
     if local:
         roles = {k: v for k, v in roles.items() if k in ("state issue", "copier") or k.startswith(("gates", "state", "split"))}
