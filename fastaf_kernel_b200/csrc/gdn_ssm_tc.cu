@@ -520,14 +520,23 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // A lane holds tokens 2 lane and 2 lane + 1 of a chunk; one turn per chunk and head.  dt
         // is loaded two turns ahead, and its lines are brought into L2 before that: with one turn
         // between a load and its use, HBM's latency was every chunk's time.
-        float d[3][2];
-        auto fetch = [&](int i, float (&to)[2]) {
-            const int k = PAIR ? i & 1 : 0;
+        // (The loads are raw and unconditional: converted or masked where they are issued, each
+        // waits for the one before it.)
+        uint32_t d[3][2];
+        const bool wide = p.dt_dtype != 1;
+        auto fetch = [&](int i, uint32_t (&to)[2]) {
             const int64_t t = s0 + static_cast<int64_t>(i / kHeads) * kL + 2 * lane;
-            const int64_t at = t * p.dt_stride + (lone ? h0 : h0 + k);
-            to[0] = t < s1 ? load_scalar(p.dt, at, p.dt_dtype) : 0.0f;
-            to[1] = t + 1 < s1 ? load_scalar(p.dt, at + p.dt_stride, p.dt_dtype) : 0.0f;
+            const int64_t at = (t < s1 ? t : s1 - 1) * p.dt_stride + (PAIR && !lone ? h0 + (i & 1) : h0);
+            const int64_t next = t + 1 < s1 ? at + p.dt_stride : at;
+            if (wide) {
+                to[0] = static_cast<const uint32_t *>(p.dt)[at];
+                to[1] = static_cast<const uint32_t *>(p.dt)[next];
+            } else {
+                to[0] = static_cast<const uint16_t *>(p.dt)[at];
+                to[1] = static_cast<const uint16_t *>(p.dt)[next];
+            }
         };
+        auto value = [&](uint32_t raw) { return __uint_as_float(wide ? raw : raw << 16); };
         auto ahead = [&](int c) {
             const int64_t t = s0 + static_cast<int64_t>(c) * kL + 2 * lane, at = t * p.dt_stride + h0;
             const char *line = static_cast<const char *>(p.dt) + (p.dt_dtype == 1 ? 2 : 4) * at;
@@ -544,8 +553,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             fetch(i + 2, d[2]);
             if (head == 0) ahead(c + kPrefetch);
             const float b0 = PAIR && head ? bias[kHeads - 1] : bias[0];
-            const float d0 = t0 < s1 ? softplus_series(d[0][0] + b0) : 0.0f;
-            const float d1 = t0 + 1 < s1 ? softplus_series(d[0][1] + b0) : 0.0f;
+            const float d0 = t0 < s1 ? softplus_series(value(d[0][0]) + b0) : 0.0f;
+            const float d1 = t0 + 1 < s1 ? softplus_series(value(d[0][1]) + b0) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 d[0][k] = d[1][k];
