@@ -313,22 +313,25 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 
     // this thread's state row: of head h0, or for the second half of a pair of head h0 + 1
     const int hrow = PAIR ? row >> 6 : 0;
-    const bool dead = lone && hrow == 1;
-    const int64_t state_at =
-        ((n * p.heads + h0 + hrow) * p.head_size + (PAIR ? row & 63 : row)) * static_cast<int64_t>(kSsmState);
-    const int64_t end_at = (slot * args.slabs + slab) * kRows + row;      // the row in the segments' workspace
+    // the slab's 128 state rows, one after the other in memory (64 for a lone head)
+    const int64_t state_at = (n * p.heads + h0) * p.head_size * static_cast<int64_t>(kSsmState);
+    const int64_t end_at = (slot * args.slabs + slab) * kRows;      // their place in the segments' workspace
     // the slab's columns in the rows of x, z and y (a lone head's twice: the copy is not stored)
     const int xc0 = h0 * p.head_size, xc1 = lone ? xc0 : xc0 + 64;
 
     if (nch == 0) {
         // An empty sequence keeps its state (or starts at zero).
-        const int64_t base = (n * p.heads + h0) * p.head_size * static_cast<int64_t>(kSsmState);
         const int vecs = (lone ? 64 : kRows) * kSsmState / 4;
         for (int i = tid; i < vecs; i += kThreads)
-            reinterpret_cast<float4 *>(p.new_state + base)[i] =
-                p.state ? reinterpret_cast<const float4 *>(p.state + base)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            reinterpret_cast<float4 *>(p.new_state + state_at)[i] =
+                p.state ? reinterpret_cast<const float4 *>(p.state + state_at)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
+    // where the state starts from, and its lines on their way into L2 meanwhile
+    const float *const first = seg == 0 ? (p.state ? p.state + state_at : nullptr)
+                               : LOCAL  ? nullptr
+                                        : args.ends + (end_at - static_cast<int64_t>(args.slabs) * kRows) * kSsmState;
+    if (first && tid < (lone ? 64 : kRows) * kSsmState / 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(first + tid * 32));
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < kStages; ++i) {
@@ -510,13 +513,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         __syncwarp();
     } else if (warp == 2) {
         // -------------------------------------------------------------- gates
-        float negA2[kHeads], bias[kHeads];       // log2 decay of dt' = 1
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) {
-            const int h = lone ? h0 : h0 + k;
-            negA2[k] = -expf(load_scalar(p.A_log, h, p.param_dtype)) * 1.4426950408889634f;
-            bias[k] = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
-        }
         // A lane holds tokens 2 lane and 2 lane + 1 of a chunk; one turn per chunk and head.  dt
         // is loaded two turns ahead, and its lines are brought into L2 before that: with one turn
         // between a load and its use, HBM's latency was every chunk's time.
@@ -545,6 +541,15 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         };
         fetch(0, d[0]);
         fetch(1, d[1]);
+        float negA2[kHeads], bias[kHeads];       // log2 decay of dt' = 1
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            const int h = lone ? h0 : h0 + k;
+            negA2[k] = load_scalar(p.A_log, h, p.param_dtype);
+            bias[k] = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) negA2[k] = -expf(negA2[k]) * 1.4426950408889634f;
         for (int c = 1; c < kPrefetch; ++c) ahead(c);
 #pragma unroll 1
         for (int i = 0; i < nch * kHeads; ++i) {
@@ -596,22 +601,27 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         }
     } else if (warp >= 4 && warp < 8) {
         // -------------------------------------------------------------- state path
-        const float *first = seg == 0 ? (p.state && !dead ? p.state + state_at : nullptr)
-                             : LOCAL  ? nullptr
-                                      : args.ends + (end_at - static_cast<int64_t>(args.slabs) * kRows) * kSsmState;
-        float *const after = LOCAL ? args.ends + end_at * kSsmState : (last && !dead ? p.new_state + state_at : nullptr);
+        // A fragment's registers hold two neighbouring columns of rows lane / 4 and lane / 4 + 8:
+        // the state goes in and out in whole 32-byte sectors.
+        const int64_t frag = static_cast<int64_t>(lane_base + (lane >> 2)) * kSsmState + 2 * (lane & 3);
+        float *const after = LOCAL ? args.ends + end_at * kSsmState : (last ? p.new_state + state_at : nullptr);
         float product = 1.0f;           // of the segment's decays
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-            uint32_t r[32];
+        for (int u = 0; u < 8; ++u) {                   // 16 rows x 32 columns
+            const int lh = u >> 2, q = u & 3;
+            const bool there = first != nullptr && !(lone && lane_base >= 64);
+            const float *from = first + frag + lh * 16 * kSsmState + 32 * q;
+            uint32_t r[16];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                const float4 x = first ? *reinterpret_cast<const float4 *>(first + 32 * q + j)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-                r[j] = __float_as_uint(x.x); r[j + 1] = __float_as_uint(x.y);
-                r[j + 2] = __float_as_uint(x.z); r[j + 3] = __float_as_uint(x.w);
-            }
-            tmem_st32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float2 v = there ? *reinterpret_cast<const float2 *>(from + k * 8 * kSsmState + 8 * m)
+                                           : make_float2(0.0f, 0.0f);
+                    r[4 * m + 2 * k] = __float_as_uint(v.x);
+                    r[4 * m + 2 * k + 1] = __float_as_uint(v.y);
+                }
+            tmem_st_acc32(tmem_addr(tm, lane_base + 16 * lh, TM::S + 32 * q), r);
         }
         tmem_wait_st();
         bool ok = true;
@@ -652,21 +662,21 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);
         }
-        if (LOCAL) args.decays[end_at] = product;
-        if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS)) {
+        if (LOCAL) args.decays[end_at + row] = product;
+        if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS) && after && !(lone && lane_base >= 64 && !LOCAL)) {
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
-                uint32_t r[32];
-                tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
+            for (int u = 0; u < 8; ++u) {
+                const int lh = u >> 2, q = u & 3;
+                float *to = after + frag + lh * 16 * kSsmState + 32 * q;
+                uint32_t r[16];
+                tmem_ld_frag32(tmem_addr(tm, lane_base + 16 * lh, TM::S + 32 * q), r);
                 tmem_wait_ld_dep(r);
-                if (after) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4 *>(after + 32 * q + j) =
-                            make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
-                                        __uint_as_float(r[j + 3]));
-                }
-                __syncwarp();
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        *reinterpret_cast<float2 *>(to + k * 8 * kSsmState + 8 * m) =
+                            make_float2(__uint_as_float(r[4 * m + 2 * k]), __uint_as_float(r[4 * m + 2 * k + 1]));
             }
         }
     } else if (!LOCAL && ((warp >= 8 && warp < 12) || (warp >= 20 && warp < 24))) {
