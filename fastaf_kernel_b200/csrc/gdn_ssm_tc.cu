@@ -210,6 +210,25 @@ struct Waiter {
         tc_fence_after();
         return true;
     }
+    // The same with no call in it: for a wait across which a warp keeps many registers.
+    __device__ __forceinline__ bool warp_inline(uint32_t bar, uint32_t phase, int site) const {
+        bool ok = mbar_try_wait(bar, phase & 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+            WaitControl *ctl = wait_control();
+            const uint64_t t0 = global_timer_ns();
+            const uint32_t hint = ctl->limit < kMaxSuspendNs ? static_cast<uint32_t>(ctl->limit) : kMaxSuspendNs;
+            while (!ok && !ctl->abort) {
+                ok = mbar_try_wait_hint(bar, phase & 1, hint);
+                if (!ok && global_timer_ns() - t0 > ctl->limit) {
+                    if (ctl->status) atomicCAS(ctl->status, 0, site);
+                    ctl->abort = 1;
+                }
+            }
+            if (!__all_sync(0xffffffffu, ok)) return false;
+        }
+        tc_fence_after();
+        return true;
+    }
     __device__ __forceinline__ void drain(uint32_t bar, uint32_t phase, int site) const {
         wait_own(bar, key(phase, site));
     }
@@ -826,7 +845,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
             if (!gates_full(c)) break;
             if (!wait.warp(bar(bars.full[st]), c / kStages, kSsmTma)) break;
-            if (c >= 1 && !wait.warp(bar(bars.s), c - 1, kSsmS)) break;
             const uint32_t xs = sbase + OFF_STAGE + st * STAGE + ST_X;
             uint32_t wh[8], wl[8];
             {
@@ -861,6 +879,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 hi[k] = mul_bf2(x[k], wh[k >> 1]);
                 lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
             }
+            // (the update of the chunk before has read the operand; all but the stores is done by then)
+            if (c >= 1 && !wait.warp_inline(bar(bars.s), c - 1, kSsmS)) break;
             tmem_st_frag32(tmem_addr(tm, p0, TM::W), hi);
             tmem_st_frag32(tmem_addr(tm, p0, TM::W + 32), lo);
             tmem_wait_st();

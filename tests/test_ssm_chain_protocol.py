@@ -224,13 +224,13 @@ def split(sim, q):
         st = c % STAGES
         if not (yield gates_full(c)) or not (yield ("wait", f"full{st}", c // STAGES)):
             return
-        if c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
-            return
         read_gates(sim, c, who)
         if sim.local:
             sim.b[f"ydone{c % GATE_STAGES}"].arrive()
         sim.read(("X", st), c, who)
         yield None
+        if c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
+            return
         sim.write(("W", q), c, who)
         yield None
         sim.b[f"update{c & 1}"].arrive()
