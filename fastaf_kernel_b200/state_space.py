@@ -37,21 +37,28 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _on(index: int, named) -> None:
-    """Every given tensor is a CUDA tensor on device ``index``."""
-    for name, t in named:
-        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index or index < 0):
-            if not isinstance(t, torch.Tensor):
-                raise TypeError(f"{name} must be a torch.Tensor")
-            if not t.is_cuda:
-                raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got {t.device}")
-            raise ValueError(f"{name} is on {t.device}, expected the device of x (cuda:{index})")
-
-
-def _index(x) -> int:
-    if not isinstance(x, torch.Tensor):
-        raise TypeError("x must be a torch.Tensor")
-    return x.get_device()
+def _device_of(names, tensors) -> int:
+    """The CUDA device index of the first tensor, which all the given ones are on."""
+    try:
+        index = tensors[0].get_device()
+        if index >= 0:
+            for t in tensors:
+                if t is not None and t.get_device() != index:
+                    break
+            else:
+                return index
+    except AttributeError:
+        pass
+    for name, t in zip(names.split(), tensors):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got {t.device}")
+        if t.get_device() != tensors[0].get_device():
+            raise ValueError(f"{name} is on {t.device}, expected {tensors[0].device}")
+    raise TypeError("x must be a torch.Tensor")
 
 
 def _call(fn, index: int, args) -> None:
@@ -208,8 +215,7 @@ def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     side, such as q, k and v for ``kernel`` or x, B and C for ``ssm_prefill``; y (and
     ``output``) is then a tuple of [T, width] tensors.  new_state must not overlap state.
     """
-    index = _index(x)
-    _on(index, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    index = _device_of("x weight bias state", (x, weight, bias, state))
     if x.dim() != 2:
         raise ValueError("x must be [T, channels]")
     cu, N = _cu(cu_seqlens, x.shape[0], x, validate)
@@ -224,8 +230,7 @@ def conv_decode(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 new_state: Optional[torch.Tensor] = None) -> Tuple[Outputs, torch.Tensor]:
     """``conv_prefill`` for one token of each sequence: x [B, C], state [B, W-1, C] bf16 or
     None.  Returns (y [B, C], new_state); pass ``new_state=state`` to update it in place."""
-    index = _index(x)
-    _on(index, (("x", x), ("weight", weight), ("bias", bias), ("state", state)))
+    index = _device_of("x weight bias state", (x, weight, bias, state))
     if x.dim() != 2:
         raise ValueError("x must be [B, channels]")
     head, tail, sizes, y, new_state, held = _conv(x, weight, bias, state, x.shape[0], activation, split, output,
@@ -247,26 +252,27 @@ def ssm_method(total_tokens: int, method: str = "auto", num_seqs: int = 1) -> st
 
 def _ssm(x, dt, A_log, B, C, D, dt_bias, state, z, num_seqs, output, new_state):
     """The checks and conversions of both scan calls."""
-    *lead, H, P = x.shape
+    shape, Bs, ds = x.shape, B.shape, dt.shape
+    rank, H, P = len(shape), shape[-2], shape[-1]
     if P != 64 and P != 128:
         raise NotImplementedError(f"head_size={P} is not supported (64 or 128)")
-    if B.dim() != x.dim() or B.shape[:-2] != x.shape[:-2]:
-        raise ValueError(f"B must be [..., groups, state_size] with x's leading shape {lead}, got {list(B.shape)}")
-    G, S = B.shape[-2:]
+    if len(Bs) != rank or Bs[:-2] != shape[:-2]:
+        raise ValueError(f"B must be [..., groups, state_size] with the leading sizes of x {list(shape)}, got {list(Bs)}")
+    G, S = Bs[-2], Bs[-1]
     if S != 128:
         raise NotImplementedError(f"state_size={S} is not supported (only 128)")
-    if C.shape != B.shape:
-        raise ValueError(f"C shape {list(C.shape)} must equal B shape {list(B.shape)}")
+    if C.shape != Bs:
+        raise ValueError(f"C shape {list(C.shape)} must equal B shape {list(Bs)}")
     if H == 0 or G == 0 or H % G:
         raise ValueError(f"{H} heads must be a positive multiple of {G} groups")
-    if dt.shape != x.shape[:-1]:
-        raise ValueError(f"dt must be {list(x.shape[:-1])}, got {list(dt.shape)}")
-    for name, t in (("A_log", A_log), ("D", D), ("dt_bias", dt_bias)):
-        if t is not None and t.shape != (H,):
-            raise ValueError(f"{name} must be [heads] = [{H}]")
-    if z is not None and z.shape != x.shape:
-        raise ValueError(f"z shape {list(z.shape)} must equal x shape {list(x.shape)}")
-    shape = x.shape
+    if ds != shape[:-1]:
+        raise ValueError(f"dt must be {list(shape[:-1])}, got {list(ds)}")
+    per_head = (H,)
+    if A_log.shape != per_head or (D is not None and D.shape != per_head) or (
+            dt_bias is not None and dt_bias.shape != per_head):
+        raise ValueError(f"A_log, D and dt_bias must be [heads] = [{H}]")
+    if z is not None and z.shape != shape:
+        raise ValueError(f"z shape {list(z.shape)} must equal x shape {list(shape)}")
     x, xp, sx = _rows("x", x, H * P)
     B, Bp, sB = _rows("B", B, G * S)
     C, Cp, sC = _rows("C", C, G * S)
@@ -312,9 +318,7 @@ def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch
     tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what
     ``ssm_method`` reports).
     """
-    index = _index(x)
-    _on(index, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
-                ("state", state), ("z", z)))
+    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C, D, dt_bias, state, z))
     if x.dim() != 3:
         raise ValueError("x must be [T, heads, head_size]")
     if method not in _METHODS:
@@ -333,9 +337,7 @@ def ssm_decode(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.
     """One step of ``ssm_prefill``'s scan for each sequence: x, z [B, 1, H, P]; dt [B, 1, H];
     B, C [B, 1, G, 128]; state [B, H, P, 128] fp32 or None.  Returns (y [B, 1, H, P] bf16,
     new_state); pass ``new_state=state`` to update the state in place."""
-    index = _index(x)
-    _on(index, (("x", x), ("dt", dt), ("A_log", A_log), ("B", B), ("C", C), ("D", D), ("dt_bias", dt_bias),
-                ("state", state), ("z", z)))
+    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C, D, dt_bias, state, z))
     if x.dim() != 4 or x.shape[1] != 1:
         raise ValueError("x must be [B, 1, heads, head_size]")
     batch = x.shape[0]
