@@ -69,7 +69,6 @@ constexpr int kThreads = 896;
 constexpr int kRows = 128;          // state rows of a CTA
 constexpr int kStages = 3;          // of C, B, x
 constexpr int kGateStages = 4;
-constexpr int64_t kMinSegment = 512;    // tokens a sequence is cut into at least
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
 constexpr int kMWarps = 3, kYWarps = 8;
 constexpr int kUpdateWarps = 12;     // of the state path and the split
@@ -975,16 +974,27 @@ cudaError_t launch_passes(const CUtensorMap *maps, const TcArgs &a, int64_t slot
     return launch_pass<PAIR, false>(maps, a, slots, stream);
 }
 
-// Tokens of a segment, or 0 for no cuts, of a call with `chains` (sequence, slab) pairs: as
-// many segments of a sequence of mean length as fill the SMs once, so that few long prompts
-// use all of them.  With more chains than half the SMs the local pass costs more than the
-// idle SMs.
+// Tokens of a segment, or 0 for no cuts, of a call with `chains` (sequence, slab) pairs, so that
+// few long prompts use all SMs.  A sequence of mean length takes about 1.15 us a chunk as one;
+// in k segments, at most as many as fill the SMs once, a segment's chunks take 0.93 us more
+// (the local pass), and the two launches more about 14 us.  The k with the least time: 1 x
+// 16,384 tokens in 32 chains 294 us uncut and 147 in four segments, 1 x 2048 in 4 chains 67
+// and 33 in eight; 1 x 1024 in 32 chains stays whole at 28 us (36 in two), and so does 2 x 4096
+// in 64 chains at 84 us (87).
 int64_t segment_tokens(int64_t tokens, int64_t num_seqs, int64_t chains, int sms) {
-    const int64_t cuts = sms / chains;
-    if (cuts < 2) return 0;
-    int64_t s = (tokens + num_seqs * cuts - 1) / (num_seqs * cuts);
-    s = (s + kL - 1) / kL * kL;
-    return s < kMinSegment ? kMinSegment : s;
+    const int64_t chunks = (tokens + num_seqs * kL - 1) / (num_seqs * kL);
+    const int64_t most = sms / chains < chunks / 4 ? sms / chains : chunks / 4;
+    int64_t best = 0;
+    double least = 1.15 * static_cast<double>(chunks);
+    for (int64_t k = 2; k <= most; ++k) {
+        const int64_t part = (chunks + k - 1) / k;
+        const double time = (1.15 + 0.93) * static_cast<double>(part) + 14.0;
+        if (time < least) {
+            least = time;
+            best = part * kL;
+        }
+    }
+    return best;
 }
 
 }  // namespace

@@ -329,8 +329,9 @@ CASES = [
     ([200, 0, 7, 128], 6, 2, 64, True, True, False),
     ([0, 3, 70, 0], 4, 4, 64, False, True, True),             # one head a group
     ([517], 2, 2, 128, True, False, False),
-    ([1700, 0, 65, 600], 2, 1, 128, False, True, True),       # cut into segments: four, one, one, two
-    ([1300, 640, 2000], 3, 1, 64, True, True, False),
+    ([4000, 0, 65, 1500], 2, 1, 128, False, True, True),       # cut into segments, sequences of mean length
+    ([1300, 1640, 2000], 3, 1, 64, True, True, False),
+    ([1, 4900, 333], 1, 1, 64, False, False, True),
 ]
 
 
