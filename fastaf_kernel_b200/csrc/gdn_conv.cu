@@ -158,7 +158,7 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
         return;
     }
     const int t0 = static_cast<int>(tile * run);
-    const int t1 = static_cast<int>(t0 + run < T ? t0 + run : T);
+    int t1 = static_cast<int>(t0 + run < T ? t0 + run : T);
     __shared__ uint2 ring[kBatches * kBatchRows][kConvThreads];
     const uint32_t slot0 = msync::smem_addr(&ring[0][threadIdx.x]);
     const __nv_bfloat16 *ahead = x + t0 * p.x_stride;      // the next row to copy, row t0 + copied
@@ -190,7 +190,7 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
     }
     int s0 = cu[n];
     s0 = s0 < 0 ? 0 : (s0 > t0 ? t0 : s0);
-    int next = n + 1 < N ? cu[n + 1] : 0x7fffffff;      // (behind the last sequence there is none to go on to)
+    int next = cu[n + 1];
     // the rows in front of token t of sequence n that starts at s0
     Row win[W - 1];
     auto window = [&](int t) {
@@ -224,10 +224,11 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
 #pragma unroll 1
             for (int u = 0; u < kBatchRows && t + u < t1; ++u) {
                 if (t + u >= next) {       // the next sequence that has tokens starts here
-                    do {
-                        ++n;
-                        next = n + 1 < N ? cu[n + 1] : 0x7fffffff;
-                    } while (t + u >= next);
+                    while (++n < N && t + u >= (next = cu[n + 1])) {}
+                    if (n >= N) {              // rows behind the last one stay as they are
+                        t1 = t;
+                        break;
+                    }
                     s0 = t + u;
                     window(t + u);
                 }
@@ -235,6 +236,7 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
             }
         }
     }
+    msync::cp_async_wait<0>();
 }
 
 // One token of each sequence; new_state may be state (a thread reads its own words of all

@@ -11,7 +11,7 @@
 namespace {
 
 constexpr int64_t kMaxStride = 0x7fffffff;
-constexpr int64_t kMaxRows = int64_t(1) << 31;
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256;      // (a run behind the last row still counts in 32 bits)
 // The tensor-core scan takes a 64-token chunk of every sequence however few tokens it has, the
 // token-serial one its tokens one after the other: with 32 heads of 128, 16 sequences of 4
 // tokens 35 and 25 us, of 8 tokens 36 and 38, of 16 tokens 37 and 64.
@@ -40,6 +40,11 @@ bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return x < y + nb && y < x + na;
 }
 
+// Whether `rows` rows of `width` bf16 elements, `stride` apart, overlap `bytes` bytes at `out`.
+bool rows_overlap(const void *p, int64_t rows, int64_t stride, int64_t width, const void *out, size_t bytes) {
+    return p && rows > 0 && ranges_overlap(p, static_cast<size_t>((rows - 1) * stride + width) * 2, out, bytes);
+}
+
 bool known_dtype(int d) { return d == GDN_DTYPE_F32 || d == GDN_DTYPE_BF16; }
 
 // A row stride in elements: 0 stands for packed rows of `width`; anything else has to hold
@@ -61,7 +66,7 @@ int conv_args(gdn::ConvArgs &p, const void *x, int64_t x_row_stride, const void 
     if (activation != GDN_ACTIVATION_NONE && activation != GDN_ACTIVATION_SILU)
         return fail(GDN_ERR_INVALID_ARGUMENT, "unknown activation %d", activation);
     if (rows < 0 || rows >= kMaxRows || num_seqs < 0 || num_seqs >= kMaxRows)
-        return fail(GDN_ERR_INVALID_ARGUMENT, "tokens and sequences must be in [0, 2^31)");
+        return fail(GDN_ERR_INVALID_ARGUMENT, "tokens and sequences must be in [0, 2^31 - 256)");
     const int64_t xs = row_stride(x_row_stride, channels);
     if (xs < 0 || xs % 8 != 0)
         return fail(GDN_ERR_INVALID_ARGUMENT, "x row stride %lld must be 0 or a multiple of 8 in [channels=%lld, 2^31)",
@@ -90,6 +95,12 @@ int conv_args(gdn::ConvArgs &p, const void *x, int64_t x_row_stride, const void 
         for (int j = 0; j < num_outputs; ++j)
             if (!outputs[j] || !aligned16(outputs[j]))
                 return fail(GDN_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned addresses");
+        for (int j = 0; j < num_outputs; ++j) {
+            const size_t bytes = static_cast<size_t>(rows * output_widths[j]) * 2;
+            bool hit = rows_overlap(x, rows, xs, channels, outputs[j], bytes);
+            for (int k = 0; k < j; ++k) hit |= rows_overlap(outputs[k], rows, output_widths[k], output_widths[k], outputs[j], bytes);
+            if (hit) return fail(GDN_ERR_INVALID_ARGUMENT, "outputs must not overlap x or each other");
+        }
     }
     p.x = x;
     p.x_stride = xs;
@@ -128,7 +139,7 @@ int ssm_args(gdn::SsmArgs &p, const void *x, int64_t x_row_stride, const void *d
     if (!known_dtype(dt_dtype) || !known_dtype(param_dtype))
         return fail(GDN_ERR_INVALID_ARGUMENT, "unknown dtype code (dt %d, params %d)", dt_dtype, param_dtype);
     if (rows < 0 || rows >= kMaxRows || num_seqs < 0 || num_seqs >= kMaxRows)
-        return fail(GDN_ERR_INVALID_ARGUMENT, "tokens and sequences must be in [0, 2^31)");
+        return fail(GDN_ERR_INVALID_ARGUMENT, "tokens and sequences must be in [0, 2^31 - 256)");
     const int64_t wide = static_cast<int64_t>(num_heads) * head_size, bc = static_cast<int64_t>(num_groups) * 128;
     p.x_stride = row_stride(x_row_stride, wide);
     p.z_stride = row_stride(z_row_stride, wide);
@@ -147,6 +158,10 @@ int ssm_args(gdn::SsmArgs &p, const void *x, int64_t x_row_stride, const void *d
         if (!x || !dt || !B || !C || !output) return fail(GDN_ERR_INVALID_ARGUMENT, "null x, dt, B, C or output");
         if (!aligned16(x) || !aligned16(B) || !aligned16(C) || !aligned16(z) || !aligned16(output))
             return fail(GDN_ERR_INVALID_ARGUMENT, "x, B, C, z and output must be 16-byte aligned");
+        const size_t bytes = static_cast<size_t>(rows * wide) * 2;
+        if (rows_overlap(x, rows, p.x_stride, wide, output, bytes) || rows_overlap(z, rows, p.z_stride, wide, output, bytes) ||
+            rows_overlap(B, rows, p.B_stride, bc, output, bytes) || rows_overlap(C, rows, p.C_stride, bc, output, bytes))
+            return fail(GDN_ERR_INVALID_ARGUMENT, "output must not overlap x, z, B or C");
     }
     p.x = x;
     p.dt = dt;

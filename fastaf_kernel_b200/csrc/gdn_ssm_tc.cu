@@ -183,6 +183,21 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t key) {
         }
     }
 }
+// The same without suspending the thread: a suspended wait ends late, but not early, so that
+// this one, for the first copies, is what notices a limit of a microsecond or less.
+__device__ __noinline__ bool wait_polled(uint32_t bar, uint32_t key) {
+    WaitControl *ctl = wait_control();
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_test_wait(bar, key & 1)) {
+        if (ctl->abort) return false;
+        if (global_timer_ns() - t0 > ctl->limit) {
+            if (ctl->status) atomicCAS(ctl->status, 0, static_cast<int>(key >> 1));
+            ctl->abort = 1;
+            return false;
+        }
+    }
+    return true;
+}
 // This CTA's own copies and MMAs, also after a give-up.
 __device__ __noinline__ void wait_own(uint32_t bar, uint32_t key) {
     const uint64_t t0 = global_timer_ns();
@@ -248,6 +263,12 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// The larger of the two, or NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
 }
 __device__ __forceinline__ uint64_t bits2(uint32_t lo, uint32_t hi) {
     return f2(__uint_as_float(lo), __uint_as_float(hi));
@@ -423,7 +444,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             ++ng;
             return true;
         };
-        bool ok = LOCAL || scores(0);
+        bool ok = __all_sync(0xffffffffu, wait_polled(bar(bars.full[0]), Waiter::key(0, kSsmTma)));
+        if (!LOCAL && ok) ok = scores(0);
 #pragma unroll 1
         for (int c = 0; ok && c < nch; ++c) {
             const uint32_t st = (c % kStages) * kSt;
@@ -502,8 +524,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const bool fetched = lane < (gated ? 8 : 6) && !(LOCAL && lane < 2);
         int issued = 0, zissued = 0;
 #pragma unroll 1
- #pragma unroll 1
-       for (int c = 0; c < nch; ++c) {
+        for (int c = 0; c < nch; ++c) {
             const int t = static_cast<int>(s0) + c * kL;
             const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
             if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
@@ -588,7 +609,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             // (a decay below 2^-150 is zero in fp32; without the bound one such token would cost
             // the sums behind it their precision)
             const float nA = PAIR && head ? negA2[kHeads - 1] : negA2[0];
-            const float a0 = fmaxf(nA * d0, -160.0f), a1 = fmaxf(nA * d1, -160.0f);
+            const float a0 = max_nan(nA * d0, -160.0f), a1 = max_nan(nA * d1, -160.0f);
             float up = a0 + a1, down = up;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {

@@ -37,20 +37,25 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _device_of(names, tensors) -> int:
+def _device_of(names, required, optional) -> int:
     """The CUDA device index of the first tensor, which all the given ones are on."""
+    tensors = required + optional
     try:
         index = tensors[0].get_device()
         if index >= 0:
-            for t in tensors:
-                if t is not None and t.get_device() != index:
+            for t in required:
+                if t.get_device() != index:
                     break
             else:
-                return index
+                for t in optional:
+                    if t is not None and t.get_device() != index:
+                        break
+                else:
+                    return index
     except AttributeError:
         pass
-    for name, t in zip(names.split(), tensors):
-        if t is None:
+    for i, (name, t) in enumerate(zip(names.split(), tensors)):
+        if t is None and i >= len(required):
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
@@ -213,9 +218,10 @@ def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 
     ``split`` gives the widths of up to four packed tensors that take the channels side by
     side, such as q, k and v for ``kernel`` or x, B and C for ``ssm_prefill``; y (and
-    ``output``) is then a tuple of [T, width] tensors.  new_state must not overlap state.
+    ``output``) is then a tuple of [T, width] tensors.  Outputs must not overlap x or each
+    other, nor new_state state.
     """
-    index = _device_of("x weight bias state", (x, weight, bias, state))
+    index = _device_of("x weight bias state", (x, weight), (bias, state))
     if x.dim() != 2:
         raise ValueError("x must be [T, channels]")
     cu, N = _cu(cu_seqlens, x.shape[0], x, validate)
@@ -230,7 +236,7 @@ def conv_decode(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 new_state: Optional[torch.Tensor] = None) -> Tuple[Outputs, torch.Tensor]:
     """``conv_prefill`` for one token of each sequence: x [B, C], state [B, W-1, C] bf16 or
     None.  Returns (y [B, C], new_state); pass ``new_state=state`` to update it in place."""
-    index = _device_of("x weight bias state", (x, weight, bias, state))
+    index = _device_of("x weight bias state", (x, weight), (bias, state))
     if x.dim() != 2:
         raise ValueError("x must be [B, channels]")
     head, tail, sizes, y, new_state, held = _conv(x, weight, bias, state, x.shape[0], activation, split, output,
@@ -312,13 +318,13 @@ def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch
     H / G consecutive heads of a group; A_log, D, dt_bias [H] (D and dt_bias may be None);
     state [N, H, P, 128] fp32 or None for zeros; cu_seqlens [N+1] as for ``kernel``.  Returns
     (y [T, H, P] bf16, new_state [N, H, P, 128] fp32); a sequence of length 0 keeps its
-    state.  new_state must not overlap state.
+    state.  ``output`` must not overlap x, z, B or C, nor new_state state.
 
     ``method`` chooses the kernel: "tcgen05" (64-token chunks on the tensor cores, from 64
     tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what
     ``ssm_method`` reports).
     """
-    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C, D, dt_bias, state, z))
+    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C), (D, dt_bias, state, z))
     if x.dim() != 3:
         raise ValueError("x must be [T, heads, head_size]")
     if method not in _METHODS:
@@ -337,7 +343,7 @@ def ssm_decode(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.
     """One step of ``ssm_prefill``'s scan for each sequence: x, z [B, 1, H, P]; dt [B, 1, H];
     B, C [B, 1, G, 128]; state [B, H, P, 128] fp32 or None.  Returns (y [B, 1, H, P] bf16,
     new_state); pass ``new_state=state`` to update the state in place."""
-    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C, D, dt_bias, state, z))
+    index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C), (D, dt_bias, state, z))
     if x.dim() != 4 or x.shape[1] != 1:
         raise ValueError("x must be [B, 1, heads, head_size]")
     batch = x.shape[0]

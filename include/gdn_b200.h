@@ -298,7 +298,7 @@ GDN_API int gdn_decode_strided(const void *q, const void *k, const void *v, cons
  *
  * Requirements: width 2, 3 or 4; channels and every output width multiples of 8; 16-byte
  * aligned pointers (weight and bias: their element's alignment).  Outputs must not overlap
- * inputs.
+ * x or each other.  total_tokens and num_seqs below 2^31 - 256.
  */
 GDN_API int gdn_conv_prefill(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
                      int weight_dtype, const void *state, const int32_t *cu_seqlens, int64_t num_seqs,
@@ -339,9 +339,9 @@ GDN_API int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *wei
  *
  * Requirements: head_size 64 or 128, state_size 128, num_heads % num_groups == 0; x, z, B,
  * C, output, state and new_state 16-byte aligned and the row strides of x, z, B and C
- * multiples of 8.  The output must not overlap inputs.  A sequence's outputs and state
+ * multiples of 8.  The output must not overlap x, z, B or C.  A sequence's outputs and state
  * depend on its own rows alone.  Within a sequence, GDN_PREFILL_TCGEN05 lets an infinity or
- * NaN in x, B or C also reach the outputs of the tokens before it in its 64-token chunk.
+ * NaN in x, dt, B or C also reach the outputs of the tokens before it in its 64-token chunk.
  */
 GDN_API int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
                     const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,

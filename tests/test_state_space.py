@@ -590,3 +590,254 @@ def test_python_refusals():
         fk.ssm_prefill(*args, new_state=i["state"])
     with pytest.raises(ValueError):
         fk.ssm_decode(*args[:8])
+
+
+def test_required_tensors_are_named():
+    x = torch.zeros(4, 16, dtype=torch.bfloat16)
+    with pytest.raises((TypeError, ValueError)):
+        fk.conv_prefill(None, x, None, None, x)
+    with pytest.raises((TypeError, ValueError)):
+        fk.ssm_decode(None, x, x, x, x, None, None, None)
+
+
+@pytest.mark.parametrize("decode", [False, True])
+def test_conv_outputs_overlap_nothing(decode):
+    """x itself, its last bytes, or another output as an output: refused before any launch."""
+    lib = _lib.load()
+    base = dict(N=4, T=4, C=16, widths=(8, 8), state=None, new=1 << 20)
+    for over in (dict(x=1 << 16, outs=(1 << 16, 1 << 17)), dict(x=1 << 16, outs=(1 << 17, (1 << 16) + 112)),
+                 dict(x=1 << 16, outs=(1 << 17, (1 << 17) + 48)), dict(x=1 << 16, xs=64, outs=(1 << 17, (1 << 16) + 400))):
+        assert _conv_c(lib, decode=decode, **base, **over) == BAD
+        assert b"overlap" in lib.gdn_last_error()
+
+
+def test_scan_outputs_overlap_nothing():
+    lib = _lib.load()
+    at = lambda x=1 << 20, B=1 << 21, C=1 << 22, z=1 << 23, out=1 << 24: lib.gdn_ssm_decode(
+        x, 0, 1 << 16, 0, 1 << 17, B, 0, C, 0, None, None, z, 0, None, 3, 2, 1, 64, 128, 0, 0, out, 1 << 25, None)
+    for over in (dict(out=1 << 20), dict(out=(1 << 21) + 752), dict(out=(1 << 22) - 752), dict(out=(1 << 23) + 16)):
+        assert at(**over) == BAD
+        assert b"overlap" in lib.gdn_last_error()
+
+
+@pytest.mark.gpu
+def test_python_refuses_missing_and_overlapping_tensors():
+    x, w, b, st = _conv_inputs([4, 2], 16, 4)
+    cu = _cu([4, 2])
+    with pytest.raises(TypeError):
+        fk.conv_prefill(x, None, b, st, cu)
+    with pytest.raises(ValueError):
+        fk.conv_prefill(x, w, b, st, cu, output=x)
+    part = torch.empty((6, 8), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError):
+        fk.conv_prefill(x, w, b, st, cu, split=(8, 8), output=(part, part))
+    i = _scan_inputs([4, 2], 4, 2, 64)
+    for at in range(1, 5):
+        args = [i["x"], i["dt"], i["A_log"], i["B"], i["C"], i["D"], i["dt_bias"], i["state"], cu]
+        args[at] = None
+        with pytest.raises(TypeError):
+            fk.ssm_prefill(*args)
+    with pytest.raises(ValueError):
+        fk.ssm_prefill(i["x"], i["dt"], i["A_log"], i["B"], i["C"], i["D"], i["dt_bias"], i["state"], cu, z=i["z"],
+                       output=i["z"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["conv"] + METHODS)
+def test_rows_behind_the_last_sequence_stay(op):
+    """Offsets that end in front of the last row (reported, as any that are not offsets over
+    all rows): the rows behind are left as they were, the sequences' own are right."""
+    lengths, T = [90, 0, 43], 200
+    if op == "conv":
+        x, w, b, st = _conv_inputs([90, 0, 110], 64, 4)
+        out = torch.full((T, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+        y, new = fk.conv_prefill(x, w, b, st, _cu(lengths), output=out)
+        want = fk.conv_prefill(x[:133], w, b, st, _cu(lengths))
+    else:
+        i = _scan_inputs([90, 0, 110], 2, 1, 64)
+        out = torch.full((T, 2, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+        y, new = fk.ssm_prefill(i["x"], i["dt"], i["A_log"], i["B"], i["C"], i["D"], i["dt_bias"], i["state"],
+                                _cu(lengths), z=i["z"], method=op, output=out)
+        s = _part(i, slice(0, 133), i["state"])
+        want = fk.ssm_prefill(s["x"], s["dt"], s["A_log"], s["B"], s["C"], s["D"], s["dt_bias"], s["state"],
+                              _cu(lengths), z=s["z"], method=op)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        fk.device_status()
+    assert y is out and bool((out[133:] == 7.0).all())
+    assert torch.equal(out[:133], want[0]) and torch.equal(new, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [2, 3, 4])
+def test_views_off_their_alignment(dtype, K):
+    """Weights that start off a 16-byte boundary, and rows that the kernels cannot read in
+    place: the bits of packed, aligned copies."""
+    off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+    lengths = [30, 7, 60]
+    x, w, b, st = _conv_inputs(lengths, 72, K, dtype=dtype)
+    want = fk.conv_prefill(x, w, b, st, _cu(lengths))
+    for args in ((x, off(w), off(b), st), (off(x), w, b, off(st)), (x.t().contiguous().t(), w.t().contiguous().t(), b, st),
+                 (torch.cat([x, x[:, :1]], 1)[:, :72], w, off(b), st)):
+        got = fk.conv_prefill(*args, _cu(lengths))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        got = fk.conv_decode(args[0][:3], *args[1:])
+        one = fk.conv_decode(x[:3], w, b, st)
+        assert torch.equal(got[0], one[0]) and torch.equal(got[1], one[1])
+    i = _scan_inputs(lengths, 2, 1, 64, dt_dtype=dtype, params=dtype, seed=2)
+    for method in METHODS:
+        want = _scan(i, lengths, method=method)
+        for other in ({k: (off(v) if v is not None else None) for k, v in i.items()},
+                      dict(i, x=i["x"].transpose(0, 1).contiguous().transpose(0, 1), z=i["z"].transpose(1, 2).contiguous().transpose(1, 2),
+                           dt=i["dt"].t().contiguous().t(), state=i["state"].transpose(2, 3).contiguous().transpose(2, 3))):
+            got = _scan(other, lengths, method=method)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["conv"] + METHODS)
+def test_hundreds_of_short_sequences(op):
+    lengths = [(7 * n) % 6 for n in range(600)]
+    if op == "conv":
+        x, w, b, st = _conv_inputs(lengths, 40, 4)
+        y, new = fk.conv_prefill(x, w, b, st, _cu(lengths))
+        ry, mag, rs = _conv_ref(x, w, b, st, lengths, "silu")
+        _check("y", y, ry, HALF * ry.abs() + 2.0 ** -16 * mag + TINY)
+        assert torch.equal(new.cpu().to(F64), rs)
+    else:
+        i = _scan_inputs(lengths, 2, 1, 64)
+        out, new = _scan(i, lengths, method=op)
+        _check_scan(out, new, _ref(i, lengths), op)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("method", METHODS)
+def test_steps_of_nothing_and_of_a_great_deal(method):
+    """A dt of -inf leaves the state alone, a very large one forgets it; NaN parameters of a
+    head stay in that head and do not vanish.  The log2 decays of a chunk sum to less than
+    1024 here (160 a step at most), so each of up to 8 fp32 additions behind an exponent is
+    off by 2^-15 at most, and the exponential by 8 ln 2 2^-15 < 2^-12 relative."""
+    lengths = [150]
+    i = _scan_inputs(lengths, 4, 1, 64, dt_dtype=torch.float32)
+    i["dt"][5:9] = float("-inf")
+    i["dt"][40, 1] = 1000.0
+    i["dt"][70:75, 2] = 300.0
+    out, new = _scan(i, lengths, method=method)
+    y, ymag, st, smag = _ref(i, lengths)
+    rounded = HALF if method == "tcgen05" else 0.0
+    _check("y", out, y, HALF * y.abs() + (rounded * (1 + HALF) + 2.0 ** -16 + 2.0 ** -12) * ymag + TINY)
+    _check("state", new, st, (2.0 ** -15 + 2.0 ** -12) * smag + TINY)
+    for name in ("A_log", "dt_bias"):
+        j = dict(i)
+        j[name] = i[name].clone()
+        j[name][1] = float("nan")
+        o2, n2 = _scan(j, lengths, method=method)
+        keep = [0, 2, 3]
+        assert torch.equal(o2[:, keep], out[:, keep]) and torch.equal(n2[:, keep], new[:, keep])
+        assert bool(torch.isnan(n2[:, 1]).all()) and bool(torch.isnan(o2[:, 1].float()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P", [64, 128])
+def test_cut_prompts_in_graphs_and_on_two_streams(P):
+    """A prompt that is cut into segments takes a workspace from the pool: two captured calls
+    replayed at once, and two eager ones on two streams, give the bits of single calls."""
+    lengths = [4133]
+    a, b = (_scan_inputs(lengths, 2, 1, P, seed=s) for s in (41, 42))
+    call = lambda i: fk.ssm_prefill(i["x"], i["dt"], i["A_log"], i["B"], i["C"], i["D"], i["dt_bias"], i["state"], cu,
+                                    z=i["z"], method="tcgen05")
+    cu = _cu(lengths)
+    want = [call(a), call(b)]
+    _check_scan(*want[0], _ref(a, lengths), "tcgen05")
+    graphs = []
+    for i in (a, b):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call(i)
+        graphs.append((graph, outs))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for graph, outs in graphs:
+            for o in outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for s, (graph, _outs) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_g, outs), w in zip(graphs, want):
+            assert torch.equal(outs[0], w[0]) and torch.equal(outs[1], w[1])
+        got = []
+        for s, i in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(call(i))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+    fk.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,H,P,z", [([700, 300, 513], 32, 128, True), ([700, 300, 513], 5, 64, False),
+                                           ([4000], 2, 128, True)])
+def test_scan_waits_run_out_then_next_call_is_correct(lengths, H, P, z):
+    """With a 1 ns limit the scan's waits run out: the call returns and the status says so; the
+    next call, which allocates the same tensor memory, gives the usual bits."""
+    lib = _lib.load()
+    i = _scan_inputs(lengths, H, 1, P, z=z, seed=43)
+    want = _scan(i, lengths, method="tcgen05")
+    prev = lib.gdn_set_wait_limit_ns(1)
+    try:
+        with pytest.raises(_lib.GdnError) as ei:
+            _scan(i, lengths, method="tcgen05")
+        assert ei.value.status == _lib.GDN_ERR_DEVICE_TIMEOUT
+    finally:
+        lib.gdn_set_wait_limit_ns(prev)
+    fk.device_status()
+    got = _scan(i, lengths, method="tcgen05")
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows so far apart, and a state so large, that element offsets pass 2^31."""
+    T, H, G, P, C = 2304, 2, 1, 64, 512
+    wide = torch.randn((T, 1 << 10), device=DEV).to(torch.bfloat16).repeat(1, 1 << 10)      # 4.8 GB
+    cols = lambda at, n: wide[:, at:at + n]
+    i = _scan_inputs([T], H, G, P, seed=50)
+    far = dict(i, x=cols(0, 128).view(T, H, P), B=cols(128, 128).view(T, G, 128), C=cols(256, 128).view(T, G, 128),
+               z=cols(384, 128).view(T, H, P), dt=cols(512, H))
+    near = {k: (v.contiguous() if v is not None else None) for k, v in far.items()}
+    for method in METHODS:
+        a, b = _scan(far, [T], method=method), _scan(near, [T], method=method)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x, w, bias, st = _conv_inputs([T], C, 4)
+    a, b = fk.conv_prefill(cols(0, C), w, bias, st, _cu([T])), fk.conv_prefill(cols(0, C).contiguous(), w, bias, st, _cu([T]))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    st = st.expand(T, -1, -1).contiguous()
+    a, b = fk.conv_decode(cols(0, C), w, bias, st), fk.conv_decode(cols(0, C).contiguous(), w, bias, st)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    del wide, far, near
+    batch, H, P = 4200, 32, 128                                                             # 8.8 GB of state
+    i = _scan_inputs([batch], H, 8, P, state=False, seed=51)
+    state = torch.randn((1, H, P, 128), device=DEV).repeat(batch, 1, 1, 1)
+    tail = slice(batch - 3, batch)
+    want = _step(_part(i, tail, state[tail].clone()))
+    got, _ = _step(i, state=state, new_state=state)
+    assert torch.equal(got[tail], want[0]) and torch.equal(state[tail], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [[0, 3000, 1000, 4133], [0, 4133, 0, 4133], [2000, 1, 4000, 4133], [0, 9000, -5, 4133]])
+def test_malformed_cu_seqlens_of_a_cut_prompt_is_reported(bad):
+    """Segments of offsets that overlap or run backwards stay inside the workspace; the next
+    good call gives the usual bits."""
+    lengths = [1300, 1333, 1500]
+    i = _scan_inputs(lengths, 2, 1, 128, seed=60)
+    want = _scan(i, lengths, method="tcgen05")
+    fk.ssm_prefill(i["x"], i["dt"], i["A_log"], i["B"], i["C"], i["D"], i["dt_bias"], i["state"],
+                   torch.tensor(bad, dtype=torch.int32, device=DEV), z=i["z"], method="tcgen05")
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        fk.device_status()
+    got = _scan(i, lengths, method="tcgen05")
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
