@@ -79,8 +79,8 @@ constexpr uint32_t kTile = 16 * 1024;
 constexpr uint32_t OFF_STAGE = 0;                                // kStages x [C | B | x]
 constexpr uint32_t STAGE = 3 * kTile;
 constexpr uint32_t ST_C = 0, ST_B = kTile, ST_X = 2 * kTile;
-constexpr uint32_t OFF_M = OFF_STAGE + kStages * STAGE;          // [head][i][j], K-major, 8 KB each
-constexpr uint32_t OFF_Y = OFF_M + kTile;                        // 2 x z, then the output rows in its place
+constexpr uint32_t OFF_M = OFF_STAGE + kStages * STAGE;          // 2 x [head][i][j], K-major, 8 KB each
+constexpr uint32_t OFF_Y = OFF_M + 2 * kTile;                        // 2 x z, then the output rows in its place
 constexpr uint32_t OFF_GATE = OFF_Y + 2 * kTile;                 // kGateStages x 2 heads x Gates
 constexpr uint32_t GATE = 1408;
 constexpr uint32_t SMEM_BYTES = OFF_GATE + kGateStages * 2 * GATE;
@@ -312,7 +312,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     const SsmArgs &p = args.a;
     constexpr int kHeads = PAIR ? 2 : 1;
     constexpr int kGateReaders = LOCAL ? kUpdateWarps : kYWarps;    // the last to read a chunk's gates
-    constexpr int kMBuffers = PAIR ? 1 : 2;    // M tiles: one of both heads, or two of the one
 
     // (warp-uniform for the compiler too, so that the MMA warp's loop and descriptors are)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -406,7 +405,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         tmem_relinquish();
     }
     // M's upper right blocks stay zero
-    for (int i = tid; i < static_cast<int>(kTile / 16); i += kThreads)
+    for (int i = tid; i < static_cast<int>(kHeads * kTile / 16); i += kThreads)
         reinterpret_cast<uint4 *>(sm + OFF_M)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
     tc_fence_before();
@@ -495,12 +494,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 mma_commit(bar(bars.cs));
             }
             __syncwarp();
-            if (!wait.warp(bar(bars.mready[c & (kMBuffers - 1)]), c / kMBuffers, kSsmM)) break;
+            if (!wait.warp(bar(bars.mready[c & 1]), c >> 1, kSsmM)) break;
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    mma_ss(tm + TM::YA, dX + st + k * kStep, dM + (PAIR ? 0 : (c & 1) * kAtom) + 2 * k, id_m, k > 0);
-                mma_commit(bar(bars.mx[c & (kMBuffers - 1)]));
+                    mma_ss(tm + TM::YA, dX + st + k * kStep, dM + (c & 1) * kHeads * kAtom + 2 * k, id_m, k > 0);
+                mma_commit(bar(bars.mx[c & 1]));
                 mma_commit(bar(bars.empty[c % kStages]));
             }
             __syncwarp();
@@ -510,8 +509,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         __syncwarp();
         wait.drain(bar(bars.last[1]), 0, kSsmIssue);
 #pragma unroll 1
-        for (int c = nmx > kMBuffers ? nmx - kMBuffers : 0; c < nmx; ++c)
-            wait.drain(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX);
+        for (int c = nmx > 2 ? nmx - 2 : 0; c < nmx; ++c)
+            wait.drain(bar(bars.mx[c & 1]), c >> 1, kSsmMX);
         __syncwarp();
     } else if (warp == 18) {
         // -------------------------------------------------------------- copies
@@ -731,7 +730,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
             // the stores two chunks before have read the staging rows (z's copy waited for them)
             if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
-            if (!wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers, kSsmMX)) break;      // (Yi went out before Ya)
+            if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
             const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
@@ -806,50 +805,60 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
             const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
             if (!gates_full(c)) break;
-            // the tile has been read by Ya two chunks before (one, with one buffer)
-            if (c >= kMBuffers &&
-                !wait.warp(bar(bars.mx[c & (kMBuffers - 1)]), c / kMBuffers - 1, kSsmMX)) break;
+            // the tile has been read by Ya two chunks before
+            if (c >= 2 &&
+                !wait.warp(bar(bars.mx[c & 1]), (c >> 1) - 1, kSsmMX)) break;
             if (!wait.warp(bar(bars.g[c & (TM::kG - 1)]), c / TM::kG, kSsmG)) break;
-#pragma unroll 1
+            // (both heads of a pair from one read of their scores)
+            float lai[kHeads], own[kHeads][8];             // the diagonal block's factors, zero above it
+#pragma unroll
             for (int k = 0; k < kHeads; ++k) {
                 const Gates *o = gates_of(c, k);
-                uint8_t *dst = sm + OFF_M + (PAIR ? k : c & 1) * 8192;
-                const float lai = o->la[row];
-                float own[8];                              // the diagonal block's factors, zero above it
+                lai[k] = o->la[row];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) own[j] = j <= (row & 7) ? ex2(lai - o->lb[(row & ~7) + j]) : 0.0f;
+                for (int j = 0; j < 8; ++j) own[k][j] = j <= (row & 7) ? ex2(lai[k] - o->lb[(row & ~7) + j]) : 0.0f;
+            }
+            uint8_t *const tiles = sm + OFF_M + (c & 1) * kHeads * 8192;
 #pragma unroll 1
-                for (int q = 0; q < 4; ++q) {              // 8 columns
-                    uint32_t r[8], b[4];
-                    tmem_ld8(tmem_addr(tm, lane_base, TM::G + (c & (TM::kG - 1)) * 64 + j0 + 8 * q), r);
-                    const float4 *col = reinterpret_cast<const float4 *>(o->cf + j0 + 8 * q);
+            for (int q = 0; q < 4; ++q) {                  // 8 columns
+                uint32_t r[8];
+                tmem_ld8(tmem_addr(tm, lane_base, TM::G + (c & (TM::kG - 1)) * 64 + j0 + 8 * q), r);
+                float rf[kHeads];
+#pragma unroll
+                for (int k = 0; k < kHeads; ++k) rf[k] = q < block ? ex2(lai[k] - gates_of(c, k)->la[j0 + 8 * q + 7]) : 0.0f;
+                tmem_wait_ld_dep(r);
+                if (nt < kL) {                             // scores with rows behind the last token: zero, not x 0
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j] = j0 + 8 * q + j < nt ? r[j] : 0u;
+                }
+#pragma unroll
+                for (int k = 0; k < kHeads; ++k) {
+                    const float4 *col = reinterpret_cast<const float4 *>(gates_of(c, k)->cf + j0 + 8 * q);
                     const float4 v0 = col[0], v1 = col[1];
                     const float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                    const float rf = q < block ? ex2(lai - o->la[j0 + 8 * q + 7]) : 0.0f;
-                    const uint64_t rf2 = f2(rf, rf);
-                    tmem_wait_ld_dep(r);
-                    if (nt < kL) {                         // scores with rows behind the last token: zero, not x 0
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) r[j] = j0 + 8 * q + j < nt ? r[j] : 0u;
-                    }
+                    const uint64_t rf2 = f2(rf[k], rf[k]);
+                    uint32_t b[4];
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
                         float f0, f1, m0, m1;
                         unf2(mul_f2(f2(f[j], f[j + 1]), rf2), f0, f1);
-                        unf2(mul_f2(bits2(r[j], r[j + 1]), f2(q == block ? own[j] : f0, q == block ? own[j + 1] : f1)), m0, m1);
+                        unf2(mul_f2(bits2(r[j], r[j + 1]), f2(q == block ? own[k][j] : f0, q == block ? own[k][j + 1] : f1)), m0, m1);
                         b[j / 2] = pack_bf16x2(m0, m1);
                     }
-                    *reinterpret_cast<uint4 *>(dst + sw128(row, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
+                    *reinterpret_cast<uint4 *>(tiles + k * 8192 + sw128(row, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
                 }
-                if (warp != 17) {                          // D on the diagonal: onto the rounded entry, rounded again
-                    auto *d = reinterpret_cast<__nv_bfloat16 *>(dst + sw128(row, row >> 3) + (row & 7) * 2);
+            }
+            if (warp != 17) {                              // D on the diagonal: onto the rounded entry, rounded again
+#pragma unroll
+                for (int k = 0; k < kHeads; ++k) {
+                    auto *d = reinterpret_cast<__nv_bfloat16 *>(tiles + k * 8192 + sw128(row, row >> 3) + (row & 7) * 2);
                     *d = __float2bfloat16_rn(__bfloat162float(*d) + (k ? D1 : D0));
                 }
             }
             tc_fence_before();
             warp_arrive(bar(bars.mread[c & (TM::kG - 1)]), lane);
             fence_proxy_async_smem();
-            warp_arrive(bar(bars.mready[c & (kMBuffers - 1)]), lane);
+            warp_arrive(bar(bars.mready[c & 1]), lane);
         }
     } else if ((warp >= 12 && warp < 16) || warp >= 24) {
         // -------------------------------------------------------------- w x, hi and lo

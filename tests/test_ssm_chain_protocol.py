@@ -31,7 +31,7 @@ def counts(heads, local=False):
 class Scan(Sim):
     def __init__(self, nch, heads, gated, plant=None, local=False):
         super().__init__(nch, plant)
-        self.heads, self.gated, self.m_buffers, self.g_buffers = heads, gated, 3 - heads, 3 - heads
+        self.heads, self.gated, self.m_buffers, self.g_buffers = heads, gated, 2, 3 - heads
         self.b = {k: Bar(k, v) for k, v in counts(heads, local).items()}
         self.local = local     # the state path alone
 
