@@ -730,18 +730,31 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
             // the stores two chunks before have read the staging rows (z's copy waited for them)
             if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
-            if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
             const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
+            // the gate's factors of 16 state rows x 16 tokens: the first while Ya is on its way, the
+            // others while the accumulators are read
+            float gate[8];
+            auto gates16 = [&](uint32_t from) {
+                uint32_t zr[4];
+                ldsm_x4_t(zr, from);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    gate[2 * k] = silu_approx(bf16_lo(zr[k]));
+                    gate[2 * k + 1] = silu_approx(bf16_hi(zr[k]));
+                }
+            };
+            if (gated) gates16(tile + at);
+            if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
                 const int lh = u & 1, hh = u >> 1;
-                uint32_t yi[8], yo[8], zr[4], y[4];
+                uint32_t yi[8], yo[8], y[4];
                 tmem_ld_frag16(yi_at + (16u * lh << 16) + 16 * hh, yi);
                 tmem_ld_frag16(ya_at + (16u * lh << 16) + 16 * hh, yo);
                 // (the second 16 rows are two 16-byte words on, under the swizzle)
                 const uint32_t to = tile + (lh ? at ^ 32u : at) + hh * 2048;
                 const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * hh), eb = *reinterpret_cast<const float2 *>(e + 16 * hh + 8);
-                if (gated) ldsm_x4_t(zr, to);
+                if (gated && u > 0) gates16(to);
                 tmem_wait_ld_dep(yi);
                 tmem_wait_ld_dep(yo);
 #pragma unroll
@@ -750,8 +763,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                     unf2(fma_f2(bits2(yi[2 * k], yi[2 * k + 1]), k < 2 ? f2(ea.x, ea.y) : f2(eb.x, eb.y),
                                 bits2(yo[2 * k], yo[2 * k + 1])), y0, y1);
                     if (gated) {
-                        y0 *= silu_approx(bf16_lo(zr[k]));
-                        y1 *= silu_approx(bf16_hi(zr[k]));
+                        y0 *= gate[2 * k];
+                        y1 *= gate[2 * k + 1];
                     }
                     y[k] = pack_bf16x2(y0, y1);
                 }
