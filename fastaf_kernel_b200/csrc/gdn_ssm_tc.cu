@@ -70,6 +70,7 @@ constexpr int kRows = 128;          // state rows of a CTA
 constexpr int kStages = 3;          // of C, B, x
 constexpr int kGateStages = 4;
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
+constexpr int kZBehind = 2;         // chunks z's copies run behind the others
 constexpr int kMWarps = 3, kYWarps = 8;
 constexpr int kUpdateWarps = 12;     // of the state path and the split
 
@@ -521,24 +522,30 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const int x = lane < 4 ? g * 128 + (lane & 1) * 64 : (lane & 1) ? xc1 : xc0;
         const bool staged = lane < 6 && !(LOCAL && lane < 2);
         const bool fetched = lane < (gated ? 8 : 6) && !(LOCAL && lane < 2);
+        // (z two chunks behind: its place is free only when the outputs two chunks before are out, and
+        // the other copies must not wait for that; at the outputs' side it is in time)
         int issued = 0, zissued = 0;
 #pragma unroll 1
-        for (int c = 0; c < nch; ++c) {
+        for (int c = 0; c < (gated ? nch + kZBehind : nch); ++c) {
             const int t = static_cast<int>(s0) + c * kL;
-            const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
-            if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
-            if (lane == 0) mbar_arrive_expect_tx(b, LOCAL ? STAGE - kTile : STAGE);
-            __syncwarp();
-            if (staged) tma_load_2d(sbase + OFF_STAGE + st * STAGE + lane * 8192, map, b, x, t);
-            if (fetched && c + kPrefetch < nch) tma_prefetch_2d(map, x, t + kPrefetch * kL);
-            ++issued;
-            if (gated) {
+            if (c < nch) {
+                const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
+                if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
+                if (lane == 0) mbar_arrive_expect_tx(b, LOCAL ? STAGE - kTile : STAGE);
+                __syncwarp();
+                if (staged) tma_load_2d(sbase + OFF_STAGE + st * STAGE + lane * 8192, map, b, x, t);
+                if (fetched && c + kPrefetch < nch) tma_prefetch_2d(map, x, t + kPrefetch * kL);
+                ++issued;
+            }
+            if (gated && c >= kZBehind) {
                 // (into the staging rows that the stores two chunks before have read)
-                if (c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
-                const uint32_t zb = bar(bars.zfull[c & 1]);
+                const int k = c - kZBehind;
+                if (k >= 2 && !wait.warp(bar(bars.yfree[k & 1]), (k >> 1) - 1, kSsmStage)) break;
+                const uint32_t zb = bar(bars.zfull[k & 1]);
                 if (lane == 0) mbar_arrive_expect_tx(zb, kTile);
                 __syncwarp();
-                if (lane == 6 || lane == 7) tma_load_2d(sbase + OFF_Y + (c & 1) * kTile + (lane - 6) * 8192, map, zb, x, t);
+                if (lane == 6 || lane == 7)
+                    tma_load_2d(sbase + OFF_Y + (k & 1) * kTile + (lane - 6) * 8192, map, zb, x, t - kZBehind * kL);
                 ++zissued;
             }
         }
@@ -727,53 +734,49 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const float *e = gates_of(c, hrow)->e + i0 + 2 * (lane & 3);
+            if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
+            uint64_t y[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
+                const int lh = u & 1, hh = u >> 1;
+                uint32_t yi[8], yo[8];
+                tmem_ld_frag16(yi_at + (16u * lh << 16) + 16 * hh, yi);
+                tmem_ld_frag16(ya_at + (16u * lh << 16) + 16 * hh, yo);
+                const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * hh), eb = *reinterpret_cast<const float2 *>(e + 16 * hh + 8);
+                tmem_wait_ld_dep(yi);
+                tmem_wait_ld_dep(yo);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    y[u][k] = fma_f2(bits2(yi[2 * k], yi[2 * k + 1]), k < 2 ? f2(ea.x, ea.y) : f2(eb.x, eb.y),
+                                     bits2(yo[2 * k], yo[2 * k + 1]));
+            }
+            // the accumulators are free for the next chunk while this one's rows are gated and stored
+            tc_fence_before();
+            warp_arrive(bar(bars.yread), lane);
+            warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
             // the stores two chunks before have read the staging rows (z's copy waited for them)
             if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
             const uint32_t tile = sbase + OFF_Y + (c & 1) * kTile;
-            // the gate's factors of 16 state rows x 16 tokens: the first while Ya is on its way, the
-            // others while the accumulators are read
-            float gate[8];
-            auto gates16 = [&](uint32_t from) {
-                uint32_t zr[4];
-                ldsm_x4_t(zr, from);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    gate[2 * k] = silu_approx(bf16_lo(zr[k]));
-                    gate[2 * k + 1] = silu_approx(bf16_hi(zr[k]));
-                }
-            };
-            if (gated) gates16(tile + at);
-            if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
-                const int lh = u & 1, hh = u >> 1;
-                uint32_t yi[8], yo[8], y[4];
-                tmem_ld_frag16(yi_at + (16u * lh << 16) + 16 * hh, yi);
-                tmem_ld_frag16(ya_at + (16u * lh << 16) + 16 * hh, yo);
+            for (int u = 0; u < 4; ++u) {
                 // (the second 16 rows are two 16-byte words on, under the swizzle)
-                const uint32_t to = tile + (lh ? at ^ 32u : at) + hh * 2048;
-                const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * hh), eb = *reinterpret_cast<const float2 *>(e + 16 * hh + 8);
-                if (gated && u > 0) gates16(to);
-                tmem_wait_ld_dep(yi);
-                tmem_wait_ld_dep(yo);
+                const uint32_t to = tile + ((u & 1) ? at ^ 32u : at) + (u >> 1) * 2048;
+                uint32_t r[4], zr[4];
+                if (gated) ldsm_x4_t(zr, to);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float y0, y1;
-                    unf2(fma_f2(bits2(yi[2 * k], yi[2 * k + 1]), k < 2 ? f2(ea.x, ea.y) : f2(eb.x, eb.y),
-                                bits2(yo[2 * k], yo[2 * k + 1])), y0, y1);
+                    unf2(y[u][k], y0, y1);
                     if (gated) {
-                        y0 *= gate[2 * k];
-                        y1 *= gate[2 * k + 1];
+                        y0 *= silu_approx(bf16_lo(zr[k]));
+                        y1 *= silu_approx(bf16_hi(zr[k]));
                     }
-                    y[k] = pack_bf16x2(y0, y1);
+                    r[k] = pack_bf16x2(y0, y1);
                 }
                 if (gated) __syncwarp();
-                stsm_x4_t(to, y);
+                stsm_x4_t(to, r);
             }
-            tc_fence_before();
-            warp_arrive(bar(bars.yread), lane);
-            warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
             fence_proxy_async_smem();
             warp_arrive(bar(bars.yst[c & 1]), lane);
         }
