@@ -17,7 +17,11 @@
 // that every thread fills (cp.async) and reads for itself, without a barrier: loaded into
 // registers a batch at a time, the loads of a batch did not overlap the arithmetic of the one
 // before (0.456 ms).  65,536 x 8192: 0.337 ms, 6.4 TB/s; batches of 8 rows or a ring of 24 cost
-// resident blocks (0.40 to 0.42 ms), batches of 2 take 0.37 ms.
+// resident blocks (0.40 to 0.42 ms), batches of 2 take 0.37 ms.  A few short prompts (1280
+// tokens) take 12 us, most of it the latency of three dependent reads (offsets, rows, window).
+//
+// Decode (512 x 8192, width 4, with a bias): 13 us, 5.2 TB/s, a thread's runs short enough to
+// fill the SMs, since its weights are read once a run; 4 x 8192: 2.5 us, a launch's latency.
 #include "gdn_common.cuh"
 #include "gdn_launch.h"
 #include "gdn_mma_sync.cuh"

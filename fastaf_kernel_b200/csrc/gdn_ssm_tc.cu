@@ -22,7 +22,9 @@
 //                                hi = bf16(x wh) and lo = bf16(x wl + (x wh - hi)), whose
 //                                inner difference is exact -- three bf16 operations for two
 //                                terms; a TMEM operand, which keeps 48 KB a chunk out of the
-//                                shared memory's bandwidth
+//                                shared memory's bandwidth.  (A third term would want 32 more TMEM
+//                                columns, which pairs of heads do not have, and a third of these
+//                                products again; the state's error is a few 2^-18 of its magnitude.)
 // M's exponentials factor by blocks of 8 columns: exp(la_i - la_j) = exp(la_i - la_r)
 // exp(la_r - la_j) with r the block's last column, both at most 1 for the rows below the
 // block; the 8 rows of the block itself take one exponential per element.  So a row of 32
@@ -44,6 +46,18 @@
 // The loops are kept rolled and the waits out of line: together they have to fit the SM's
 // instruction caches (with everything unrolled a chunk took 7,200 cycles, two thirds of the
 // issue slots waiting for instructions).
+//
+// What bounds it.  A chunk of one head takes 2,000 to 2,300 cycles, of which the tensor pipe
+// works 1,150 and HBM less; 16 x 8192 tokens, 32 heads of 128 in 16 groups: 0.87 ms, 3.8 TB/s,
+// 375 TFLOP/s (the 512 chains are 3.5 waves of 148 CTAs, run as four).  No unit is full: every
+// product waits for a role to turn accumulators into operands, and each hand-over (TMEM load,
+// conversion, store, fence, barrier, issue) costs 400 to 700 cycles.  Pairs take 3,400: three
+// warps form both heads' M in 2,500, and G has one buffer to wait for them.  With z a chunk of
+// one head takes 3,000: its 16 K hardware exponentials and reciprocals alone are 1,024.
+// Measured and not kept: a third issuing warp or 30 warps (64 registers: spills, twice the time),
+// M's scores 16 columns at a time with the diagonal block apart (4 x 2048 tokens in pairs with z,
+// 71 -> 75 us), three stages of z in place of two (16 x 2048 tokens, 283 -> 278 us with z, 205
+// -> 212 without).
 //
 // Every wait is bounded as in gdn_prefill_tc.cu: one that gives up records its site in the
 // device status word and raises a shared flag, every role stops at its next wait, the
