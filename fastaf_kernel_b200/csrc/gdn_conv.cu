@@ -162,7 +162,7 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
         return;
     }
     const int t0 = static_cast<int>(tile * run);
-    int t1 = static_cast<int>(t0 + run < T ? t0 + run : T);
+    const int t1 = static_cast<int>(t0 + run < T ? t0 + run : T);
     __shared__ uint2 ring[kBatches * kBatchRows][kConvThreads];
     const uint32_t slot0 = msync::smem_addr(&ring[0][threadIdx.x]);
     const __nv_bfloat16 *ahead = x + t0 * p.x_stride;      // the next row to copy, row t0 + copied
@@ -194,7 +194,8 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
     }
     int s0 = cu[n];
     s0 = s0 < 0 ? 0 : (s0 > t0 ? t0 : s0);
-    int next = cu[n + 1];
+    int next = n + 1 < N ? cu[n + 1] : 0x7fffffff;
+    const int end = cu[N] < t1 ? cu[N] : t1;            // rows behind the last sequence stay as they are
     // the rows in front of token t of sequence n that starts at s0
     Row win[W - 1];
     auto window = [&](int t) {
@@ -216,23 +217,22 @@ conv_prefill_kernel(const ConvArgs p, int run, int64_t runs) {
         win[W - 2] = cur;
     };
     window(t0);
-    for (int t = t0; t < t1; t += kBatchRows) {
+    for (int t = t0; t < end; t += kBatchRows) {
         copy_batch();                               // (into the batch read last)
         msync::cp_async_wait<kBatches - 1>();
         const uint2(*rows)[kConvThreads] = ring + (t - t0) % (kBatches * kBatchRows);
-        if (t1 - t >= kBatchRows && next - t >= kBatchRows) {
+        if (end - t >= kBatchRows && next - t >= kBatchRows) {
             // whole batches inside a sequence, nearly all of them: nothing to check per row
 #pragma unroll
             for (int u = 0; u < kBatchRows; ++u) put_row(rows[u][threadIdx.x]);
         } else {
 #pragma unroll 1
-            for (int u = 0; u < kBatchRows && t + u < t1; ++u) {
+            for (int u = 0; u < kBatchRows && t + u < end; ++u) {
                 if (t + u >= next) {       // the next sequence that has tokens starts here
-                    while (++n < N && t + u >= (next = cu[n + 1])) {}
-                    if (n >= N) {              // rows behind the last one stay as they are
-                        t1 = t;
-                        break;
-                    }
+                    do {
+                        ++n;
+                        next = n + 1 < N ? cu[n + 1] : 0x7fffffff;
+                    } while (t + u >= next);
                     s0 = t + u;
                     window(t + u);
                 }
