@@ -8,7 +8,8 @@
  *   o_t = scale * S_t q_t,
  *   alpha = exp(-exp(A_log) * softplus(a + dt_bias)),  beta = sigmoid(b),
  *
- * with q/k heads shared by Hv/Hq consecutive v-heads (GVA).
+ * with q/k heads shared by Hv/Hq consecutive v-heads (GVA); and the short causal convolution
+ * and the selective scan of the layers around it, for prompts and single tokens.
  *
  * All tensor arguments are raw DEVICE pointers to contiguous row-major
  * buffers; no framework types cross this boundary.  Every entry point is
@@ -382,7 +383,7 @@ GDN_API int gdn_device_status(void *stream);
 
 /*
  * Limit, in nanoseconds, of every bounded device-side wait of the tcgen05 prefill
- * chains launched after this call (process-wide; 0 restores the default of 2 s).
+ * chains and the tcgen05 scan launched after this call (process-wide; 0 restores the default of 2 s).
  * Returns the previous setting (0 = default).  A serving process can lower it to
  * detect a stalled kernel sooner; a limit below a chunk's normal latency makes
  * healthy calls give up (gdn_device_status then reports GDN_ERR_DEVICE_TIMEOUT).

@@ -66,3 +66,29 @@ def test_chain_kernel_does_not_spill(tmp_path):
     for name, (regs, st, ld) in chain.items():
         assert (regs + 7) // 8 * 8 * threads <= 65536, f"{name}: {regs} registers x {threads} threads exceed the SM"
         assert st == 0 and ld == 0, f"{name}: spills {st}/{ld} bytes"
+
+
+def test_scan_step_keeps_three_ctas_per_sm(tmp_path):
+    rep = _ptxas_report("gdn_ssm.cu", tmp_path)
+    dec = {k: v for k, v in rep.items() if "ssm_decode_kernel" in k}
+    assert len(dec) == 2, sorted(rep)          # rows per thread 1, 2
+    for name, (regs, st, ld) in dec.items():
+        assert regs <= 80, f"{name}: {regs} registers (> 80 leaves two CTAs per SM)"
+        assert st == 0 and ld == 0, f"{name}: spills {st}/{ld} bytes"
+
+
+def test_convolution_does_not_spill(tmp_path):
+    rep = _ptxas_report("gdn_conv.cu", tmp_path)
+    assert len(rep) == 6, sorted(rep)          # widths 2, 3, 4 x prompts, single tokens
+    for name, (regs, st, ld) in rep.items():
+        assert st == 0 and ld == 0, f"{name}: spills {st}/{ld} bytes"
+        assert regs <= (64 if "prefill" in name else 80), f"{name}: {regs} registers"
+
+
+def test_scan_main_pass_does_not_spill(tmp_path):
+    """One CTA of 28 warps per SM: 65,536 registers / 896 threads = 73, in steps of 8 a thread."""
+    rep = _ptxas_report("gdn_ssm_tc.cu", tmp_path)
+    main = {k: v for k, v in rep.items() if "ssm_tc_kernel" in k and "ELb0EE" in k}
+    assert len(main) == 2, sorted(rep)         # one head of 128, pairs of 64
+    for name, (regs, st, ld) in main.items():
+        assert regs <= 72 and st == 0 and ld == 0, f"{name}: {regs} registers, spills {st}/{ld} bytes"
