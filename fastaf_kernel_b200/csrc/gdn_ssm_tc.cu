@@ -86,7 +86,7 @@ constexpr int kGateStages = 4;
 constexpr int kPrefetch = 6;        // chunks the L2 prefetch runs ahead
 constexpr int kZBehind = 2;         // chunks z's copies run behind the others
 constexpr int kMWarps = 3, kYWarps = 8;
-constexpr int kUpdateWarps = 12;     // of the state path and the split
+constexpr int kSplitWarps = 8, kUpdateWarps = 12;     // of the split; of the state path and the split
 
 // Shared memory (bytes from the 1024-aligned base).  Tiles are 64 rows of 64 bf16 (one
 // 128-byte swizzled atom, 8 KB), two atoms side by side.
@@ -137,8 +137,7 @@ constexpr uint32_t kMaxSuspendNs = 1000000;
 // are, without cuts) that run side by side.  Segment j of sequence n has slot
 // cu_seqlens[n] / segment + n + j, so that the slots of different sequences are distinct
 // whatever their lengths; a first pass (LOCAL) leaves in `ends` what every segment but a
-// sequence's last adds to the state (the first one: the state behind it) and in `decays` its
-// decay, ssm_combine_kernel turns `ends` into the states behind the segments, and the main
+// sequence's last adds to the state and in `decays` its decay, ssm_combine_kernel turns `ends` into the states behind the segments, and the main
 // pass starts every segment from the one in front of it.
 struct TcArgs {
     SsmArgs a;
@@ -314,7 +313,12 @@ __device__ __forceinline__ float softplus_series(float x) {
     return fmaxf(x, 0.0f) + 2.0f * v;
 }
 
-// PAIR: two heads of 64 rows; else one head of 128.  LOCAL: the state path alone (see TcArgs).
+// PAIR: two heads of 64 rows; else one head of 128.  LOCAL: the state update alone (see TcArgs),
+// from a segment's last chunk to its first: a token's weight, its decay to the segment's end, is
+// then known when it comes, so the products accumulate without a pass over the state in between
+// (0.75 us a chunk; in order, with the state decayed chunk by chunk, 0.93).  The scaled x has two
+// places, one in TM::G; its barriers are those of G.  A pair's gates take two warps (with one,
+// 1 x 16,384 tokens in 32 chains of pairs took 222 us in place of 209).
 template <bool PAIR, bool LOCAL>
 __global__ void __launch_bounds__(kThreads, 1)
 ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap bmap,
@@ -327,6 +331,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     const SsmArgs &p = args.a;
     constexpr int kHeads = PAIR ? 2 : 1;
     constexpr int kGateReaders = LOCAL ? kUpdateWarps : kYWarps;    // the last to read a chunk's gates
+    constexpr int kGateWriters = LOCAL && PAIR ? 2 : 1;             // warps that take the gates' turns
+    constexpr int kUpdateArrivals = LOCAL ? kSplitWarps : kUpdateWarps;
 
     // (warp-uniform for the compiler too, so that the MMA warp's loop and descriptors are)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -381,9 +387,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         return;
     }
     // where the state starts from, and its lines on their way into L2 meanwhile
-    const float *const first = seg == 0 ? (p.state ? p.state + state_at : nullptr)
-                               : LOCAL  ? nullptr
-                                        : args.ends + (end_at - static_cast<int64_t>(args.slabs) * kRows) * kSsmState;
+    const float *const first = LOCAL      ? nullptr
+                               : seg == 0 ? (p.state ? p.state + state_at : nullptr)
+                                          : args.ends + (end_at - static_cast<int64_t>(args.slabs) * kRows) * kSsmState;
     if (first && tid < (lone ? 64 : kRows) * kSsmState / 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(first + tid * 32));
     if (warp == 0) {
         if (lane == 0) {
@@ -392,7 +398,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 mbar_init(bar(bars.empty[i]), 2);
             }
             for (int i = 0; i < kGateStages; ++i) {
-                mbar_init(bar(bars.gates[i]), 1);
+                mbar_init(bar(bars.gates[i]), kGateWriters);
                 mbar_init(bar(bars.ydone[i]), kGateReaders);
             }
             for (int i = 0; i < 2; ++i) {
@@ -401,7 +407,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 mbar_init(bar(bars.yfree[i]), 1);
                 mbar_init(bar(bars.mx[i]), 1);
                 mbar_init(bar(bars.mready[i]), kMWarps);
-                mbar_init(bar(bars.update[i]), kUpdateWarps);
+                mbar_init(bar(bars.update[i]), kUpdateArrivals);
                 mbar_init(bar(bars.last[i]), 1);
                 mbar_init(bar(bars.g[i]), 1);
                 mbar_init(bar(bars.mread[i]), kMWarps);
@@ -464,12 +470,14 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         for (int c = 0; ok && c < nch; ++c) {
             const uint32_t st = (c % kStages) * kSt;
             if (LOCAL && !(ok = wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma))) break;
-            // (the state path's and the split's warps)
+            // (the split's warps and, but for the local pass, the state path's)
             if (!(ok = wait.warp(bar(bars.update[c & 1]), c >> 1, kSsmUpdate))) break;
             if (elect_one()) {                  // S += (w x)^T B: hi, then lo against the same B
 #pragma unroll
-                for (int k = 0; k < 8; ++k) mma_ts(tm + TM::S, tm + TM::W + 8 * k, dBm + st + (k & 3) * kStep, id_s, 1);
-                mma_commit(bar(bars.s));
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tm + TM::S, tm + (LOCAL && (c & 1) ? TM::G : TM::W) + 8 * k, dBm + st + (k & 3) * kStep, id_s,
+                           !LOCAL || c > 0 || k > 0);
+                mma_commit(bar(LOCAL ? bars.g[c & 1] : bars.s));
                 mma_commit(bar(bars.empty[c % kStages]));
                 if (LOCAL) mma_commit(bar(bars.empty[c % kStages]));   // (for the other issuing warp)
             }
@@ -485,7 +493,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll 1
         for (int c = ng > TM::kG ? ng - TM::kG : 0; c < ng; ++c)
             wait.drain(bar(bars.g[c & (TM::kG - 1)]), c / TM::kG, kSsmG);
-        if (ns) wait.drain(bar(bars.s), ns - 1, kSsmS);
+        if (LOCAL) {
+#pragma unroll 1
+            for (int c = ns > 2 ? ns - 2 : 0; c < ns; ++c) wait.drain(bar(bars.g[c & 1]), c >> 1, kSsmS);
+        } else if (ns) {
+            wait.drain(bar(bars.s), ns - 1, kSsmS);
+        }
         __syncwarp();
     } else if (!LOCAL && warp == 3) {
         // -------------------------------------------------------------- Yi and Ya
@@ -541,14 +554,14 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         int issued = 0, zissued = 0;
 #pragma unroll 1
         for (int c = 0; c < (gated ? nch + kZBehind : nch); ++c) {
-            const int t = static_cast<int>(s0) + c * kL;
+            const int t = static_cast<int>(s0) + (LOCAL ? nch - 1 - c : c) * kL;
             if (c < nch) {
                 const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
                 if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
                 if (lane == 0) mbar_arrive_expect_tx(b, LOCAL ? STAGE - kTile : STAGE);
                 __syncwarp();
                 if (staged) tma_load_2d(sbase + OFF_STAGE + st * STAGE + lane * 8192, map, b, x, t);
-                if (fetched && c + kPrefetch < nch) tma_prefetch_2d(map, x, t + kPrefetch * kL);
+                if (fetched && c + kPrefetch < nch) tma_prefetch_2d(map, x, LOCAL ? t - kPrefetch * kL : t + kPrefetch * kL);
                 ++issued;
             }
             if (gated && c >= kZBehind) {
@@ -570,17 +583,19 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         for (int c = zissued > 2 ? zissued - 2 : 0; c < zissued; ++c)
             wait.drain(bar(bars.zfull[c & 1]), c >> 1, kSsmZ);
         __syncwarp();
-    } else if (warp == 2) {
+    } else if (kGateWriters == 2 ? (warp == 2 || warp == 19) : warp == 2) {
         // -------------------------------------------------------------- gates
-        // A lane holds tokens 2 lane and 2 lane + 1 of a chunk; one turn per chunk and head.  dt
+        // A lane holds tokens 2 lane and 2 lane + 1 of a chunk; one turn per chunk and head (a pair's
+        // heads side by side in the local pass, where nothing else takes as long).  dt
         // is loaded two turns ahead, and its lines are brought into L2 before that: with one turn
         // between a load and its use, HBM's latency was every chunk's time.
         // (The loads are raw and unconditional: converted or masked where they are issued, each
         // waits for the one before it.)
         uint32_t d[3][2];
         const bool wide = p.dt_dtype != 1;
+        auto place = [&](int c) { return LOCAL ? (c < nch ? nch - 1 - c : 0) : c; };     // of the c-th chunk
         auto fetch = [&](int i, uint32_t (&to)[2]) {
-            const int64_t t = s0 + static_cast<int64_t>(i / kHeads) * kL + 2 * lane;
+            const int64_t t = s0 + static_cast<int64_t>(place(i / kHeads)) * kL + 2 * lane;
             const int64_t at = (t < s1 ? t : s1 - 1) * p.dt_stride + (PAIR && !lone ? h0 + (i & 1) : h0);
             const int64_t next = t + 1 < s1 ? at + p.dt_stride : at;
             if (wide) {
@@ -593,13 +608,14 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         };
         auto value = [&](uint32_t raw) { return __uint_as_float(wide ? raw : raw << 16); };
         auto ahead = [&](int c) {
-            const int64_t t = s0 + static_cast<int64_t>(c) * kL + 2 * lane, at = t * p.dt_stride + h0;
+            const int64_t t = s0 + static_cast<int64_t>(place(c)) * kL + 2 * lane, at = t * p.dt_stride + h0;
             const char *line = static_cast<const char *>(p.dt) + (p.dt_dtype == 1 ? 2 : 4) * at;
             if (t < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
             if (t + 1 < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (p.dt_dtype == 1 ? 2 : 4) * p.dt_stride));
         };
-        fetch(0, d[0]);
-        fetch(1, d[1]);
+        const int turn0 = kGateWriters == 2 && warp == 19 ? 1 : 0;
+        fetch(turn0, d[0]);
+        fetch(turn0 + kGateWriters, d[1]);
         float negA2[kHeads], bias[kHeads];       // log2 decay of dt' = 1
 #pragma unroll
         for (int k = 0; k < kHeads; ++k) {
@@ -610,11 +626,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < kHeads; ++k) negA2[k] = -expf(negA2[k]) * 1.4426950408889634f;
         for (int c = 1; c < kPrefetch; ++c) ahead(c);
+        float later[2] = {0.0f, 0.0f};           // of the chunks behind, in the local pass
 #pragma unroll 1
-        for (int i = 0; i < nch * kHeads; ++i) {
+        for (int i = turn0; i < nch * kHeads; i += kGateWriters) {
             const int c = i / kHeads, head = PAIR ? i & 1 : 0;
-            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL + 2 * lane;
-            fetch(i + 2, d[2]);
+            const int64_t t0 = s0 + static_cast<int64_t>(place(c)) * kL + 2 * lane;
+            fetch(i + 2 * kGateWriters, d[2]);
             if (head == 0) ahead(c + kPrefetch);
             const float b0 = PAIR && head ? bias[kHeads - 1] : bias[0];
             const float d0 = t0 < s1 ? softplus_series(value(d[0][0]) + b0) : 0.0f;
@@ -646,17 +663,25 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                         n3 = __shfl_down_sync(0xffffffffu, a0 + a1, 3, 4);
             const int q = lane & 3;
             const float rest = (q < 3 ? n1 : 0.0f) + (q < 2 ? n2 : 0.0f) + (q < 1 ? n3 : 0.0f);
-            if (head == 0 && c >= kGateStages &&
+            if ((kGateWriters == 2 || head == 0) && c >= kGateStages &&
                 !wait.warp(bar(bars.ydone[c & (kGateStages - 1)]), c / kGateStages - 1, kSsmY)) break;
             Gates *o = gates_of(c, head);
             auto put = [&](float *to, float v0, float v1) { reinterpret_cast<float2 *>(to)[lane] = make_float2(v0, v1); };
-            put(o->la, l0, l1);
-            put(o->lb, l0 - __log2f(d0), l1 - __log2f(d1));
-            put(o->cf, ex2(rest + a1) * d0, ex2(rest) * d1);
-            put(o->e, ex2(l0), ex2(l1));
-            split2_bf16(ex2(behind + a1) * d0, ex2(behind) * d1, o->wh[lane & 3][lane >> 2], o->wl[lane & 3][lane >> 2]);
-            if (lane == 31) o->total = ex2(l1);
-            if (head == kHeads - 1) warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
+            if (!LOCAL) {
+                put(o->la, l0, l1);
+                put(o->lb, l0 - __log2f(d0), l1 - __log2f(d1));
+                put(o->cf, ex2(rest + a1) * d0, ex2(rest) * d1);
+                put(o->e, ex2(l0), ex2(l1));
+            }
+            const float end = LOCAL ? (head ? later[1] : later[0]) : 0.0f;
+            split2_bf16(ex2(behind + a1 + end) * d0, ex2(behind + end) * d1, o->wh[lane & 3][lane >> 2], o->wl[lane & 3][lane >> 2]);
+            if (lane == 31) o->total = ex2(l1 + end);
+            if (LOCAL) {
+                const float sum = __shfl_sync(0xffffffffu, up, 31);
+                later[0] += head ? 0.0f : sum;
+                later[1] += head ? sum : 0.0f;
+            }
+            if (kGateWriters == 2 || head == kHeads - 1) warp_arrive(bar(bars.gates[c & (kGateStages - 1)]), lane);
         }
     } else if (warp >= 4 && warp < 8) {
         // -------------------------------------------------------------- state path
@@ -664,11 +689,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // the state goes in and out in whole 32-byte sectors.
         const int64_t frag = static_cast<int64_t>(lane_base + (lane >> 2)) * kSsmState + 2 * (lane & 3);
         float *const after = LOCAL ? args.ends + end_at * kSsmState : (last ? p.new_state + state_at : nullptr);
-        float product = 1.0f;           // of the segment's decays
+        const bool there = first != nullptr && !(lone && lane_base >= 64);
+        bool ok = true;
+        if (!LOCAL) {
 #pragma unroll 1
         for (int u = 0; u < 8; ++u) {                   // 16 rows x 32 columns
             const int lh = u >> 2, q = u & 3;
-            const bool there = first != nullptr && !(lone && lane_base >= 64);
             const float *from = first + frag + lh * 16 * kSsmState + 32 * q;
             uint32_t r[16];
 #pragma unroll
@@ -683,18 +709,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             tmem_st_acc32(tmem_addr(tm, lane_base + 16 * lh, TM::S + 32 * q), r);
         }
         tmem_wait_st();
-        bool ok = true;
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             if (!(ok = gates_full(c))) break;
             const float decay = gates_of(c, hrow)->total;
-            if (LOCAL) {
-                product *= decay;
-                warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
-            } else if (c >= 1) {
-                // Yi of the chunk before has read the copy
-                if (!(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
-            }
+            // Yi of the chunk before has read the copy
+            if (c >= 1 && !(ok = wait.warp(bar(bars.cs), c - 1, kSsmCS))) break;
             // the state is up to date
             if (c >= 1 && !(ok = wait.warp(bar(bars.s), c - 1, kSsmS))) break;
             const uint64_t d2 = f2(decay, decay);
@@ -703,11 +723,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 uint32_t r[32], b[16];
                 tmem_ld32(tmem_addr(tm, lane_base, TM::S + 32 * q), r);
                 tmem_wait_ld_dep(r);
-                if (!LOCAL) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                    tmem_st16(tmem_addr(tm, lane_base, TM::SB + 16 * q), b);
-                }
+                for (int j = 0; j < 16; ++j) b[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                tmem_st16(tmem_addr(tm, lane_base, TM::SB + 16 * q), b);
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
                     float v0, v1;
@@ -721,8 +739,24 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);
         }
-        if (LOCAL) args.decays[end_at + row] = product;
-        if (ok && wait.warp(bar(bars.s), nch - 1, kSsmS) && after && !(lone && lane_base >= 64 && !LOCAL)) {
+        }
+        if (LOCAL) {
+            // (a thread suspended for a whole segment wakes microseconds late: along with the gates)
+#pragma unroll 1
+            for (int c = 0; c < nch; ++c) {
+                if (!gates_full(c)) break;
+                if (c + 1 < nch) warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);
+            }
+            __syncwarp();
+            // the products are all done, also after a give-up; the gates' last total is the segment's
+            wait.drain(bar(bars.last[0]), 0, kSsmS);
+            ok = __all_sync(0xffffffffu, wait_control()->abort == 0);
+            tc_fence_after();
+        } else {
+            ok = ok && wait.warp(bar(bars.s), nch - 1, kSsmS);
+        }
+        if (LOCAL && ok) args.decays[end_at + row] = gates_of(nch - 1, hrow)->total;
+        if (ok && after && !(lone && lane_base >= 64 && !LOCAL)) {
 #pragma unroll 1
             for (int u = 0; u < 8; ++u) {
                 const int lh = u >> 2, q = u & 3;
@@ -901,7 +935,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         for (int c = 0; c < nch; ++c) {
             const int st = c % kStages;
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
-            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
+            const int nt = LOCAL ? kL : static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
             if (!gates_full(c)) break;
             if (!wait.warp(bar(bars.full[st]), c / kStages, kSsmTma)) break;
             const uint32_t xs = sbase + OFF_STAGE + st * STAGE + ST_X;
@@ -939,9 +973,11 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
             }
             // (the update of the chunk before has read the operand; all but the stores is done by then)
-            if (c >= 1 && !wait.warp_inline(bar(bars.s), c - 1, kSsmS)) break;
-            tmem_st_frag32(tmem_addr(tm, p0, TM::W), hi);
-            tmem_st_frag32(tmem_addr(tm, p0, TM::W + 32), lo);
+            if (LOCAL ? c >= 2 && !wait.warp_inline(bar(bars.g[c & 1]), (c >> 1) - 1, kSsmS)
+                      : c >= 1 && !wait.warp_inline(bar(bars.s), c - 1, kSsmS)) break;
+            const uint32_t w_at = tmem_addr(tm, p0, LOCAL && (c & 1) ? TM::G : TM::W);
+            tmem_st_frag32(w_at, hi);
+            tmem_st_frag32(w_at + 32, lo);
             tmem_wait_st();
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);
@@ -956,8 +992,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 }
 // ends[slot of segment j] <- the state behind segment j, for all but a sequence's last: what
 // the segment added, plus the state in front of it times the segment's decay.  One thread per
-// four state elements; nothing to do for the first segment, whose local pass started from
-// the sequence's state.
+// four state elements.
 constexpr int kCombineThreads = 256, kCombineCtas = kRows * kSsmState / 4 / kCombineThreads;
 __global__ void __launch_bounds__(kCombineThreads) ssm_combine_kernel(const TcArgs args) {
     const int64_t chain = blockIdx.x / kCombineCtas, n = chain / args.slabs;
@@ -967,12 +1002,17 @@ __global__ void __launch_bounds__(kCombineThreads) ssm_combine_kernel(const TcAr
     int64_t s0, s1;
     sequence_of(args.a, n, s0, s1);
     const int64_t segments = segments_of(args, s1 - s0), slot = first_slot(args, n);
-    if (segments < 3) return;
+    if (segments < 2) return;
     auto block = [&](int64_t j) { return (slot + j) * args.slabs + slab; };
     auto *ends = reinterpret_cast<float4 *>(args.ends);
     constexpr int kVecs = kRows * kSsmState / 4;
-    float4 state = ends[block(0) * kVecs + at];
-    for (int64_t j = 1; j < segments - 1; ++j) {
+    const SsmArgs &p = args.a;
+    const int R = p.heads / p.groups, in_group = slab % args.per_group, heads = kRows / p.head_size;
+    const int h0 = slab / args.per_group * R + in_group * heads;
+    float4 state = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (p.state && h0 + row / p.head_size < (slab / args.per_group + 1) * R)      // (a pair's second head may be missing)
+        state = reinterpret_cast<const float4 *>(p.state + (n * p.heads + h0) * p.head_size * static_cast<int64_t>(kSsmState))[at];
+    for (int64_t j = 0; j < segments - 1; ++j) {
         float4 e = ends[block(j) * kVecs + at];
         const float d = args.decays[block(j) * kRows + row];
         e.x = fmaf(d, state.x, e.x);
@@ -1036,11 +1076,10 @@ cudaError_t launch_passes(const CUtensorMap *maps, const TcArgs &a, int64_t slot
 
 // Tokens of a segment, or 0 for no cuts, of a call with `chains` (sequence, slab) pairs, so that
 // few long prompts use all SMs.  A sequence of mean length takes about 1.15 us a chunk as one;
-// in k segments, at most as many as fill the SMs once, a segment's chunks take 0.93 us more
+// in k segments, at most as many as fill the SMs once, a segment's chunks take 0.75 us more
 // (the local pass), and the two launches more about 14 us.  The k with the least time: 1 x
-// 16,384 tokens in 32 chains 294 us uncut and 147 in four segments, 1 x 2048 in 4 chains 67
-// and 33 in eight; 1 x 1024 in 32 chains stays whole at 28 us (36 in two), and so does 2 x 4096
-// in 64 chains at 84 us (87).
+// 16,384 tokens in 32 chains 294 us uncut and 138 in four segments, 1 x 2048 in 4 chains 67
+// and 30 in eight; 1 x 1024 in 32 chains stays whole at 28 us (36 in two).
 int64_t segment_tokens(int64_t tokens, int64_t num_seqs, int64_t chains, int sms) {
     const int64_t chunks = (tokens + num_seqs * kL - 1) / (num_seqs * kL);
     const int64_t most = sms / chains < chunks / 4 ? sms / chains : chunks / 4;
@@ -1048,7 +1087,7 @@ int64_t segment_tokens(int64_t tokens, int64_t num_seqs, int64_t chains, int sms
     double least = 1.15 * static_cast<double>(chunks);
     for (int64_t k = 2; k <= most; ++k) {
         const int64_t part = (chunks + k - 1) / k;
-        const double time = (1.15 + 0.93) * static_cast<double>(part) + 14.0;
+        const double time = (1.15 + 0.75) * static_cast<double>(part) + 14.0;
         if (time < least) {
             least = time;
             best = part * kL;

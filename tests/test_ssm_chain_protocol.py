@@ -22,8 +22,8 @@ STAGES, GATE_STAGES = 3, 4
 
 def counts(heads, local=False):
     c = dict(s=1, cs=1, yread=Y_WARPS)
-    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, 4 + SPLIT_WARPS), ("last", 2, 1),
-                    ("g", 2, 1), ("mread", 2, M_WARPS), ("gates", GATE_STAGES, 1), ("ydone", GATE_STAGES, 4 + SPLIT_WARPS if local else Y_WARPS),
+    for k, n, v in (("full", STAGES, 1), ("empty", STAGES, 2), ("update", 2, SPLIT_WARPS if local else 4 + SPLIT_WARPS), ("last", 2, 1),
+                    ("g", 2, 1), ("mread", 2, M_WARPS), ("gates", GATE_STAGES, heads if local else 1), ("ydone", GATE_STAGES, 4 + SPLIT_WARPS if local else Y_WARPS),
                     ("mx", 2, 1), ("mready", 2, M_WARPS), ("zfull", 2, 1), ("yst", 2, Y_WARPS), ("yfree", 2, 1)):
         c.update({f"{k}{i}": v for i in range(n)})
     return c
@@ -60,9 +60,9 @@ def issue_state(sim):
             break
         if not (yield ("wait", f"update{c & 1}", c >> 1)):
             break
-        sim.mma({("B", c % STAGES): c, **{("W", w): c for w in range(SPLIT_WARPS)}},
-                {("S", q): (("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
-        sim.commit("s")
+        sim.mma({("B", c % STAGES): c, **{("W", c & 1 if sim.local else 0, w): c for w in range(SPLIT_WARPS)}},
+                {("S", q): ((("S", c) if c else None) if sim.local else ("dec", c), ("S", c + 1)) for q in Q4}, f"S update({c})")
+        sim.commit(f"g{c & 1}" if sim.local else "s")
         for _ in range(2 if sim.local else 1):
             sim.commit(f"empty{c % STAGES}")
         ns += 1
@@ -74,7 +74,10 @@ def issue_state(sim):
     yield ("drain", "last0", 0)
     for c in range(max(0, ng - sim.g_buffers), ng):
         yield ("drain", f"g{c % sim.g_buffers}", c // sim.g_buffers)
-    if ns:
+    if sim.local:
+        for c in range(max(0, ns - 2), ns):
+            yield ("drain", f"g{c & 1}", c >> 1)
+    elif ns:
         yield ("drain", "s", ns - 1)
 
 
@@ -124,13 +127,13 @@ def copier(sim):
         yield ("drain", f"zfull{c & 1}", c >> 1)
 
 
-def gates(sim):
+def gates(sim, heads):
     for c in range(sim.nch):
         gs = c % GATE_STAGES
-        for head in range(sim.heads):
-            if head == 0 and c >= GATE_STAGES and not (yield ("wait", f"ydone{gs}", c // GATE_STAGES - 1)):
+        for head in heads:
+            if head == heads[0] and c >= GATE_STAGES and not (yield ("wait", f"ydone{gs}", c // GATE_STAGES - 1)):
                 return
-            sim.write(("GT", gs, head), c, "gates")
+            sim.write(("GT", gs, head), c, f"gates{heads[0]}")
             yield None
         sim.b[f"gates{gs}"].arrive()
 
@@ -146,21 +149,29 @@ def read_gates(sim, c, who):
 
 def state(sim, q):
     who, ok = f"state{q}", True
+    if sim.local:
+        for c in range(sim.nch):
+            if not (yield gates_full(c)):
+                break
+            if c + 1 < sim.nch:
+                sim.b[f"ydone{c % GATE_STAGES}"].arrive()
+        yield ("drain", "last0", 0)
+        if not sim.abort:
+            read_gates(sim, sim.nch - 1, who)
+            sim.read(("S", q), ("S", sim.nch), who)
+        return
     sim.write(("S", q), ("S", 0), who)
     for c in range(sim.nch):
         if not (ok := (yield gates_full(c))):
             break
         read_gates(sim, c, who)
-        if sim.local:
-            sim.b[f"ydone{c % GATE_STAGES}"].arrive()
-        elif c >= 1 and sim.plant != "late_copy" and not (ok := (yield ("wait", "cs", c - 1))):
+        if c >= 1 and sim.plant != "late_copy" and not (ok := (yield ("wait", "cs", c - 1))):
             break
         if c >= 1 and not (ok := (yield ("wait", "s", c - 1))):
             break
         sim.read(("S", q), ("S", c), who)
         yield None
-        if not sim.local:
-            sim.write(("SB", q), c, who)
+        sim.write(("SB", q), c, who)
         sim.write(("S", q), ("dec", c), who)
         yield None
         sim.b[f"update{c & 1}"].arrive()
@@ -235,9 +246,12 @@ def split(sim, q):
             sim.b[f"ydone{c % GATE_STAGES}"].arrive()
         sim.read(("X", st), c, who)
         yield None
-        if c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
+        if sim.local:
+            if c >= 2 and sim.plant != "no_s" and not (yield ("wait", f"g{c & 1}", (c >> 1) - 1)):
+                return
+        elif c >= 1 and sim.plant != "no_s" and not (yield ("wait", "s", c - 1)):
             return
-        sim.write(("W", q), c, who)
+        sim.write(("W", c & 1 if sim.local else 0, q), c, who)
         yield None
         sim.b[f"update{c & 1}"].arrive()
 
@@ -246,7 +260,8 @@ def run(nch, seed, heads=2, gated=True, plant=None, timeouts=False, local=False,
     sim = Scan(nch, heads, gated, plant, local)
     rng = random.Random(seed)
     roles = {"state issue": issue_state(sim), "output issue": issue_outputs(sim), "copier": copier(sim)}
-    roles["gates"] = gates(sim)
+    turns = [[h] for h in range(heads)] if local else [list(range(heads))]      # of the gates' warps
+    roles.update({f"gates{t[0]}": gates(sim, t) for t in turns})
     roles.update({f"state{q}": state(sim, q) for q in Q4})
     roles.update({f"out{w}": outputs(sim, w) for w in range(Y_WARPS)})
     roles.update({f"m{w}": scores(sim, w) for w in range(M_WARPS)})
@@ -346,6 +361,13 @@ def test_barrier_counts_match_the_kernel():
         if bound:
             loop = sizes.get(bound) or int(bound)
             continue
-        v = {"kHeads": 2, "kGateReaders": Y_WARPS}.get(n) or (int(n) if n.isdigit() else consts[n])
+        v = {"kHeads": 2, "kGateReaders": Y_WARPS, "kUpdateArrivals": 4 + SPLIT_WARPS, "kGateWriters": 1}.get(n) or (int(n) if n.isdigit() else consts[n])
         found.update({name + i: v for i in (map(str, range(loop)) if many else ("",))})
     assert found == counts(2)
+
+
+def test_planted_mistakes_of_the_local_pass_are_caught():
+    for plant in ("no_s", "no_empty"):
+        with pytest.raises(ProtocolError):
+            for seed in range(300):
+                run(6, seed, gated=False, plant=plant, local=True)
