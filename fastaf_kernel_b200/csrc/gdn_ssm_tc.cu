@@ -16,7 +16,7 @@
 //   G    = C B^T                 scores [i][j]; A is the C tile's 64 rows (the other 64 rows
 //                                of the M = 128 tile read what lies behind it and are unused)
 //   Yi^T = bf16(S) C^T           the state's part, scaled by exp(la_i) per column afterwards
-//   Ya^T = x^T bf16(M)^T         the chunk's own part; D sits on M's diagonal
+//   Ya^T = x^T bf16(M)^T         the chunk's own part
 //   S   += (w x)^T B             w x as bf16 hi + lo (two products), so the fp32 state loses
 //                                2^-16 per term, not 2^-8: with w = wh + wl in bf16,
 //                                hi = bf16(x wh) and lo = bf16(x wl + (x wh - hi)), whose
@@ -30,6 +30,10 @@
 // block; the 8 rows of the block itself take one exponential per element.  So a row of 32
 // columns takes 12 exponentials, and none overflows however strong the decays are.
 //
+// D x is added in fp32 where the outputs are formed, from the staged x tile.  On M's diagonal,
+// where it needs no read of x, it is rounded to bf16 together with the token's own score: D to 8
+// bits, an error of one sign for all tokens of a head, and own scores below half a step of D lost.
+//
 // Roles (28 warps), handing chunks to each other through mbarriers:
 //   warp 0        issues the state update(c), then G(c + 1); allocates TMEM
 //   warp 3        issues Yi(c), Ya(c) (one thread alone could not keep the tensor pipe busy)
@@ -40,8 +44,8 @@
 //   warps 12-15, 24-27   w x hi / lo into TMEM, 16 state rows each; the rows behind the last
 //                 token set to zero
 //   warps 16, 17, 1   M, a 32 x 32 block each
-//   warps 8-11, 20-23   outputs, 32 tokens each: Yi, Ya from TMEM as accumulator fragments, the
-//                 gate z, transposed into bf16 rows in shared memory (stmatrix)
+//   warps 8-11, 20-23   outputs, 32 tokens each: Yi, Ya from TMEM as accumulator fragments, D x,
+//                 the gate z, transposed into bf16 rows in shared memory (stmatrix)
 //   warp 19       output rows to global memory (TMA; the last, partial chunk by hand)
 // The loops are kept rolled and the waits out of line: together they have to fit the SM's
 // instruction caches (with everything unrolled a chunk took 7,200 cycles, two thirds of the
@@ -558,6 +562,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (c < nch) {
                 const uint32_t st = static_cast<uint32_t>(c % kStages), b = bar(bars.full[st]);
                 if (c >= kStages && !wait.warp(bar(bars.empty[st]), c / kStages - 1, kSsmFree)) break;
+                // (the products have read the stage; so have the outputs, for D x)
+                if (!LOCAL && c >= kStages && !wait.warp(bar(bars.ydone[(c - kStages) & (kGateStages - 1)]),
+                                                         (c - kStages) / kGateStages, kSsmY)) break;
                 if (lane == 0) mbar_arrive_expect_tx(b, LOCAL ? STAGE - kTile : STAGE);
                 __syncwarp();
                 if (staged) tma_load_2d(sbase + OFF_STAGE + st * STAGE + lane * 8192, map, b, x, t);
@@ -779,10 +786,13 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const int mi = lane >> 3, r8 = lane & 7, i0 = warp >= 20 ? 32 : 0;      // the warp's first token
         const uint32_t yi_at = tmem_addr(tm, lane_base, TM::YI + i0), ya_at = tmem_addr(tm, lane_base, TM::YA + (PAIR ? hrow * 64 : 0) + i0);
         const uint32_t at = (lane_base >> 6) * 8192 + sw128(i0 + 8 * (mi >> 1) + r8, ((lane_base & 63) >> 3) + (mi & 1));
+        const float D = p.D ? load_scalar(p.D, lone ? h0 : h0 + hrow, p.param_dtype) : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const float *e = gates_of(c, hrow)->e + i0 + 2 * (lane & 3);
+            const uint32_t xs = sbase + OFF_STAGE + (c % kStages) * STAGE + ST_X;
             if (!wait.warp(bar(bars.mx[c & 1]), c >> 1, kSsmMX)) break;      // (Yi went out before Ya)
+            if (p.D && !wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma)) break;
             uint64_t y[4][4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {          // 16 state rows x 16 tokens
@@ -801,7 +811,16 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             // the accumulators are free for the next chunk while this one's rows are gated and stored
             tc_fence_before();
             warp_arrive(bar(bars.yread), lane);
-            warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates read)
+            if (p.D) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t xr[4];
+                    ldsm_x4_t(xr, xs + ((u & 1) ? at ^ 32u : at) + (u >> 1) * 2048);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[u][k] = fma_f2(f2(D, D), f2(bf16_lo(xr[k]), bf16_hi(xr[k])), y[u][k]);
+                }
+            }
+            warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);     // (gates and x read)
             if (gated && !wait.warp(bar(bars.zfull[c & 1]), c >> 1, kSsmZ)) break;
             // the stores two chunks before have read the staging rows (z's copy waited for them)
             if (!gated && c >= 2 && !wait.warp(bar(bars.yfree[c & 1]), (c >> 1) - 1, kSsmStage)) break;
@@ -862,8 +881,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // columns 32..63.
         const int j0 = warp == 1 ? 32 : 0;
         const int block = (row - j0) >> 3;      // the 8 of its columns that hold the row's diagonal entry
-        const float D0 = p.D && warp != 17 ? load_scalar(p.D, h0, p.param_dtype) : 0.0f;
-        const float D1 = p.D && warp != 17 && PAIR && !lone ? load_scalar(p.D, h0 + 1, p.param_dtype) : D0;
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
@@ -910,13 +927,6 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                         b[j / 2] = pack_bf16x2(m0, m1);
                     }
                     *reinterpret_cast<uint4 *>(tiles + k * 8192 + sw128(row, (j0 >> 3) + q)) = make_uint4(b[0], b[1], b[2], b[3]);
-                }
-            }
-            if (warp != 17) {                              // D on the diagonal: onto the rounded entry, rounded again
-#pragma unroll
-                for (int k = 0; k < kHeads; ++k) {
-                    auto *d = reinterpret_cast<__nv_bfloat16 *>(tiles + k * 8192 + sw128(row, row >> 3) + (row & 7) * 2);
-                    *d = __float2bfloat16_rn(__bfloat162float(*d) + (k ? D1 : D0));
                 }
             }
             tc_fence_before();
