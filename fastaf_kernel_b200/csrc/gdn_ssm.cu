@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kSsmThreads, 3) ssm_decode_kernel(const SsmArg
     load_cols(p.C, b * p.C_stride + g * kSsmState, lane8, raw);
     unpack_cols(raw, Cf);
     const float dt = ssm_step(p, b, h);
-    const float decay = expf(-expf(load_scalar(p.A_log, h, p.param_dtype)) * dt);
+    const float decay = expf(-ssm_rate(load_scalar(p.A_log, h, p.param_dtype)) * dt);
     const float D = p.D ? load_scalar(p.D, h, p.param_dtype) : 0.0f;
 
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kSsmThreads) ssm_recurrent_kernel(const SsmArg
         s[4 * m + 0] = v.x; s[4 * m + 1] = v.y;
         s[4 * m + 2] = v.z; s[4 * m + 3] = v.w;
     }
-    const float negA = -expf(load_scalar(p.A_log, h, p.param_dtype));
+    const float negA = -ssm_rate(load_scalar(p.A_log, h, p.param_dtype));
     const float D = p.D ? load_scalar(p.D, h, p.param_dtype) : 0.0f;
 
     uint2 rb[4], rc[4];

@@ -21,4 +21,12 @@ __device__ __forceinline__ float ssm_step(const SsmArgs &p, int64_t row, int h) 
     return softplus_torch(v);
 }
 
+// exp(A_log), NaN if A_log is, and at most the largest finite number: with an infinite rate a
+// step of length zero, such as that of a row behind the last token, would be 0 x inf.
+__device__ __forceinline__ float ssm_rate(float A_log) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(expf(A_log)), "f"(3.402823466e38f));
+    return r;
+}
+
 }  // namespace gdn

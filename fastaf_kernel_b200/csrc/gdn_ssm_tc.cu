@@ -631,7 +631,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             bias[k] = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < kHeads; ++k) negA2[k] = -expf(negA2[k]) * 1.4426950408889634f;
+        for (int k = 0; k < kHeads; ++k) negA2[k] = max_nan(-1.4426950408889634f * ssm_rate(negA2[k]), -3.402823466e38f);
         for (int c = 1; c < kPrefetch; ++c) ahead(c);
         float later[2] = {0.0f, 0.0f};           // of the chunks behind, in the local pass
 #pragma unroll 1

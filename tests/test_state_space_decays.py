@@ -69,8 +69,7 @@ def test_single_tokens_at_rates_beyond_fp32():
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,P", [(2, 128), (3, 64)])
 def test_rates_beyond_fp32_in_cut_prompts(H, P):
-    """Segments, whose local pass sums decays from their ends: the bits of the token-serial
-    kernel's tolerance, and nothing that is not finite."""
+    """Segments, whose local pass sums decays from their ends."""
     lengths = [2500, 2533]
     i = _scan_inputs(lengths, H, 1, P, seed=83)
     i["A_log"][1] = 100.0
