@@ -40,10 +40,39 @@ bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return x < y + nb && y < x + na;
 }
 
-// Whether `rows` rows of `width` bf16 elements, `stride` apart, overlap `bytes` bytes at `out`.
-bool rows_overlap(const void *p, int64_t rows, int64_t stride, int64_t width, const void *out, size_t bytes) {
-    return p && rows > 0 && ranges_overlap(p, static_cast<size_t>((rows - 1) * stride + width) * 2, out, bytes);
+// What a call reads: `rows` rows of `width` bytes, `stride` bytes apart; or what it writes, in one
+// row.  No address or no rows: nothing.
+struct Span {
+    const char *name;
+    const void *at;
+    int64_t rows, stride, width;
+};
+Span whole(const char *name, const void *at, int64_t bytes) { return {name, at, bytes > 0, bytes, bytes}; }
+
+bool overlap(const Span &in, const Span &out) {
+    if (!in.at || in.rows <= 0 || !out.at || out.rows <= 0) return false;
+    const auto p = reinterpret_cast<uintptr_t>(in.at), o = reinterpret_cast<uintptr_t>(out.at);
+    // the first row that does not end in front of the destination starts in front of its end?
+    const uintptr_t k = p + in.width > o ? 0 : (o - p - in.width) / in.stride + 1;
+    return k < static_cast<uintptr_t>(in.rows) && p + k * in.stride < o + out.width;
 }
+
+// Threads write what others have yet to read, or write too, where a destination overlaps an input
+// or another destination.  (state and new_state, which may be one for single tokens, are checked
+// by themselves.)
+int refuse_overlaps(const Span *in, int num_in, const Span *out, int num_out) {
+    for (int j = 0; j < num_out; ++j) {
+        for (int i = 0; i < num_in; ++i)
+            if (overlap(in[i], out[j]))
+                return fail(GDN_ERR_INVALID_ARGUMENT, "%s must not overlap %s", out[j].name, in[i].name);
+        for (int i = 0; i < j; ++i)
+            if (overlap(out[i], out[j]))
+                return fail(GDN_ERR_INVALID_ARGUMENT, "%s and %s must not overlap", out[j].name, out[i].name);
+    }
+    return GDN_OK;
+}
+
+int64_t size_of(int dtype) { return dtype == GDN_DTYPE_F32 ? 4 : 2; }
 
 bool known_dtype(int d) { return d == GDN_DTYPE_F32 || d == GDN_DTYPE_BF16; }
 
@@ -56,8 +85,8 @@ int64_t row_stride(int64_t given, int64_t width) {
 
 // The arguments prefill and decode of the convolution share, into `p`.
 int conv_args(gdn::ConvArgs &p, const void *x, int64_t x_row_stride, const void *weight, const void *bias,
-              int weight_dtype, const void *state, int64_t num_seqs, int64_t rows, int64_t channels, int width,
-              int activation, void *const *outputs, const int64_t *output_widths, int num_outputs, void *new_state) {
+              int weight_dtype, const void *state, const int32_t *cu_seqlens, int64_t num_seqs, int64_t rows,
+              int64_t channels, int width, int activation, void *const *outputs, const int64_t *output_widths, int num_outputs, void *new_state) {
     gdn::set_last_error("");
     if (width < 2 || width > 4) return fail(GDN_ERR_UNSUPPORTED, "width=%d is not supported (2, 3 or 4)", width);
     if (channels <= 0 || channels % 8 != 0 || channels > kMaxStride)
@@ -95,13 +124,20 @@ int conv_args(gdn::ConvArgs &p, const void *x, int64_t x_row_stride, const void 
         for (int j = 0; j < num_outputs; ++j)
             if (!outputs[j] || !aligned16(outputs[j]))
                 return fail(GDN_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned addresses");
-        for (int j = 0; j < num_outputs; ++j) {
-            const size_t bytes = static_cast<size_t>(rows * output_widths[j]) * 2;
-            bool hit = rows_overlap(x, rows, xs, channels, outputs[j], bytes);
-            for (int k = 0; k < j; ++k) hit |= rows_overlap(outputs[k], rows, output_widths[k], output_widths[k], outputs[j], bytes);
-            if (hit) return fail(GDN_ERR_INVALID_ARGUMENT, "outputs must not overlap x or each other");
-        }
     }
+    const int64_t state_bytes = num_seqs * (width - 1) * channels * 2;
+    const Span in[] = {{"x", x, rows, xs * 2, channels * 2},
+                       whole("weight", weight, channels * width * size_of(weight_dtype)),
+                       whole("bias", bias, channels * size_of(weight_dtype)),
+                       whole("cu_seqlens", cu_seqlens, (num_seqs + 1) * 4),
+                       whole("state", state, state_bytes)};
+    Span out[gdn::kConvMaxOutputs];
+    for (int j = 0; j < num_outputs; ++j) out[j] = whole("output", outputs[j], rows * output_widths[j] * 2);
+    int rc = refuse_overlaps(in, 5, out, num_outputs);
+    if (rc != GDN_OK) return rc;
+    const Span kept = whole("new_state", new_state, state_bytes);
+    if ((rc = refuse_overlaps(in, 4, &kept, 1)) != GDN_OK || (rc = refuse_overlaps(out, num_outputs, &kept, 1)) != GDN_OK)
+        return rc;
     p.x = x;
     p.x_stride = xs;
     p.weight = weight;
@@ -126,8 +162,8 @@ size_t conv_state_bytes(const gdn::ConvArgs &p) {
 // The arguments prefill and decode of the scan share, into `p`.
 int ssm_args(gdn::SsmArgs &p, const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
              const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride, const void *D,
-             const void *dt_bias, const void *z, int64_t z_row_stride, const float *state, int64_t num_seqs,
-             int64_t rows, int num_heads, int num_groups, int head_size, int state_size, int dt_dtype, int param_dtype,
+             const void *dt_bias, const void *z, int64_t z_row_stride, const float *state, const int32_t *cu_seqlens,
+             int64_t num_seqs, int64_t rows, int num_heads, int num_groups, int head_size, int state_size, int dt_dtype, int param_dtype,
              void *output, float *new_state) {
     gdn::set_last_error("");
     if (state_size != 128) return fail(GDN_ERR_UNSUPPORTED, "state_size=%d is not supported (only 128)", state_size);
@@ -158,11 +194,23 @@ int ssm_args(gdn::SsmArgs &p, const void *x, int64_t x_row_stride, const void *d
         if (!x || !dt || !B || !C || !output) return fail(GDN_ERR_INVALID_ARGUMENT, "null x, dt, B, C or output");
         if (!aligned16(x) || !aligned16(B) || !aligned16(C) || !aligned16(z) || !aligned16(output))
             return fail(GDN_ERR_INVALID_ARGUMENT, "x, B, C, z and output must be 16-byte aligned");
-        const size_t bytes = static_cast<size_t>(rows * wide) * 2;
-        if (rows_overlap(x, rows, p.x_stride, wide, output, bytes) || rows_overlap(z, rows, p.z_stride, wide, output, bytes) ||
-            rows_overlap(B, rows, p.B_stride, bc, output, bytes) || rows_overlap(C, rows, p.C_stride, bc, output, bytes))
-            return fail(GDN_ERR_INVALID_ARGUMENT, "output must not overlap x, z, B or C");
     }
+    const int64_t state_bytes = num_seqs * num_heads * head_size * 128 * 4, each = size_of(dt_dtype);
+    const int64_t params = num_heads * size_of(param_dtype);
+    const Span in[] = {{"x", x, rows, p.x_stride * 2, wide * 2},
+                       {"dt", dt, rows, p.dt_stride * each, num_heads * each},
+                       {"B", B, rows, p.B_stride * 2, bc * 2},
+                       {"C", C, rows, p.C_stride * 2, bc * 2},
+                       {"z", z, rows, p.z_stride * 2, wide * 2},
+                       whole("A_log", A_log, params),
+                       whole("D", D, params),
+                       whole("dt_bias", dt_bias, params),
+                       whole("cu_seqlens", cu_seqlens, (num_seqs + 1) * 4),
+                       whole("state", state, state_bytes)};
+    const Span out = whole("output", output, rows * wide * 2), kept = whole("new_state", new_state, state_bytes);
+    int rc = refuse_overlaps(in, 10, &out, 1);
+    if (rc != GDN_OK || (rc = refuse_overlaps(in, 9, &kept, 1)) != GDN_OK || (rc = refuse_overlaps(&out, 1, &kept, 1)) != GDN_OK)
+        return rc;
     p.x = x;
     p.dt = dt;
     p.B = B;
@@ -197,8 +245,8 @@ int gdn_conv_prefill(const void *x, int64_t x_row_stride, const void *weight, co
                      int64_t channels, int width, int activation, void *const *outputs, const int64_t *output_widths,
                      int num_outputs, void *new_state, void *stream) {
     gdn::ConvArgs p{};
-    const int rc = conv_args(p, x, x_row_stride, weight, bias, weight_dtype, state, num_seqs, total_tokens, channels,
-                             width, activation, outputs, output_widths, num_outputs, new_state);
+    const int rc = conv_args(p, x, x_row_stride, weight, bias, weight_dtype, state, cu_seqlens, num_seqs, total_tokens,
+                             channels, width, activation, outputs, output_widths, num_outputs, new_state);
     if (rc != GDN_OK || num_seqs == 0) return rc;
     if (!cu_seqlens) return fail(GDN_ERR_INVALID_ARGUMENT, "null cu_seqlens");
     // (a long sequence is split over threads: its end writes what its start reads)
@@ -214,8 +262,8 @@ int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *weight, con
                     void *const *outputs, const int64_t *output_widths, int num_outputs, void *new_state,
                     void *stream) {
     gdn::ConvArgs p{};
-    const int rc = conv_args(p, x, x_row_stride, weight, bias, weight_dtype, state, batch, batch, channels, width,
-                             activation, outputs, output_widths, num_outputs, new_state);
+    const int rc = conv_args(p, x, x_row_stride, weight, bias, weight_dtype, state, nullptr, batch, batch, channels,
+                             width, activation, outputs, output_widths, num_outputs, new_state);
     if (rc != GDN_OK || batch == 0) return rc;
     if (state && state != new_state && ranges_overlap(state, conv_state_bytes(p), new_state, conv_state_bytes(p)))
         return fail(GDN_ERR_INVALID_ARGUMENT, "new_state partially overlaps state (only exact aliasing is allowed)");
@@ -239,8 +287,8 @@ int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t
                     int method, void *stream) {
     gdn::SsmArgs p{};
     const int rc = ssm_args(p, x, x_row_stride, dt, dt_row_stride, A_log, B, B_row_stride, C, C_row_stride, D, dt_bias,
-                            z, z_row_stride, state, num_seqs, total_tokens, num_heads, num_groups, head_size,
-                            state_size, dt_dtype, param_dtype, output, new_state);
+                            z, z_row_stride, state, cu_seqlens, num_seqs, total_tokens, num_heads, num_groups,
+                            head_size, state_size, dt_dtype, param_dtype, output, new_state);
     if (rc != GDN_OK) return rc;
     if (method != GDN_PREFILL_AUTO && method != GDN_PREFILL_RECURRENT && method != GDN_PREFILL_TCGEN05)
         return fail(GDN_ERR_INVALID_ARGUMENT, "unknown scan method %d", method);
@@ -266,8 +314,8 @@ int gdn_ssm_decode(const void *x, int64_t x_row_stride, const void *dt, int64_t 
                    void *output, float *new_state, void *stream) {
     gdn::SsmArgs p{};
     const int rc = ssm_args(p, x, x_row_stride, dt, dt_row_stride, A_log, B, B_row_stride, C, C_row_stride, D, dt_bias,
-                            z, z_row_stride, state, batch, batch, num_heads, num_groups, head_size, state_size,
-                            dt_dtype, param_dtype, output, new_state);
+                            z, z_row_stride, state, nullptr, batch, batch, num_heads, num_groups, head_size,
+                            state_size, dt_dtype, param_dtype, output, new_state);
     if (rc != GDN_OK || batch == 0) return rc;
     if (state && state != new_state && ranges_overlap(state, ssm_state_bytes(p), new_state, ssm_state_bytes(p)))
         return fail(GDN_ERR_INVALID_ARGUMENT, "new_state partially overlaps state (only exact aliasing is allowed)");

@@ -218,8 +218,8 @@ def conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
 
     ``split`` gives the widths of up to four packed tensors that take the channels side by
     side, such as q, k and v for ``kernel`` or x, B and C for ``ssm_prefill``; y (and
-    ``output``) is then a tuple of [T, width] tensors.  Outputs must not overlap x or each
-    other, nor new_state state.
+    ``output``) is then a tuple of [T, width] tensors.  Outputs and new_state must overlap
+    neither each other nor an input.
     """
     index = _device_of("x weight bias state", (x, weight), (bias, state))
     if x.dim() != 2:
@@ -318,7 +318,7 @@ def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch
     H / G consecutive heads of a group; A_log, D, dt_bias [H] (D and dt_bias may be None);
     state [N, H, P, 128] fp32 or None for zeros; cu_seqlens [N+1] as for ``kernel``.  Returns
     (y [T, H, P] bf16, new_state [N, H, P, 128] fp32); a sequence of length 0 keeps its
-    state.  ``output`` must not overlap x, z, B or C, nor new_state state.
+    state.  ``output`` and new_state must overlap neither each other nor an input.
 
     ``method`` chooses the kernel: "tcgen05" (64-token chunks on the tensor cores, from 64
     tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what

@@ -298,8 +298,9 @@ GDN_API int gdn_decode_strided(const void *q, const void *k, const void *v, cons
  *               each sequence (its state unchanged when it is empty); must not overlap state
  *
  * Requirements: width 2, 3 or 4; channels and every output width multiples of 8; 16-byte
- * aligned pointers (weight and bias: their element's alignment).  Outputs must not overlap
- * x or each other.  total_tokens and num_seqs below 2^31 - 256.
+ * aligned pointers (weight and bias: their element's alignment).  Outputs and new_state must
+ * overlap neither each other nor anything that the call reads.  total_tokens and num_seqs below
+ * 2^31 - 256.
  */
 GDN_API int gdn_conv_prefill(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
                      int weight_dtype, const void *state, const int32_t *cu_seqlens, int64_t num_seqs,
@@ -308,7 +309,7 @@ GDN_API int gdn_conv_prefill(const void *x, int64_t x_row_stride, const void *we
 
 /* The same convolution for one token of each of `batch` sequences: x [batch][channels]
  * (rows x_row_stride apart), outputs [batch][output_widths[j]].  new_state may be the same
- * pointer as state (in place), but must not partially overlap it. */
+ * pointer as state (in place), but must not partially overlap it; other overlaps as above. */
 GDN_API int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *weight, const void *bias,
                     int weight_dtype, const void *state, int64_t batch, int64_t channels, int width,
                     int activation, void *const *outputs, const int64_t *output_widths, int num_outputs,
@@ -340,9 +341,10 @@ GDN_API int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *wei
  *
  * Requirements: head_size 64 or 128, state_size 128, num_heads % num_groups == 0; x, z, B,
  * C, output, state and new_state 16-byte aligned and the row strides of x, z, B and C
- * multiples of 8.  The output must not overlap x, z, B or C.  A sequence's outputs and state
- * depend on its own rows alone.  Within a sequence, GDN_PREFILL_TCGEN05 lets an infinity or
- * NaN in x, dt, B or C also reach the outputs of the tokens before it in its 64-token chunk.
+ * multiples of 8.  output and new_state must overlap neither each other nor anything that the
+ * call reads.  A sequence's outputs and state depend on its own rows alone.  Within a sequence,
+ * GDN_PREFILL_TCGEN05 lets an infinity or NaN in x, dt, B or C also reach the outputs of the
+ * tokens before it in its 64-token chunk.
  */
 GDN_API int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
                     const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,
@@ -357,7 +359,7 @@ GDN_API int gdn_ssm_resolve(int64_t total_tokens, int64_t num_seqs, int method);
 
 /* One step of the scan for each of `batch` sequences (rows of one token each; state, and
  * output [batch][num_heads][head_size]).  new_state may be the same pointer as state (in
- * place), but must not partially overlap it. */
+ * place), but must not partially overlap it; other overlaps as above. */
 GDN_API int gdn_ssm_decode(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
                    const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,
                    const void *D, const void *dt_bias, const void *z, int64_t z_row_stride, const float *state,
