@@ -17,14 +17,14 @@
 //                                of the M = 128 tile read what lies behind it and are unused)
 //   Yi^T = bf16(S) C^T           the state's part, scaled by exp(la_i) per column afterwards
 //   Ya^T = x^T bf16(M)^T         the chunk's own part
-//   S   += (w x)^T B             w x as bf16 hi + lo (two products), so the fp32 state loses
-//                                2^-16 per term, not 2^-8: with w = wh + wl in bf16,
-//                                hi = bf16(x wh) and lo = bf16(x wl + (x wh - hi)), whose
-//                                inner difference is exact -- three bf16 operations for two
-//                                terms; a TMEM operand, which keeps 48 KB a chunk out of the
-//                                shared memory's bandwidth.  (A third term would want 32 more TMEM
-//                                columns, which pairs of heads do not have, and a third of these
-//                                products again; the state's error is a few 2^-18 of its magnitude.)
+//   S   += (w x)^T B             w x in fp32, cut into three bf16 numbers (8 of its 24 bits each, so
+//                                exactly), three products: the fp32 state is as good as fp32 sums
+//                                (relative error 3e-7; two terms left 4e-6).  Terms one and two are
+//                                a TMEM operand, which keeps 48 KB a chunk out of the shared
+//                                memory's bandwidth.  The third has no TMEM columns of its own: with
+//                                one head it lies in shared memory, where M leaves room; with two
+//                                it takes the place of bf16(S) when Yi has read that; the local
+//                                pass, which has neither M nor Yi, holds all three in TMEM.
 // M's exponentials factor by blocks of 8 columns: exp(la_i - la_j) = exp(la_i - la_r)
 // exp(la_r - la_j) with r the block's last column, both at most 1 for the rows below the
 // block; the 8 rows of the block itself take one exponential per element.  So a row of 32
@@ -35,14 +35,15 @@
 // bits, an error of one sign for all tokens of a head, and own scores below half a step of D lost.
 //
 // Roles (28 warps), handing chunks to each other through mbarriers:
-//   warp 0        issues the state update(c), then G(c + 1); allocates TMEM
+//   warp 0        issues the state update(c), then G(c + 1) (with two heads the update's third term
+//                 behind that); allocates TMEM
 //   warp 3        issues Yi(c), Ya(c) (one thread alone could not keep the tensor pipe busy)
 //   warp 18       copies (TMA): three stages of C, B and x, two of z, and boxes further ahead
 //                 into L2
 //   warp 2        the chunk's gates
 //   warps 4-7     state path: S -> bf16 copy (TMEM operand of Yi) and the decay of S
-//   warps 12-15, 24-27   w x hi / lo into TMEM, 16 state rows each; the rows behind the last
-//                 token set to zero
+//   warps 12-15, 24-27   the terms of w x, 16 state rows each; the rows behind the last token set
+//                 to zero
 //   warps 16, 17, 1   M, a 32 x 32 block each
 //   warps 8-11, 20-23   outputs, 32 tokens each: Yi, Ya from TMEM as accumulator fragments, D x,
 //                 the gate z, transposed into bf16 rows in shared memory (stmatrix)
@@ -99,6 +100,7 @@ constexpr uint32_t OFF_STAGE = 0;                                // kStages x [C
 constexpr uint32_t STAGE = 3 * kTile;
 constexpr uint32_t ST_C = 0, ST_B = kTile, ST_X = 2 * kTile;
 constexpr uint32_t OFF_M = OFF_STAGE + kStages * STAGE;          // 2 x [head][i][j], K-major, 8 KB each
+constexpr uint32_t OFF_W3 = OFF_M + kTile;                       // one head: third term of w x, [token][row] as x
 constexpr uint32_t OFF_Y = OFF_M + 2 * kTile;                        // 2 x z, then the output rows in its place
 constexpr uint32_t OFF_GATE = OFF_Y + 2 * kTile;                 // kGateStages x 2 heads x Gates
 constexpr uint32_t GATE = 1408;
@@ -110,10 +112,11 @@ struct alignas(16) Gates {
     float lb[64];         // la_j - log2(dt'_j): 2^(la_i - lb_j) = exp(la_i - la_j) dt'_j
     float cf[64];         // exp(la_r - la_j) dt'_j, r = j | 7
     float e[64];          // exp(la_i)
-    // w_j = exp(la_63 - la_j) dt'_j as bf16 hi + lo, two tokens a word, word (j / 2) % 4 of all
-    // 8-token blocks side by side: what one lane of a fragment needs
-    uint32_t wh[4][8], wl[4][8];
+    // w_j = exp(la_63 - la_j) dt'_j, pairs of tokens with equal (j / 2) % 4 side by side: what one
+    // lane of a fragment needs (rows of 80 bytes: four lanes' reads in different banks)
+    float w[4][20];
     float total;          // exp(la_63)
+    float D;              // the skip term's, for the outputs
 };
 static_assert(sizeof(Gates) <= GATE, "gate block");
 
@@ -127,13 +130,15 @@ struct Tm {
     static constexpr uint32_t G = 192;                       // lanes 0..63, 64 columns a buffer
     static constexpr int kG = PAIR ? 1 : 2;
     static constexpr uint32_t YI = G + 64 * kG, YA = YI + 64;
-    static constexpr uint32_t W = YA + (PAIR ? 128 : 64);    // bf16x2 w x: 32 columns hi, 32 lo
+    static constexpr uint32_t W = YA + (PAIR ? 128 : 64);    // bf16x2 w x: 32 columns a term, two terms
+    static constexpr uint32_t W3 = SB;                       // the third, with two heads
     static_assert(W + 64 == 512, "TMEM map");
+    static constexpr uint32_t WL = 128;                      // local pass: three terms, two buffers
 };
 
 enum WaitSite { kSsmTma = 41, kSsmZ = 42, kSsmGates = 43, kSsmG = 44, kSsmM = 45, kSsmS = 46,
                 kSsmMX = 48, kSsmUpdate = 47, kSsmCS = 53, kSsmIssue = 49, kSsmY = 50, kSsmStage = 51, kSsmFree = 52,
-                kSsmRead = 54 };
+                kSsmRead = 54, kSsmThird = 55 };
 constexpr uint64_t kDrainNs = 2000000000ull;
 constexpr uint32_t kMaxSuspendNs = 1000000;
 
@@ -171,15 +176,18 @@ __device__ __forceinline__ int64_t segments_of(const TcArgs &a, int64_t tokens) 
 struct Bars {
     uint64_t full[kStages], empty[kStages], gates[kGateStages], ydone[kGateStages];
     uint64_t zfull[2], yst[2], yfree[2], mx[2], mready[2], update[2], last[2], g[2], mread[2];
-    uint64_t s, cs, yread;
+    uint64_t s, cs, yread, third;
 };
 
 // What a wait looks at besides its barrier, at the end of the dynamic shared memory.
 struct WaitControl {
     uint64_t limit;
+    uint32_t hint, units;       // the limit, at most kMaxSuspendNs, and in units of wait_clock()
     int *status;
     volatile int abort;
 };
+// A clock of one register: units of 1024 ns.
+__device__ __forceinline__ uint32_t wait_clock() { return static_cast<uint32_t>(global_timer_ns() >> 10); }
 __device__ __forceinline__ WaitControl *wait_control() {
     extern __shared__ __align__(1024) uint8_t sm[];
     return reinterpret_cast<WaitControl *>(sm + SMEM_BYTES);
@@ -190,7 +198,7 @@ __device__ __forceinline__ WaitControl *wait_control() {
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t key) {
     WaitControl *ctl = wait_control();
     const uint64_t t0 = global_timer_ns(), limit = ctl->limit;
-    const uint32_t hint = limit < kMaxSuspendNs ? static_cast<uint32_t>(limit) : kMaxSuspendNs;
+    const uint32_t hint = ctl->hint;
     for (;;) {
         if (mbar_try_wait_hint(bar, key & 1, hint)) return true;
         if (ctl->abort) return false;
@@ -247,13 +255,13 @@ struct Waiter {
         bool ok = mbar_try_wait(bar, phase & 1);
         if (!__all_sync(0xffffffffu, ok)) {
             WaitControl *ctl = wait_control();
-            const uint64_t t0 = global_timer_ns();
-            const uint32_t hint = ctl->limit < kMaxSuspendNs ? static_cast<uint32_t>(ctl->limit) : kMaxSuspendNs;
+            const uint32_t t0 = wait_clock();
             while (!ok && !ctl->abort) {
-                ok = mbar_try_wait_hint(bar, phase & 1, hint);
-                if (!ok && global_timer_ns() - t0 > ctl->limit) {
+                ok = mbar_try_wait_hint(bar, phase & 1, ctl->hint);
+                if (!ok && wait_clock() - t0 > ctl->units) {
                     if (ctl->status) atomicCAS(ctl->status, 0, site);
                     ctl->abort = 1;
+                    break;
                 }
             }
             if (!__all_sync(0xffffffffu, ok)) return false;
@@ -291,16 +299,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ uint64_t bits2(uint32_t lo, uint32_t hi) {
     return f2(__uint_as_float(lo), __uint_as_float(hi));
 }
-// Two bf16 products / fused multiply-adds, one rounding each.
-__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-__device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
+// The leading 8 bits of two numbers as a pair of bf16 (cut off, not rounded), and what is left of
+// them, exactly.
+__device__ __forceinline__ uint32_t cut_bf2(uint64_t &v) {
+    float a, b;
+    unf2(v, a, b);
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    v = sub_f2(v, bits2(ua & 0xffff0000u, ub & 0xffff0000u));
+    return __byte_perm(ua, ub, 0x7632);
 }
 // softplus(x) = max(x, 0) + log(1 + u), u = exp(-|x|) in (0, 1], with the logarithm from the
 // series log(1 + u) = 2 (s + s^3/3 + s^5/5 + ...), s = u / (2 + u) <= 1/3, whose first term
@@ -321,7 +327,7 @@ __device__ __forceinline__ float softplus_series(float x) {
 // from a segment's last chunk to its first: a token's weight, its decay to the segment's end, is
 // then known when it comes, so the products accumulate without a pass over the state in between
 // (0.75 us a chunk; in order, with the state decayed chunk by chunk, 0.93).  The scaled x has two
-// places, one in TM::G; its barriers are those of G.  A pair's gates take two warps (with one,
+// places; its barriers are those of G.  A pair's gates take two warps (with one,
 // 1 x 16,384 tokens in 32 chains of pairs took 222 us in place of 209).
 template <bool PAIR, bool LOCAL>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -368,14 +374,14 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
     if (seg < 0 || seg >= segments || (LOCAL && last)) return;      // (no such segment, or none needed)
     s0 += seg * args.segment;
     s1 = last ? s1 : s0 + args.segment;
-    const int nch = static_cast<int>((s1 - s0 + kL - 1) / kL);
+    const int tokens = static_cast<int>(s1 - s0), nch = (tokens + kL - 1) / kL;
     const bool gated = !LOCAL && p.z != nullptr;
     const uint32_t sbase = smem_u32(sm);
     auto bar = [&](const uint64_t &b) { return smem_u32(&b); };
     const Waiter wait;
 
     // this thread's state row: of head h0, or for the second half of a pair of head h0 + 1
-    const int hrow = PAIR ? row >> 6 : 0;
+    const int hrow = PAIR ? (warp & 2) >> 1 : 0;
     // the slab's 128 state rows, one after the other in memory (64 for a lone head)
     const int64_t state_at = (n * p.heads + h0) * p.head_size * static_cast<int64_t>(kSsmState);
     const int64_t end_at = (slot * args.slabs + slab) * kRows;      // their place in the segments' workspace
@@ -419,8 +425,11 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             mbar_init(bar(bars.s), 1);
             mbar_init(bar(bars.cs), 1);
             mbar_init(bar(bars.yread), kYWarps);
+            mbar_init(smem_u32(&bars.third), kSplitWarps);
             WaitControl *ctl = wait_control();
             ctl->limit = args.wait_ns;
+            ctl->hint = args.wait_ns < kMaxSuspendNs ? static_cast<uint32_t>(args.wait_ns) : kMaxSuspendNs;
+            ctl->units = args.wait_ns >> 41 ? 0x7fffffffu : static_cast<uint32_t>(args.wait_ns >> 10);
             ctl->status = p.status;
             ctl->abort = 0;
             fence_mbar_init();
@@ -451,7 +460,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const uint64_t dBm = smem_desc_sw128(sbase + OFF_STAGE + ST_B, 8192, 1024);   // MN-major
         constexpr int kAtom = 8192 >> 4, kStep = 2048 >> 4, kSt = STAGE >> 4;
         constexpr uint32_t id_g = idesc_bf16_f32(128, 64, false, false);
-        constexpr uint32_t id_s = idesc_bf16_f32(128, 128, false, true);
+        constexpr uint32_t id_s = idesc_bf16_f32(128, 128, false, true), id_w3 = idesc_bf16_f32(128, 128, true, true);
+        constexpr int kW3 = (OFF_W3 - OFF_STAGE - ST_B) >> 4;
         int ng = 0, ns = 0;
         auto scores = [&](int c) -> bool {      // G(c)
             const uint32_t st = (c % kStages) * kSt;
@@ -476,18 +486,35 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             if (LOCAL && !(ok = wait.warp(bar(bars.full[c % kStages]), c / kStages, kSsmTma))) break;
             // (the split's warps and, but for the local pass, the state path's)
             if (!(ok = wait.warp(bar(bars.update[c & 1]), c >> 1, kSsmUpdate))) break;
-            if (elect_one()) {                  // S += (w x)^T B: hi, then lo against the same B
+            if (elect_one()) {                  // S += (w x)^T B: one term after the other against the same B
+                const uint32_t w = tm + (LOCAL ? TM::WL + (c & 1) * 96 : TM::W);
+#pragma unroll 4
+                for (int k = 0; k < (LOCAL ? 12 : 8); ++k)
+                    mma_ts(tm + TM::S, w + 8 * k, dBm + st + (k & 3) * kStep, id_s, !LOCAL || c > 0 || k > 0);
+                if (!LOCAL && !PAIR) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_ts(tm + TM::S, tm + (LOCAL && (c & 1) ? TM::G : TM::W) + 8 * k, dBm + st + (k & 3) * kStep, id_s,
-                           !LOCAL || c > 0 || k > 0);
-                mma_commit(bar(LOCAL ? bars.g[c & 1] : bars.s));
-                mma_commit(bar(bars.empty[c % kStages]));
-                if (LOCAL) mma_commit(bar(bars.empty[c % kStages]));   // (for the other issuing warp)
+                    for (int k = 0; k < 4; ++k) mma_ss(tm + TM::S, dBm + kW3 + k * kStep, dBm + st + k * kStep, id_w3, 1);
+                }
+                if (LOCAL || !PAIR) {
+                    mma_commit(bar(LOCAL ? bars.g[c & 1] : bars.s));
+                    mma_commit(bar(bars.empty[c % kStages]));
+                    if (LOCAL) mma_commit(bar(bars.empty[c % kStages]));   // (for the other issuing warp)
+                }
             }
             __syncwarp();
-            ++ns;
-            if (!LOCAL && c + 1 < nch) ok = scores(c + 1);
+            if (LOCAL || !PAIR) ++ns;
+            if (!LOCAL && c + 1 < nch && !(ok = scores(c + 1))) break;
+            if (!LOCAL && PAIR) {
+                if (!(ok = wait.warp(smem_u32(&bars.third), c, kSsmThird))) break;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_ts(tm + TM::S, tm + TM::W3 + 8 * k, dBm + st + k * kStep, id_s, 1);
+                    mma_commit(bar(bars.s));
+                    mma_commit(bar(bars.empty[c % kStages]));
+                }
+                __syncwarp();
+                ++ns;
+            }
         }
         // No MMA or barrier arrive is in flight when the CTA leaves (after a give-up some may
         // have gone out without a commit of their own).
@@ -602,9 +629,9 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const bool wide = p.dt_dtype != 1;
         auto place = [&](int c) { return LOCAL ? (c < nch ? nch - 1 - c : 0) : c; };     // of the c-th chunk
         auto fetch = [&](int i, uint32_t (&to)[2]) {
-            const int64_t t = s0 + static_cast<int64_t>(place(i / kHeads)) * kL + 2 * lane;
-            const int64_t at = (t < s1 ? t : s1 - 1) * p.dt_stride + (PAIR && !lone ? h0 + (i & 1) : h0);
-            const int64_t next = t + 1 < s1 ? at + p.dt_stride : at;
+            const int t = place(i / kHeads) * kL + 2 * lane;
+            const int64_t at = (s0 + (t < tokens ? t : tokens - 1)) * p.dt_stride + (PAIR && !lone ? h0 + (i & 1) : h0);
+            const int64_t next = t + 1 < tokens ? at + p.dt_stride : at;
             if (wide) {
                 to[0] = static_cast<const uint32_t *>(p.dt)[at];
                 to[1] = static_cast<const uint32_t *>(p.dt)[next];
@@ -615,20 +642,22 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         };
         auto value = [&](uint32_t raw) { return __uint_as_float(wide ? raw : raw << 16); };
         auto ahead = [&](int c) {
-            const int64_t t = s0 + static_cast<int64_t>(place(c)) * kL + 2 * lane, at = t * p.dt_stride + h0;
+            const int t = place(c) * kL + 2 * lane;
+            const int64_t at = (s0 + t) * p.dt_stride + h0;
             const char *line = static_cast<const char *>(p.dt) + (p.dt_dtype == 1 ? 2 : 4) * at;
-            if (t < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
-            if (t + 1 < s1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (p.dt_dtype == 1 ? 2 : 4) * p.dt_stride));
+            if (t < tokens) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            if (t + 1 < tokens) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + (p.dt_dtype == 1 ? 2 : 4) * p.dt_stride));
         };
         const int turn0 = kGateWriters == 2 && warp == 19 ? 1 : 0;
         fetch(turn0, d[0]);
         fetch(turn0 + kGateWriters, d[1]);
-        float negA2[kHeads], bias[kHeads];       // log2 decay of dt' = 1
+        float negA2[kHeads], bias[kHeads], skip[kHeads];       // (negA2: log2 decay of dt' = 1)
 #pragma unroll
         for (int k = 0; k < kHeads; ++k) {
             const int h = lone ? h0 : h0 + k;
             negA2[k] = load_scalar(p.A_log, h, p.param_dtype);
             bias[k] = p.dt_bias ? load_scalar(p.dt_bias, h, p.param_dtype) : 0.0f;
+            skip[k] = !LOCAL && p.D ? load_scalar(p.D, h, p.param_dtype) : 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < kHeads; ++k) negA2[k] = max_nan(-1.4426950408889634f * ssm_rate(negA2[k]), -3.402823466e38f);
@@ -637,12 +666,12 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll 1
         for (int i = turn0; i < nch * kHeads; i += kGateWriters) {
             const int c = i / kHeads, head = PAIR ? i & 1 : 0;
-            const int64_t t0 = s0 + static_cast<int64_t>(place(c)) * kL + 2 * lane;
+            const int t0 = place(c) * kL + 2 * lane;
             fetch(i + 2 * kGateWriters, d[2]);
             if (head == 0) ahead(c + kPrefetch);
             const float b0 = PAIR && head ? bias[kHeads - 1] : bias[0];
-            const float d0 = t0 < s1 ? softplus_series(value(d[0][0]) + b0) : 0.0f;
-            const float d1 = t0 + 1 < s1 ? softplus_series(value(d[0][1]) + b0) : 0.0f;
+            const float d0 = t0 < tokens ? softplus_series(value(d[0][0]) + b0) : 0.0f;
+            const float d1 = t0 + 1 < tokens ? softplus_series(value(d[0][1]) + b0) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 d[0][k] = d[1][k];
@@ -679,9 +708,10 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 put(o->lb, l0 - __log2f(d0), l1 - __log2f(d1));
                 put(o->cf, ex2(rest + a1) * d0, ex2(rest) * d1);
                 put(o->e, ex2(l0), ex2(l1));
+                if (lane == 0) o->D = PAIR && head ? skip[kHeads - 1] : skip[0];
             }
             const float end = LOCAL ? (head ? later[1] : later[0]) : 0.0f;
-            split2_bf16(ex2(behind + a1 + end) * d0, ex2(behind + end) * d1, o->wh[lane & 3][lane >> 2], o->wl[lane & 3][lane >> 2]);
+            reinterpret_cast<float2 *>(o->w[lane & 3])[lane >> 2] = make_float2(ex2(behind + a1 + end) * d0, ex2(behind + end) * d1);
             if (lane == 31) o->total = ex2(l1 + end);
             if (LOCAL) {
                 const float sum = __shfl_sync(0xffffffffu, up, 31);
@@ -784,9 +814,8 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         // A fragment's registers hold two neighbouring tokens of one state row; stmatrix
         // writes eight rows' worth of them transposed, as 16 bytes of each token's row.
         const int mi = lane >> 3, r8 = lane & 7, i0 = warp >= 20 ? 32 : 0;      // the warp's first token
-        const uint32_t yi_at = tmem_addr(tm, lane_base, TM::YI + i0), ya_at = tmem_addr(tm, lane_base, TM::YA + (PAIR ? hrow * 64 : 0) + i0);
+        const uint32_t yi_at = tmem_addr(tm, lane_base, TM::YI + i0), ya = TM::YA - TM::YI + (PAIR ? hrow * 64 : 0);
         const uint32_t at = (lane_base >> 6) * 8192 + sw128(i0 + 8 * (mi >> 1) + r8, ((lane_base & 63) >> 3) + (mi & 1));
-        const float D = p.D ? load_scalar(p.D, lone ? h0 : h0 + hrow, p.param_dtype) : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const float *e = gates_of(c, hrow)->e + i0 + 2 * (lane & 3);
@@ -799,7 +828,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 const int lh = u & 1, hh = u >> 1;
                 uint32_t yi[8], yo[8];
                 tmem_ld_frag16(yi_at + (16u * lh << 16) + 16 * hh, yi);
-                tmem_ld_frag16(ya_at + (16u * lh << 16) + 16 * hh, yo);
+                tmem_ld_frag16(yi_at + ya + (16u * lh << 16) + 16 * hh, yo);
                 const float2 ea = *reinterpret_cast<const float2 *>(e + 16 * hh), eb = *reinterpret_cast<const float2 *>(e + 16 * hh + 8);
                 tmem_wait_ld_dep(yi);
                 tmem_wait_ld_dep(yo);
@@ -812,6 +841,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             tc_fence_before();
             warp_arrive(bar(bars.yread), lane);
             if (p.D) {
+                const float D = gates_of(c, hrow)->D;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint32_t xr[4];
@@ -852,7 +882,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
-            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
+            const int nt = tokens - c * kL < kL ? tokens - c * kL : kL;
             if (!wait.warp(bar(bars.yst[c & 1]), c >> 1, kSsmStage)) break;
             const uint32_t off = OFF_Y + (c & 1) * kTile;
             if (nt == kL) {
@@ -883,8 +913,7 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
         const int block = (row - j0) >> 3;      // the 8 of its columns that hold the row's diagonal entry
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
-            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
-            const int nt = static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
+            const int nt = tokens - c * kL;
             if (!gates_full(c)) break;
             // the tile has been read by Ya two chunks before
             if (c >= 2 &&
@@ -935,31 +964,18 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
             warp_arrive(bar(bars.mready[c & 1]), lane);
         }
     } else if ((warp >= 12 && warp < 16) || warp >= 24) {
-        // -------------------------------------------------------------- w x, hi and lo
+        // -------------------------------------------------------------- w x in three terms
         // ldmatrix.trans reads the x tile [token][row] as fragments [row][token pair], the
-        // layout of the TMEM operand's 32-bit columns.
+        // layout of the TMEM operand's 32-bit columns (and stmatrix.trans writes it back).
         const int mi = lane >> 3, r8 = lane & 7, q1 = lane & 3;
         const int p0 = static_cast<int>(lane_base) + (warp >= 24 ? 16 : 0);      // the warp's first state row
-        const uint32_t from = (p0 >> 6) * 8192 + sw128(8 * (mi >> 1) + r8, ((p0 & 63) >> 3) + (mi & 1));
+        const uint32_t x0 = sbase + OFF_STAGE + ST_X + (p0 >> 6) * 8192 + sw128(8 * (mi >> 1) + r8, ((p0 & 63) >> 3) + (mi & 1));
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
             const int st = c % kStages;
-            const int64_t t0 = s0 + static_cast<int64_t>(c) * kL;
-            const int nt = LOCAL ? kL : static_cast<int>(s1 - t0 < kL ? s1 - t0 : kL);
+            const int nt = LOCAL || tokens - c * kL > kL ? kL : tokens - c * kL;
             if (!gates_full(c)) break;
             if (!wait.warp(bar(bars.full[st]), c / kStages, kSsmTma)) break;
-            const uint32_t xs = sbase + OFF_STAGE + st * STAGE + ST_X;
-            uint32_t wh[8], wl[8];
-            {
-                const Gates *o = gates_of(c, hrow);
-#pragma unroll
-                for (int k = 0; k < 8; k += 4) {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(&o->wh[q1][k]), b = *reinterpret_cast<const uint4 *>(&o->wl[q1][k]);
-                    wh[k] = a.x; wh[k + 1] = a.y; wh[k + 2] = a.z; wh[k + 3] = a.w;
-                    wl[k] = b.x; wl[k + 1] = b.y; wl[k + 2] = b.z; wl[k + 3] = b.w;
-                }
-                if (LOCAL) warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);
-            }
             if (nt < kL) {
                 // Rows behind the last token, which may hold anything: zero in this warp's 16
                 // columns of x and of B.
@@ -973,31 +989,53 @@ ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ 
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            uint32_t x[16], hi[16], lo[16];
+            uint32_t w1[16], w2[16], w3[16];
+            const float4 *w = reinterpret_cast<const float4 *>(gates_of(c, hrow)->w[q1]);
 #pragma unroll
-            for (int gp = 0; gp < 4; ++gp)
-                ldsm_x4_t(*reinterpret_cast<uint32_t(*)[4]>(x + 4 * gp), xs + from + gp * 2048);
+            for (int gp = 0; gp < 4; ++gp) {
+                uint32_t x[4];
+                ldsm_x4_t(x, x0 + st * STAGE + gp * 2048);
+                const float4 wv = w[gp];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                hi[k] = mul_bf2(x[k], wh[k >> 1]);
-                lo[k] = fma_bf2(x[k], wl[k >> 1], fma_bf2(x[k], wh[k >> 1], hi[k] ^ 0x80008000u));
+                for (int k = 0; k < 4; ++k) {
+                    uint64_t v = mul_f2(f2(bf16_lo(x[k]), bf16_hi(x[k])), k < 2 ? f2(wv.x, wv.y) : f2(wv.z, wv.w));
+                    w1[4 * gp + k] = cut_bf2(v);
+                    w2[4 * gp + k] = cut_bf2(v);
+                    w3[4 * gp + k] = cut_bf2(v);
+                }
             }
+            if (LOCAL) warp_arrive(bar(bars.ydone[c & (kGateStages - 1)]), lane);
             // (the update of the chunk before has read the operand; all but the stores is done by then)
             if (LOCAL ? c >= 2 && !wait.warp_inline(bar(bars.g[c & 1]), (c >> 1) - 1, kSsmS)
                       : c >= 1 && !wait.warp_inline(bar(bars.s), c - 1, kSsmS)) break;
-            const uint32_t w_at = tmem_addr(tm, p0, LOCAL && (c & 1) ? TM::G : TM::W);
-            tmem_st_frag32(w_at, hi);
-            tmem_st_frag32(w_at + 32, lo);
+            const uint32_t w_at = tmem_addr(tm, p0, LOCAL ? TM::WL + (c & 1) * 96 : TM::W);
+            tmem_st_frag32(w_at, w1);
+            tmem_st_frag32(w_at + 32, w2);
+            if (LOCAL) tmem_st_frag32(w_at + 64, w3);
+            if (!LOCAL && !PAIR) {
+#pragma unroll
+                for (int gp = 0; gp < 4; ++gp)
+                    stsm_x4_t(x0 - (OFF_STAGE + ST_X) + OFF_W3 + gp * 2048, *reinterpret_cast<const uint32_t(*)[4]>(w3 + 4 * gp));
+                fence_proxy_async_smem();
+            }
             tmem_wait_st();
             tc_fence_before();
             warp_arrive(bar(bars.update[c & 1]), lane);
+            if (!LOCAL && PAIR) {
+                // the third term in the place of bf16(S), which Yi has read
+                if (!wait.warp_inline(bar(bars.cs), c, kSsmCS)) break;
+                tmem_st_frag32(tmem_addr(tm, p0, TM::W3), w3);
+                tmem_wait_st();
+                tc_fence_before();
+                warp_arrive(smem_u32(&bars.third), lane);
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (threadIdx.x < 32) {      // (from their sources again: no register is held for it through the roles)
         tc_fence_after();
-        tmem_dealloc(tm, 512);
+        tmem_dealloc(tmem_slot, 512);
     }
 }
 // ends[slot of segment j] <- the state behind segment j, for all but a sequence's last: what
