@@ -10,7 +10,7 @@
 // The token-serial prefill takes about 3 us a token where every SM has more CTAs than fit (a
 // CTA's tokens depend on each other: the row sums' shuffles and the next token's loads are its
 // latency), so it serves prompts too short for a 64-token chunk: 16 sequences x 4 tokens, 32
-// heads of 128, 25 us, and 35 in chunks.
+// heads of 128, 26 us, and 41 in chunks.
 #include "gdn_ssm_common.cuh"
 
 namespace gdn {

@@ -14,7 +14,7 @@ constexpr int64_t kMaxStride = 0x7fffffff;
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256;      // (a run behind the last row still counts in 32 bits)
 // The tensor-core scan takes a 64-token chunk of every sequence however few tokens it has, the
 // token-serial one its tokens one after the other: with 32 heads of 128, 16 sequences of 4
-// tokens 35 and 25 us, of 8 tokens 36 and 38, of 16 tokens 37 and 64.
+// tokens 41 and 26 us, of 8 tokens 42 and 39, of 16 tokens 43 and 67.
 constexpr int64_t kAutoTcMinTokens = 64;
 constexpr int64_t kAutoTcMinPerSeq = 8;
 

@@ -52,13 +52,16 @@
 // instruction caches (with everything unrolled a chunk took 7,200 cycles, two thirds of the
 // issue slots waiting for instructions).
 //
-// What bounds it.  A chunk of one head takes 2,000 to 2,300 cycles, of which the tensor pipe
-// works 1,150 and HBM less; 16 x 8192 tokens, 32 heads of 128 in 16 groups: 0.87 ms, 3.8 TB/s,
-// 375 TFLOP/s (the 512 chains are 3.5 waves of 148 CTAs, run as four).  No unit is full: every
-// product waits for a role to turn accumulators into operands, and each hand-over (TMEM load,
-// conversion, store, fence, barrier, issue) costs 400 to 700 cycles.  Pairs take 3,400: three
+// What bounds it.  A chunk of one head takes about 2,500 cycles (1.35 us alone on its SM), of which
+// the tensor pipe works 1,400 and HBM less; 16 x 8192 tokens, 32 heads of 128 in 16 groups: 1.0 ms,
+// 3.3 TB/s, 324 TFLOP/s (the 512 chains are 3.5 waves of 148 CTAs, run as four).  No unit is full:
+// every product waits for a role to turn accumulators into operands, and each hand-over (TMEM
+// load, conversion, store, fence, barrier, issue) costs 400 to 700 cycles.  Pairs take 3,800: three
 // warps form both heads' M in 2,500, and G has one buffer to wait for them.  With z a chunk of
-// one head takes 3,000: its 16 K hardware exponentials and reciprocals alone are 1,024.
+// one head takes 3,300: its 16 K hardware exponentials and reciprocals alone are 1,024.
+// What fp32 precision costs at 16 x 8192 (865 us in a graph, 735 without either): the third term's
+// products 45 us, its way through shared memory 24, cutting w x in three instead of two about 30,
+// D x in the epilogue 30.
 // Measured and not kept: a third issuing warp or 30 warps (64 registers: spills, twice the time),
 // M's scores 16 columns at a time with the diagonal block apart (4 x 2048 tokens in pairs with z,
 // 71 -> 75 us), three stages of z in place of two (16 x 2048 tokens, 283 -> 278 us with z, 205
@@ -326,9 +329,9 @@ __device__ __forceinline__ float softplus_series(float x) {
 // PAIR: two heads of 64 rows; else one head of 128.  LOCAL: the state update alone (see TcArgs),
 // from a segment's last chunk to its first: a token's weight, its decay to the segment's end, is
 // then known when it comes, so the products accumulate without a pass over the state in between
-// (0.75 us a chunk; in order, with the state decayed chunk by chunk, 0.93).  The scaled x has two
-// places; its barriers are those of G.  A pair's gates take two warps (with one,
-// 1 x 16,384 tokens in 32 chains of pairs took 222 us in place of 209).
+// (0.75 us a chunk; in order, with the state decayed chunk by chunk, 0.2 more).  The scaled x has
+// two places; its barriers are those of G.  A pair's gates take two warps (with one, 1 x 16,384
+// tokens in 32 chains of pairs took 13 us more).
 template <bool PAIR, bool LOCAL>
 __global__ void __launch_bounds__(kThreads, 1)
 ssm_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap bmap,
@@ -1123,19 +1126,19 @@ cudaError_t launch_passes(const CUtensorMap *maps, const TcArgs &a, int64_t slot
 }
 
 // Tokens of a segment, or 0 for no cuts, of a call with `chains` (sequence, slab) pairs, so that
-// few long prompts use all SMs.  A sequence of mean length takes about 1.15 us a chunk as one;
+// few long prompts use all SMs.  A sequence of mean length takes about 1.35 us a chunk as one;
 // in k segments, at most as many as fill the SMs once, a segment's chunks take 0.75 us more
 // (the local pass), and the two launches more about 14 us.  The k with the least time: 1 x
-// 16,384 tokens in 32 chains 294 us uncut and 138 in four segments, 1 x 2048 in 4 chains 67
-// and 30 in eight; 1 x 1024 in 32 chains stays whole at 28 us (36 in two).
+// 16,384 tokens in 32 chains 355 us uncut and 163 in four segments, 1 x 2048 in 4 chains 52
+// and 29 in eight; 1 x 1024 in 32 chains stays whole at 32 us (38 in two, 31 in four).
 int64_t segment_tokens(int64_t tokens, int64_t num_seqs, int64_t chains, int sms) {
     const int64_t chunks = (tokens + num_seqs * kL - 1) / (num_seqs * kL);
     const int64_t most = sms / chains < chunks / 4 ? sms / chains : chunks / 4;
     int64_t best = 0;
-    double least = 1.15 * static_cast<double>(chunks);
+    double least = 1.35 * static_cast<double>(chunks);
     for (int64_t k = 2; k <= most; ++k) {
         const int64_t part = (chunks + k - 1) / k;
-        const double time = (1.15 + 0.75) * static_cast<double>(part) + 14.0;
+        const double time = (1.35 + 0.75) * static_cast<double>(part) + 14.0;
         if (time < least) {
             least = time;
             best = part * kL;

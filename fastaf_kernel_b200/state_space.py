@@ -322,7 +322,10 @@ def ssm_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch
 
     ``method`` chooses the kernel: "tcgen05" (64-token chunks on the tensor cores, from 64
     tokens), "recurrent" (CUDA cores, one token after the other) or "auto" (what
-    ``ssm_method`` reports).
+    ``ssm_method`` reports).  State and D x are as good as fp32 sums from either; "tcgen05"
+    rounds one operand of each of y's products to bf16 (the state in S C, the scores of a
+    chunk's own tokens).  "auto" and the cutting of few long prompts go by the whole batch, so
+    a prompt may come out with other last bits in another batch.
     """
     index = _device_of("x dt A_log B C D dt_bias state z", (x, dt, A_log, B, C), (D, dt_bias, state, z))
     if x.dim() != 3:

@@ -342,9 +342,18 @@ GDN_API int gdn_conv_decode(const void *x, int64_t x_row_stride, const void *wei
  * Requirements: head_size 64 or 128, state_size 128, num_heads % num_groups == 0; x, z, B,
  * C, output, state and new_state 16-byte aligned and the row strides of x, z, B and C
  * multiples of 8.  output and new_state must overlap neither each other nor anything that the
- * call reads.  A sequence's outputs and state depend on its own rows alone.  Within a sequence,
+ * call reads.
+ *
+ * A sequence's outputs and state depend on its own rows alone, up to rounding: the kernel that
+ * GDN_PREFILL_AUTO takes and the segments that few long prompts are cut into go by the whole
+ * batch, so a sequence may come out with other last bits in another batch.  Within a sequence,
  * GDN_PREFILL_TCGEN05 lets an infinity or NaN in x, dt, B or C also reach the outputs of the
  * tokens before it in its 64-token chunk.
+ *
+ * Precision: the state and D x are as good as fp32 sums in every kernel; so is y before it is
+ * rounded, with GDN_PREFILL_RECURRENT.  GDN_PREFILL_TCGEN05 rounds one operand of each of y's two
+ * products to bf16, the state in S C and the scores (C . B) decay dt' of a chunk's own tokens:
+ * 2^-8 of S C's and the scores' terms at most.
  */
 GDN_API int gdn_ssm_prefill(const void *x, int64_t x_row_stride, const void *dt, int64_t dt_row_stride,
                     const void *A_log, const void *B, int64_t B_row_stride, const void *C, int64_t C_row_stride,
