@@ -85,13 +85,21 @@ cudaError_t pool_alloc(void **ptr, size_t bytes, cudaStream_t stream) {
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;
             props.location.id = dev;
+            // (not a stream's work, but refused to a thread whose capture mode is not relaxed: the
+            // first call may be a captured one)
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            e = cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return e;
             e = cudaMemPoolCreate(&pools[dev], &props);
+            if (e == cudaSuccess) {
+                uint64_t keep = ~uint64_t(0);
+                cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
+            }
+            cudaThreadExchangeStreamCaptureMode(&mode);
             if (e != cudaSuccess) {
                 pools[dev] = nullptr;
                 return e;
             }
-            uint64_t keep = ~uint64_t(0);
-            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
         }
         pool = pools[dev];
     }
